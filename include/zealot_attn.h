@@ -125,6 +125,69 @@ zl_status zl_reshape_and_cache(zl_ctx* ctx, const void* k /*device*/, const void
                                int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
                                zl_dtype dtype, zl_stream stream);
 
+/* ------------------------------------------------------------- step tables */
+
+/* Block tables, slot mapping, positions and row offsets of one step, built on
+ * the device from the requests' lengths. The reference builds them on the host
+ * (src/cuda_runner.rs:446, src/kv_cache.rs:107-161). Request i adds
+ * query_lens[i] tokens to context_lens[i] cached ones; its table is row
+ * rows[i] (rows NULL: row i) of seq_blocks [num_rows][max_blocks_per_seq], the
+ * caller's persistent tables. The blocks that its new tokens open are taken
+ * from new_blocks in request order, ceil((c+q)/bs) - ceil(c/bs) for each
+ * request, and are written into seq_blocks as well.
+ * Outputs: block_tables [num_seqs][max_blocks_per_seq] (-1 after each request's
+ * last block), cu_seqlens [num_seqs+1] (first token row of each request),
+ * seq_lens [num_seqs] (c + q), positions and slot_mapping [num_tokens] (token
+ * rows at and after cu_seqlens[num_seqs], the padding of a fixed-size step, get
+ * position 0 and slot -1) and last_rows [num_seqs] (the request's last token
+ * row; a request without tokens gets the row before, at least 0).
+ * rows[i] < 0 makes request i an empty slot: its token rows are counted, with
+ * slot -1, and its length is 0. So is, with ZL_ERR_OOB_BLOCK in the status
+ * word, a request that cannot be served: negative lengths, a row outside
+ * seq_blocks or listed more than once, more blocks than a table row has, or
+ * token rows beyond num_tokens; the new blocks that its lengths ask for are
+ * passed over, so that the other requests keep theirs. An id outside the pool
+ * (or one that new_blocks does not have) becomes -1, with slot -1, and is
+ * reported too. seq_blocks entries that open no new block are left as they were.
+ * At most 8192 requests and, with rows, 262144 table rows: ZL_ERR_UNSUPPORTED. */
+zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks /*device*/, int num_rows,
+                         const int32_t* rows /*device*/, const int32_t* context_lens /*device*/,
+                         const int32_t* query_lens /*device*/, const int32_t* new_blocks /*device*/,
+                         int64_t num_new, int32_t* block_tables /*device*/, int32_t* cu_seqlens /*device*/,
+                         int32_t* seq_lens /*device*/, int32_t* positions /*device*/,
+                         int64_t* slot_mapping /*device*/, int32_t* last_rows /*device*/, int num_seqs,
+                         int64_t num_tokens, int max_blocks_per_seq, int block_size, int64_t num_blocks,
+                         zl_stream stream);
+
+/* ------------------------------- query and key norm, rotation, cache write */
+
+/* One pass over a projection's output: RMS norm of every query and key head
+ * over head_dim (x / sqrt(mean(x^2) + eps) * weight; a NULL weight leaves that
+ * side as it is), rotation of its first rotary_dim elements by the angle
+ * positions[t] * inv_freq[i], taken in 64 bits, and the stores. Pair i is
+ * elements (i, i + rotary_dim/2), or (2i, 2i+1) with interleaved != 0;
+ * inv_freq is device double [rotary_dim/2], the weights are [head_dim] in
+ * `dtype`. No reference counterpart (its runner has no rotary embedding).
+ * q, k and v are rows of num_heads / num_kv_heads heads with q_stride,
+ * k_stride and v_stride elements from token to token (the three parts of one
+ * projection's row, or packed rows of their own). Outputs, each optional:
+ * q_out [T][H][d], k_out and v_out [T][Hkv][d] packed (what zl_prefill_varlen
+ * takes), and k_pool / v_pool, both or neither, at slot_mapping[t] as
+ * zl_reshape_and_cache writes them: slot < 0 skips the token's write, slot >=
+ * num_blocks * block_size is reported and skipped, and slots are distinct.
+ * Values are copied bit for bit; the rest is computed in fp32 and rounded once.
+ * An output may be its own input where that is packed; otherwise outputs do
+ * not overlap inputs. head_dim up to 256 (larger: ZL_ERR_UNSUPPORTED). */
+zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q /*device*/, const void* k /*device*/,
+                          const void* v /*device*/, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                          const void* q_weight /*device*/, const void* k_weight /*device*/, float eps,
+                          const int32_t* positions /*device*/, const double* inv_freq /*device*/,
+                          int rotary_dim, int interleaved, void* q_out /*device*/, void* k_out /*device*/,
+                          void* v_out /*device*/, void* k_pool /*device*/, void* v_pool /*device*/,
+                          const int64_t* slot_mapping /*device*/, int block_size, int64_t num_blocks,
+                          int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                          zl_dtype dtype, zl_stream stream);
+
 /* ------------------------------------------------------------ paged decode */
 
 /* Replaces CudaAttention::paged_forward (src/attention/cuda.rs:126-210) and
@@ -191,6 +254,65 @@ zl_status zl_paged_decode_partial(zl_ctx* ctx, const void* q, const void* k_pool
 zl_status zl_merge_partials(zl_ctx* ctx, const float* m, const float* l, const float* o,
                             int num_parts, int64_t rows, int head_dim, void* out, zl_dtype dtype,
                             zl_stream stream);
+
+/* ------------------------------------------- decode over selected blocks */
+
+/* Attention of one token per sequence over some of its blocks, in four calls:
+ * zl_block_bounds after keys are written, then per step zl_block_scores,
+ * zl_select_blocks and zl_paged_decode_selected. No reference counterpart.
+ * Tables, lengths, pools and the head mapping are those of zl_paged_decode; a
+ * negative table entry is a block that is not there (it does not end the
+ * sequence). Several tokens of one sequence are served as several rows with
+ * the same table and their own lengths. */
+
+/* Bounds of the keys of every block that holds a token in [tok_begin[b],
+ * seq_lens[b]) (tok_begin NULL: from 0): bounds [num_blocks][Hkv][2][d] in
+ * `dtype`, the elementwise minimum and maximum over the block's tokens below
+ * seq_lens[b]. After a decode step tok_begin is the length before it. A block
+ * shared by sequences is shared whole. NaN keys give NaN bounds. */
+zl_status zl_block_bounds(zl_ctx* ctx, const void* k_pool /*device*/, const int32_t* block_tables /*device*/,
+                          const int32_t* tok_begin /*device*/, const int32_t* seq_lens /*device*/,
+                          void* bounds /*device*/, int num_seqs, int num_kv_heads, int head_dim,
+                          int block_size, int max_blocks_per_seq, int64_t num_blocks, zl_dtype dtype,
+                          zl_stream stream);
+
+/* scores [B][Hkv][max_blocks_per_seq] fp32: for block j of sequence b the
+ * largest, over the query heads of the kv head, of
+ *   scale * sum_i max(q_i, 0) * hi_i + min(q_i, 0) * lo_i,
+ * which no attention score in the block exceeds (scale <= 0: 1/sqrt(d)).
+ * -inf after the sequence's last block and for blocks that are not there. */
+zl_status zl_block_scores(zl_ctx* ctx, const void* q /*device*/, const void* bounds /*device*/,
+                          const int32_t* block_tables /*device*/, const int32_t* seq_lens /*device*/,
+                          float* scores /*device*/, int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                          int block_size, int max_blocks_per_seq, int64_t num_blocks, float scale,
+                          zl_gqa_map gqa_map, zl_dtype dtype, zl_stream stream);
+
+/* selected [B][Hkv][max_selected]: of the ceil(seq_lens[b]/block_size) blocks
+ * of each sequence the first num_first, the last num_last and the best of the
+ * others by score, max_selected in all, as ascending block indices; all blocks,
+ * then -1, where there are not more than that. Equal scores go to the lower
+ * index, -0 equals +0 and NaN ranks above every score. num_first + num_last <=
+ * max_selected. */
+zl_status zl_select_blocks(zl_ctx* ctx, const float* scores /*device*/, const int32_t* seq_lens /*device*/,
+                           int32_t* selected /*device*/, int num_seqs, int num_kv_heads, int block_size,
+                           int max_blocks_per_seq, int max_selected, int num_first, int num_last,
+                           zl_stream stream);
+
+/* Paged decode over the tokens of the blocks that selected [B][Hkv][max_selected]
+ * lists for each (sequence, kv head): indices into the sequence's table row, in
+ * any order, a negative one ending the list. Tokens at or after seq_lens[b] are
+ * masked; an index listed twice counts twice; an index outside the table row or
+ * a block id outside the pool is reported and skipped. A row without tokens is
+ * zeros. q and out [B][H][d]; any block_size; head_dim up to 256 (larger:
+ * ZL_ERR_UNSUPPORTED). Takes no workspace: calls on different streams do not
+ * disturb one another. */
+zl_status zl_paged_decode_selected(zl_ctx* ctx, const void* q /*device*/, const void* k_pool /*device*/,
+                                   const void* v_pool /*device*/, const int32_t* block_tables /*device*/,
+                                   const int32_t* seq_lens /*device*/, const int32_t* selected /*device*/,
+                                   void* out /*device*/, int num_seqs, int num_heads, int num_kv_heads,
+                                   int head_dim, int block_size, int max_blocks_per_seq, int64_t num_blocks,
+                                   int max_selected, float scale, zl_gqa_map gqa_map, zl_dtype dtype,
+                                   zl_stream stream);
 
 /* ---------------------------------------------------------- varlen prefill */
 

@@ -1,0 +1,146 @@
+"""The serving-step operators in a row, as a decode loop uses them: tables from lengths,
+norm + rotation + cache write, block bounds, scores, selection and attention over the
+selected blocks, eagerly and as one replayed CUDA graph."""
+import numpy as np
+import pytest
+
+import test_gpu_block_select as blocks
+import test_gpu_rope as rope
+import test_gpu_selected_decode as selected
+import test_gpu_step_tables as tables
+
+pytestmark = pytest.mark.gpu
+
+H, HKV, D, BS, MB, NB, TOP, B = 8, 2, 64, 16, 12, 80, 5, 3
+
+
+class Loop:
+    """Three sequences in the rows of a persistent table, with everything on the device."""
+
+    def __init__(self, ctx, seed):
+        import torch
+        import zealot_b200 as zb
+        self.ctx, self.attn, self.rng = ctx, zb.CudaAttention(ctx), np.random.default_rng(seed)
+        i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+        bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")
+        self.seq_blocks = torch.full((6, MB), -1, dtype=torch.int32, device="cuda")
+        self.rows = torch.tensor([4, 0, 2], dtype=torch.int32, device="cuda")
+        self.ctx_lens, self.q_lens, self.new = i32(B), i32(B), torch.full((16,), -1, dtype=torch.int32, device="cuda")
+        self.k_pool, self.v_pool, self.bounds = bf(NB, HKV, BS, D), bf(NB, HKV, BS, D), bf(NB, HKV, 2, D)
+        self.freq = torch.from_numpy(rope.freqs(D)).cuda()
+        self.weights = [bf(D).add_(1.0), bf(D).add_(0.5)]
+        self.free = list(self.rng.permutation(NB))
+        self.out = dict(block_tables=i32(B, MB), cu_seqlens=i32(B + 1), seq_lens=i32(B), last_rows=i32(B))
+        self.scores = torch.zeros((B, HKV, MB), device="cuda")
+        self.sel, self.q_out, self.o = i32(B, HKV, TOP), bf(B, H, D), bf(B, H, D)
+        self.decode_qkv = bf(B, (H + 2 * HKV) * D)
+        self.decode_pos, self.decode_slots = i32(B), torch.zeros(B, dtype=torch.int64, device="cuda")
+
+    def set_step(self, context, query):
+        """Uploads a step's lengths and the ids of the blocks that it opens."""
+        import torch
+        need = sum(-(-(c + q) // BS) - -(-c // BS) for c, q in zip(context, query))
+        new = np.full(16, -1, np.int32)
+        new[:need] = [self.free.pop() for _ in range(need)]
+        self.new.copy_(torch.from_numpy(new))
+        self.ctx_lens.copy_(torch.tensor(context, dtype=torch.int32))
+        self.q_lens.copy_(torch.tensor(query, dtype=torch.int32))
+        return new
+
+    def write(self, qkv, pos, slots, q_out):
+        t = qkv.shape[0]
+        q, k, v = (x.reshape(t, -1, D) for x in qkv.split((H * D, HKV * D, HKV * D), dim=1))
+        self.attn.step_tables(self.seq_blocks, self.rows, self.ctx_lens, self.q_lens, self.new, self.out["block_tables"],
+                              self.out["cu_seqlens"], self.out["seq_lens"], pos, slots, self.out["last_rows"], BS, NB)
+        self.attn.qk_norm_rope(q, k, v, pos, self.freq, q_out=q_out, q_weight=self.weights[0], k_weight=self.weights[1],
+                               k_pool=self.k_pool, v_pool=self.v_pool, slot_mapping=slots)
+        self.attn.block_bounds(self.k_pool, self.out["block_tables"], self.out["seq_lens"], self.bounds,
+                               tok_begin=self.ctx_lens)
+
+    def decode(self):
+        self.write(self.decode_qkv, self.decode_pos, self.decode_slots, self.q_out)
+        t, n = self.out["block_tables"], self.out["seq_lens"]
+        self.attn.block_scores(self.q_out, self.bounds, t, n, self.scores, BS)
+        self.attn.select_blocks(self.scores, n, self.sel, BS, num_first=1, num_last=1)
+        self.attn.paged_forward_selected(self.q_out, self.k_pool, self.v_pool, t, n, self.sel, self.o)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_decode_loop(ctx, graph):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(11)
+    loop = Loop(ctx, 5)
+    keys = [np.zeros((0, HKV, D)) for _ in range(B)]  # what each sequence's cache should hold, in 64 bits
+    vals = [np.zeros((0, HKV, D)) for _ in range(B)]
+    lens = [0, 0, 0]
+
+    def expect(qkv, query):
+        """Appends a step's keys and values from the formula; returns the queries."""
+        x = qkv.float().cpu().numpy().reshape(len(qkv), -1, D)
+        pos = np.concatenate([np.arange(c, c + n) for c, n in zip(lens, query)])
+        w = [t.float().cpu().numpy() for t in loop.weights]
+        q, _ = rope.formula(x[:, :H], w[0], 1e-6, pos, rope.freqs(D), False)
+        k, _ = rope.formula(x[:, H:H + HKV], w[1], 1e-6, pos, rope.freqs(D), False)
+        at = 0
+        for b in range(B):
+            keys[b] = np.concatenate([keys[b], k[at:at + query[b]]])
+            vals[b] = np.concatenate([vals[b], x[at:at + query[b], H + HKV:]])
+            at += query[b]
+            lens[b] += query[b]
+        return q
+
+    # prompts of 100, 1 and 47 tokens, with two padding rows
+    query = [100, 1, 47]
+    qkv = torch.randn((150, (H + 2 * HKV) * D), generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.zeros(150, dtype=torch.int32, device="cuda")
+    slots = torch.zeros(150, dtype=torch.int64, device="cuda")
+    loop.set_step(lens, query)
+    loop.write(qkv, pos, slots, torch.empty((150, H, D), dtype=torch.bfloat16, device="cuda"))
+    expect(qkv[:148], query)
+    ctx.check_status()
+
+    run = loop.decode
+    if graph:
+        # capture on lengths of no tokens, so that the warm-up leaves the state as it is
+        loop.q_lens.zero_(), loop.ctx_lens.zero_()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            loop.decode()
+        torch.cuda.current_stream().wait_stream(stream)
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured):
+            loop.decode()
+        run = captured.replay
+    for step in range(20):
+        qkv = torch.randn((B, (H + 2 * HKV) * D), generator=g, device="cuda").to(torch.bfloat16)
+        loop.decode_qkv.copy_(qkv)
+        loop.set_step(lens, [1, 1, 1])
+        run()
+        q = expect(qkv, [1, 1, 1])
+        ctx.check_status()
+        t = loop.out["block_tables"].cpu().numpy()
+        assert loop.out["seq_lens"].tolist() == lens
+        assert loop.decode_pos.tolist() == [n - 1 for n in lens]
+        # queries and cache: within their rounding to bf16 (and fp32 work, far below it)
+        assert np.allclose(loop.q_out.double().cpu().numpy(), q, rtol=2.0 ** -8, atol=1e-4)
+        kp, vp = loop.k_pool.double().cpu().numpy(), loop.v_pool.double().cpu().numpy()
+        for b in range(B):
+            rows = t[b, np.arange(lens[b]) // BS], np.arange(lens[b]) % BS
+            assert np.allclose(kp[rows[0], :, rows[1]], keys[b], rtol=2.0 ** -8, atol=1e-4)
+            assert np.array_equal(vp[rows[0], :, rows[1]], vals[b])
+        # each later stage against what it was given
+        bounds = blocks.plain_bounds(loop.k_pool, t, lens, None, loop.bounds, BS)
+        for b in range(B):
+            ids = t[b, :-(-lens[b] // BS)]
+            assert np.array_equal(loop.bounds.float().cpu().numpy()[ids], bounds[ids])
+        want, tol = blocks.plain_scores(loop.q_out, loop.bounds, t, lens, HKV, BS, D ** -0.5, False)
+        got = loop.scores.double().cpu().numpy()
+        assert np.array_equal(np.isinf(got), np.isinf(want)) and np.all(np.abs(got - want)[np.isfinite(want)]
+                                                                      <= tol[np.isfinite(want)])
+        sel = loop.sel.cpu().numpy()
+        assert np.array_equal(sel, blocks.plain_select(loop.scores.cpu().numpy(), lens, BS, TOP, 1, 1))
+        want, tol = selected.plain(loop.q_out.double().cpu().numpy(), kp, vp, t, lens, sel, D ** -0.5, False, True)
+        assert np.all(np.abs(loop.o.double().cpu().numpy() - want) <= tol)
+    if graph:
+        del captured

@@ -8,6 +8,7 @@
 // the chunk max and sum, and the threads that own output dims accumulate
 // p*v with an online rescale. fp32 accumulation throughout.
 #include "zl_internal.h"
+#include "zl_pages.h"
 
 #include <cfloat>
 
@@ -169,6 +170,54 @@ decode_generic_kernel(const T* __restrict__ q, const T* __restrict__ k_pool,
   }
 }
 
+// -------------------------------------------- decode over selected blocks
+
+// Keys are the tokens of the blocks that `selected` lists for (b, kv head), in
+// its order; a negative entry ends the list. Tokens at or after seq_lens[b] and
+// blocks without a table entry are masked.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+decode_selected_generic_kernel(const T* __restrict__ q, const T* __restrict__ k_pool,
+                               const T* __restrict__ v_pool, const int32_t* __restrict__ block_tables,
+                               const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ selected,
+                               T* __restrict__ out, int H, int Hkv, int d, int bs, int max_blocks,
+                               int max_selected, int64_t num_blocks, float scale, int gqa_modulo, int* status) {
+  __shared__ AttendShared sh;
+  const int b = blockIdx.x / H;
+  const int h = blockIdx.x - b * H;
+  const int tid = threadIdx.x;
+  const int kvh = gqa_modulo ? h % Hkv : h / (H / Hkv);
+  const int64_t qoff = ((int64_t)b * H + h) * d;
+  for (int e = tid; e < d; e += kThreads) sh.q[e] = to_f(q[qoff + e]);
+  if (tid == 0) sh.first_neg = max_selected;
+  __syncthreads();
+  const int64_t len = seq_lens[b];
+  const int32_t* table = block_tables + (int64_t)b * max_blocks;
+  const int32_t* list = selected + ((int64_t)b * Hkv + kvh) * max_selected;
+  for (int i = tid; i < max_selected; i += kThreads)
+    if (list[i] < 0) atomicMin(&sh.first_neg, i);
+  __syncthreads();
+  auto row_of = [&](int64_t j) -> int64_t {
+    const int64_t i = j / bs, t = j - i * bs, blk = list[i];
+    if (blk >= max_blocks) {
+      atomicOr(status, ZL_DEV_OOB);
+      return -1;
+    }
+    if (blk * bs + t >= len) return -1;
+    const int64_t id = table[blk];
+    if (id >= num_blocks) atomicOr(status, ZL_DEV_OOB);
+    const int64_t row = zl::pool_row(id, num_blocks, Hkv, kvh, bs, (int)t);
+    return row < 0 ? -1 : row * d;
+  };
+  float m, l, acc[2];
+  attend<T>(k_pool, v_pool, d, scale, 0, (int64_t)sh.first_neg * bs, row_of, sh, m, l, acc);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  for (int r = 0; r < 2; r++) {
+    const int e = tid + r * kThreads;
+    if (e < d) out[qoff + e] = from_f<T>(acc[r] * inv);
+  }
+}
+
 // ----------------------------------------------------------------- prefill
 
 template <typename T>
@@ -260,6 +309,26 @@ zl_status launch_decode_generic(zl_ctx* ctx, const void* q, const void* k_pool, 
         (const __nv_bfloat16*)q, (const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool,
         block_tables, seq_lens, tok_begin, (__nv_bfloat16*)out, m_out, l_out, o_out, H, Hkv, d, bs,
         max_blocks, num_blocks, scale, mod, ctx->d_status);
+  ZL_LAUNCH_CHECK(ctx);
+  return ZL_OK;
+}
+
+zl_status launch_decode_selected_generic(zl_ctx* ctx, const void* q, const void* k_pool, const void* v_pool,
+                                         const int32_t* block_tables, const int32_t* seq_lens,
+                                         const int32_t* selected, void* out, int B, int H, int Hkv, int d, int bs,
+                                         int max_blocks, int64_t num_blocks, int max_selected, float scale,
+                                         zl_gqa_map map, zl_dtype dtype, cudaStream_t st) {
+  const int64_t grid = (int64_t)B * H;
+  const int mod = map == ZL_GQA_MODULO;
+  if (dtype == ZL_F32)
+    decode_selected_generic_kernel<float><<<(unsigned)grid, kThreads, 0, st>>>(
+        (const float*)q, (const float*)k_pool, (const float*)v_pool, block_tables, seq_lens, selected, (float*)out,
+        H, Hkv, d, bs, max_blocks, max_selected, num_blocks, scale, mod, ctx->d_status);
+  else
+    decode_selected_generic_kernel<__nv_bfloat16><<<(unsigned)grid, kThreads, 0, st>>>(
+        (const __nv_bfloat16*)q, (const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool, block_tables, seq_lens,
+        selected, (__nv_bfloat16*)out, H, Hkv, d, bs, max_blocks, max_selected, num_blocks, scale, mod,
+        ctx->d_status);
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }

@@ -103,6 +103,31 @@ zl_status zl_paged_decode_partial(zl_ctx* ctx, const void* q, const void* k_pool
                                gqa_map, dtype, S(stream));
 }
 
+zl_status zl_paged_decode_selected(zl_ctx* ctx, const void* q, const void* k_pool, const void* v_pool,
+                                   const int32_t* block_tables, const int32_t* seq_lens, const int32_t* selected,
+                                   void* out, int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                   int block_size, int max_blocks_per_seq, int64_t num_blocks, int max_selected,
+                                   float scale, zl_gqa_map gqa_map, zl_dtype dtype, zl_stream stream) {
+  zl_status s;
+  if (!dtype_ok(dtype)) return set_error(ZL_ERR_INVALID_ARG, "paged_decode_selected: bad dtype");
+  if ((s = check_heads(num_heads, num_kv_heads, head_dim, "paged_decode_selected")) != ZL_OK) return s;
+  if (head_dim > 256)
+    return set_error(ZL_ERR_UNSUPPORTED, "paged_decode_selected: head_dim %d > 256", head_dim);
+  if (num_seqs < 0 || block_size <= 0 || max_blocks_per_seq < 0 || num_blocks < 0 || max_selected < 0)
+    return set_error(ZL_ERR_INVALID_ARG, "paged_decode_selected: bad sizes B=%d bs=%d max_blocks=%d max_selected=%d",
+                     num_seqs, block_size, max_blocks_per_seq, max_selected);
+  if (num_seqs == 0) return ZL_OK;
+  if ((int64_t)num_seqs * num_heads > INT32_MAX)
+    return set_error(ZL_ERR_INVALID_ARG, "paged_decode_selected: B*H too large");
+  if (!q || !out || !seq_lens || (max_selected && (!selected || !k_pool || !v_pool || !block_tables)))
+    return set_error(ZL_ERR_INVALID_ARG, "paged_decode_selected: null pointer");
+  DeviceScope dev(ctx);
+  if (dev.status != ZL_OK) return dev.status;
+  return launch_decode_selected_generic(ctx, q, k_pool, v_pool, block_tables, seq_lens, selected, out, num_seqs,
+                                        num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks,
+                                        max_selected, resolve_scale(scale, head_dim), gqa_map, dtype, S(stream));
+}
+
 zl_status zl_merge_partials(zl_ctx* ctx, const float* m, const float* l, const float* o,
                             int num_parts, int64_t rows, int head_dim, void* out, zl_dtype dtype,
                             zl_stream stream) {

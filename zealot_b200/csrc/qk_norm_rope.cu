@@ -1,0 +1,166 @@
+// qk_norm_rope.cu -- RMS norm of every query and key head, rotation by the
+// token's position and the write of keys and values into the paged pools, in
+// one pass over a projection's output.
+//
+// For a head x of a token at position p, with weight w and frequencies f:
+//   y = x / sqrt(mean(x^2) + eps) * w              (without w: y = x)
+//   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = p f_i
+// for the pairs i < rotary_dim / 2, which are elements (i, i + rotary_dim / 2)
+// or, interleaved, (2i, 2i + 1). Elements from rotary_dim on are not turned.
+// Keys go to the slot of kv_cache.rs:245-247 (reshape_and_cache.cu) and, where
+// asked for, into packed rows for zl_prefill_varlen; values are copied.
+//
+// Everything is kept in fp32 and rounded once, at the store. The angle is
+// p f_i in 64 bits, taken off its whole turns in 64 bits too (Cody and Waite's
+// reduction with 2 pi in two parts): at p = 10^6 the product in fp32 would be
+// off by 0.06 radians.
+#include "zl_internal.h"
+#include "zl_pages.h"
+
+namespace {
+
+constexpr int kMaxDim = 256;
+
+struct RopeArgs {
+  const void *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  const void *q_weight, *k_weight;
+  float eps;
+  const int32_t* positions;
+  const double* inv_freq;
+  int rot, interleaved;
+  void *q_out, *k_out, *v_out, *k_pool, *v_pool;
+  const int64_t* slots;
+  int bs;
+  int64_t num_blocks, tokens;
+  int H, Hkv, d;
+  int* status;
+};
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void put(float* p, float x) { *p = x; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+// cos and sin of position * frequency.
+__device__ __forceinline__ float2 turn(int32_t pos, double freq) {
+  const double a = (double)pos * freq;
+  const double k = rint(a * 0.15915494309189533577);
+  double r = fma(-k, 6.283185307179586232, a);
+  r = fma(-k, 2.449293598294706539e-16, r);
+  float s, c;
+  sincosf((float)r, &s, &c);
+  return make_float2(c, s);
+}
+
+// Row of the pools that token t's kv head h is written to, -1 for none.
+__device__ __forceinline__ int64_t cache_row(const RopeArgs& g, int64_t t, int h) {
+  if (!g.slots) return -1;
+  const int64_t slot = g.slots[t];
+  if (slot < 0) return -1;
+  const int64_t blk = slot / g.bs;
+  if (blk >= g.num_blocks) {
+    atomicOr(g.status, ZL_DEV_OOB);
+    return -1;
+  }
+  return zl::pool_row(blk, g.num_blocks, g.Hkv, h, g.bs, (int)(slot - blk * g.bs));
+}
+
+// Any head_dim up to 256, any alignment: one warp per (token, head), the row in
+// the warp's shared memory so that a pair's elements meet.
+template <typename T>
+__global__ void __launch_bounds__(256) rope_elem_kernel(RopeArgs g) {
+  __shared__ float rows[8][kMaxDim];
+  const int lane = threadIdx.x & 31;
+  float* x = rows[threadIdx.x >> 5];
+  const int heads = g.H + 2 * g.Hkv;
+  const int64_t warps = (int64_t)gridDim.x * 8;
+  for (int64_t u = blockIdx.x * 8ll + (threadIdx.x >> 5); u < g.tokens * heads; u += warps) {
+    const int64_t t = u / heads;
+    const int h = (int)(u - t * heads);
+    const bool isq = h < g.H, isk = !isq && h < g.H + g.Hkv;
+    const int hh = isq ? h : isk ? h - g.H : h - g.H - g.Hkv;
+    const T* src = (const T*)(isq ? g.q : isk ? g.k : g.v);
+    T* out = (T*)(isq ? g.q_out : isk ? g.k_out : g.v_out);
+    T* pool = (T*)(isq ? nullptr : isk ? g.k_pool : g.v_pool);
+    if (!out && !pool) continue;
+    src += t * (isq ? g.q_stride : isk ? g.k_stride : g.v_stride) + (int64_t)hh * g.d;
+    float ss = 0.f;
+    __syncwarp();
+    for (int e = lane; e < g.d; e += 32) {
+      const float f = to_f(src[e]);
+      x[e] = f;
+      ss = fmaf(f, f, ss);
+    }
+    const T* w = (const T*)(isq ? g.q_weight : isk ? g.k_weight : nullptr);
+    if (w) {
+      for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float inv = 1.f / sqrtf(ss / g.d + g.eps);
+      for (int e = lane; e < g.d; e += 32) x[e] = x[e] * inv * to_f(w[e]);
+    }
+    __syncwarp();
+    if (isq || isk) {
+      for (int i = lane; i < g.rot / 2; i += 32) {
+        const float2 cs = turn(g.positions[t], g.inv_freq[i]);
+        const int ia = g.interleaved ? 2 * i : i, ib = g.interleaved ? 2 * i + 1 : i + g.rot / 2;
+        const float a = x[ia], b = x[ib];
+        x[ia] = a * cs.x - b * cs.y;
+        x[ib] = b * cs.x + a * cs.y;
+      }
+    }
+    __syncwarp();
+    if (out) {
+      out += (t * (isq ? g.H : g.Hkv) + hh) * (int64_t)g.d;
+      for (int e = lane; e < g.d; e += 32) put(out + e, x[e]);
+    }
+    if (pool) {
+      const int64_t row = cache_row(g, t, hh);
+      if (row >= 0)
+        for (int e = lane; e < g.d; e += 32) put(pool + row * g.d + e, x[e]);
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, const void* v, int64_t q_stride,
+                                     int64_t k_stride, int64_t v_stride, const void* q_weight, const void* k_weight,
+                                     float eps, const int32_t* positions, const double* inv_freq, int rotary_dim,
+                                     int interleaved, void* q_out, void* k_out, void* v_out, void* k_pool,
+                                     void* v_pool, const int64_t* slot_mapping, int block_size, int64_t num_blocks,
+                                     int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                                     zl_dtype dtype, zl_stream stream) {
+  using namespace zl;
+  if (!dtype_ok(dtype)) return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: bad dtype %d", (int)dtype);
+  if (num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0)
+    return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: bad sizes T=%lld H=%d Hkv=%d d=%d", (long long)num_tokens,
+                     num_heads, num_kv_heads, head_dim);
+  if (head_dim > kMaxDim) return set_error(ZL_ERR_UNSUPPORTED, "qk_norm_rope: head_dim %d > %d", head_dim, kMaxDim);
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2)
+    return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: rotary_dim %d of head_dim %d", rotary_dim, head_dim);
+  if (!k_pool != !v_pool || (k_pool && (!slot_mapping || block_size <= 0 || num_blocks < 0)))
+    return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: both pools with slots, block_size and num_blocks, or neither");
+  if (num_tokens == 0) return ZL_OK;
+  const bool need_k = k_out || k_pool, need_v = v_out || v_pool;
+  if ((!q_out && !need_k && !need_v) || (q_out && !q) || (need_k && !k) || (need_v && !v) ||
+      (rotary_dim && (q_out || need_k) && (!positions || !inv_freq)))
+    return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: null pointer");
+  const int64_t nq = (int64_t)num_heads * head_dim, nk = (int64_t)num_kv_heads * head_dim;
+  if (num_tokens > 1 && ((q_out && q_stride < nq) || (need_k && k_stride < nk) || (need_v && v_stride < nk)))
+    return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: a token stride is below its row");
+  if ((q_out == q && q_stride != nq && num_tokens > 1) || (k_out && k_out == k && k_stride != nk && num_tokens > 1) ||
+      (v_out && v_out == v && v_stride != nk && num_tokens > 1))
+    return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: in place only on packed rows");
+  DeviceScope dev(ctx);
+  if (dev.status != ZL_OK) return dev.status;
+  RopeArgs g{q, k, v, q_stride, k_stride, v_stride, q_weight, k_weight, eps, positions, inv_freq, rotary_dim,
+             interleaved, q_out, k_out, v_out, k_pool, v_pool, k_pool ? slot_mapping : nullptr, block_size,
+             num_blocks, num_tokens, num_heads, num_kv_heads, head_dim, ctx->d_status};
+  const int64_t units = num_tokens * (num_heads + 2 * (int64_t)num_kv_heads);
+  int64_t blocks = (units + 7) / 8;
+  if (blocks > (int64_t)ctx->num_sms * 32) blocks = (int64_t)ctx->num_sms * 32;
+  if (dtype == ZL_F32) rope_elem_kernel<float><<<(unsigned)blocks, 256, 0, S(stream)>>>(g);
+  else rope_elem_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, S(stream)>>>(g);
+  ZL_LAUNCH_CHECK(ctx);
+  return ZL_OK;
+}

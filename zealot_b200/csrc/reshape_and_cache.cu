@@ -68,8 +68,6 @@ reshape_and_cache_elem(const T* __restrict__ k, const T* __restrict__ v, T* __re
   }
 }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 }  // namespace
 
 extern "C" zl_status zl_reshape_and_cache(zl_ctx* ctx, const void* k, const void* v, void* k_pool,

@@ -1,0 +1,226 @@
+// step_tables.cu -- the metadata of one serving step, built on the device from
+// the requests' lengths.
+//
+// The reference builds it on the host, one sequence at a time
+// (src/cuda_runner.rs:446, src/kv_cache.rs:107-161); zl_decode_graph advances
+// one token of a fixed set of rows. Here request i adds q_i tokens to c_i
+// cached ones. With had = ceil(c/bs) and has = ceil((c+q)/bs) it opens
+// has - had new blocks, taken from the list of new block ids in request order:
+// two exclusive sums, of q_i (the packed token rows) and of has - had (where a
+// request's new ids start), give everything else by indexing.
+//
+// One launch and no communication between CTAs: every CTA takes both sums over
+// all requests itself (a few numbers per thread, from L2), then its share of
+// the table entries and of the token rows. No CTA reads what another writes:
+// entries below `had` are only read, entries from `had` on are taken from the
+// list of new ids.
+#include "zl_internal.h"
+#include "zl_pages.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxSeqs = 8192;      // requests of one step: 12 bytes of shared memory each
+constexpr int kMaxRows = 1 << 18;   // rows of the persistent table: 2 bits of shared memory each
+
+struct StepArgs {
+  int32_t* seq_blocks;
+  const int32_t* rows;
+  const int32_t* context_lens;
+  const int32_t* query_lens;
+  const int32_t* new_blocks;
+  int32_t* block_tables;
+  int32_t* cu_seqlens;
+  int32_t* seq_lens;
+  int32_t* positions;
+  int64_t* slot_mapping;
+  int32_t* last_rows;
+  int64_t num_new, num_tokens, num_blocks;
+  int num_rows, num_seqs, max_blocks, bs;
+  int* status;
+};
+
+// Exclusive sums of a[0..n) and b[0..n) in place, total of a returned in a[n].
+__device__ void scan2(int32_t* a, int32_t* b, int n) {
+  __shared__ int32_t wa[kThreads / 32], wb[kThreads / 32];
+  const int per = (n + kThreads - 1) / kThreads, lo = min(n, (int)threadIdx.x * per), hi = min(n, lo + per);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int32_t sa = 0, sb = 0;
+  for (int i = lo; i < hi; i++) {
+    sa = zl::sat_add(sa, a[i]);
+    sb = zl::sat_add(sb, b[i]);
+  }
+  int32_t ia = sa, ib = sb;  // inclusive over the warp
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t ua = __shfl_up_sync(0xffffffffu, ia, o), ub = __shfl_up_sync(0xffffffffu, ib, o);
+    if (lane >= o) {
+      ia = zl::sat_add(ia, ua);
+      ib = zl::sat_add(ib, ub);
+    }
+  }
+  if (lane == 31) {
+    wa[warp] = ia;
+    wb[warp] = ib;
+  }
+  int32_t ea = __shfl_up_sync(0xffffffffu, ia, 1), eb = __shfl_up_sync(0xffffffffu, ib, 1);
+  if (lane == 0) ea = eb = 0;
+  __syncthreads();
+  for (int w = 0; w < warp; w++) {
+    ea = zl::sat_add(ea, wa[w]);
+    eb = zl::sat_add(eb, wb[w]);
+  }
+  for (int i = lo; i < hi; i++) {
+    const int32_t va = a[i], vb = b[i];
+    a[i] = ea;
+    b[i] = eb;
+    ea = zl::sat_add(ea, va);
+    eb = zl::sat_add(eb, vb);
+  }
+  if (threadIdx.x == kThreads - 1) a[n] = ea;
+}
+
+__global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
+  extern __shared__ int32_t sh[];
+  const int n = g.num_seqs;
+  int32_t* cu = sh;                                             // [n + 1] first token row
+  int32_t* fresh = cu + n + 1;                                  // [n] first new id
+  int32_t* row = fresh + n;                                     // [n] row of seq_blocks, -1: nothing to serve
+  uint32_t* once = reinterpret_cast<uint32_t*>(row + n);        // rows seen
+  const int words = g.rows ? (g.num_rows + 31) / 32 : 0;
+  uint32_t* twice = once + words;                               // rows seen again
+  int bad = 0;
+
+  for (int w = threadIdx.x; w < 2 * words; w += kThreads) once[w] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int r = g.rows ? g.rows[i] : i;
+    const zl::StepRequest q = zl::step_request(g.context_lens[i], g.query_lens[i], g.bs, g.max_blocks);
+    cu[i] = q.tokens;
+    fresh[i] = r < 0 ? 0 : q.need;
+    row[i] = r >= 0 && r < g.num_rows && q.ok ? r : -1;
+    bad |= r >= 0 && row[i] < 0;
+    if (g.rows && row[i] >= 0) {
+      const uint32_t bit = 1u << (r & 31);
+      if (atomicOr(once + (r >> 5), bit) & bit) atomicOr(twice + (r >> 5), bit);
+    }
+  }
+  __syncthreads();
+  scan2(cu, fresh, n);
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int r = row[i];
+    // every request of a row that is listed twice, or whose tokens do not fit
+    if (r >= 0 && ((g.rows && (twice[r >> 5] >> (r & 31) & 1)) || cu[i + 1] > g.num_tokens)) {
+      row[i] = -1;
+      bad = 1;
+    }
+  }
+  __syncthreads();
+
+  const int gtid = blockIdx.x * kThreads + threadIdx.x, gsize = gridDim.x * kThreads;
+  const int32_t cap = (int32_t)(g.num_tokens < 0x7fffffff ? g.num_tokens : 0x7fffffff);
+  for (int i = gtid; i <= n; i += gsize) {
+    const int32_t c = min(cu[i], cap);
+    g.cu_seqlens[i] = c;
+    if (i < n) {
+      g.seq_lens[i] = row[i] < 0 ? 0 : g.context_lens[i] + g.query_lens[i];
+      g.last_rows[i] = max(min(cu[i + 1], cap) - 1, 0);
+    }
+  }
+  // table rows: a warp per row and 128 columns
+  const int segs = (g.max_blocks + 127) / 128;
+  for (int64_t u = gtid >> 5; u < (int64_t)n * segs; u += gsize >> 5) {
+    const int i = (int)(u / segs), c0 = (int)(u - (int64_t)i * segs) * 128 + (threadIdx.x & 31);
+    const int r = row[i];
+    int had = 0, has = 0;
+    if (r >= 0) {
+      const zl::StepRequest q = zl::step_request(g.context_lens[i], g.query_lens[i], g.bs, g.max_blocks);
+      had = q.had;
+      has = q.had + q.need;
+    }
+    for (int c = c0; c < min(c0 + 128, g.max_blocks); c += 32) {
+      int32_t id = -1;
+      if (c < has) {
+        int32_t* at = g.seq_blocks + (int64_t)r * g.max_blocks + c;
+        const int64_t k = (int64_t)fresh[i] + c - had;
+        id = c < had ? *at : k < g.num_new ? g.new_blocks[k] : -1;
+        if (id < 0 || id >= g.num_blocks) {
+          id = -1;
+          bad = 1;
+        }
+        if (c >= had) *at = id;
+      }
+      g.block_tables[(int64_t)i * g.max_blocks + c] = id;
+    }
+  }
+  // token rows
+  for (int64_t t = gtid; t < g.num_tokens; t += gsize) {
+    int32_t pos = 0;
+    int64_t slot = -1;
+    if (t < cu[n]) {
+      int lo = 0, hi = n;  // the last request that starts at or before t: cu[lo] <= t < cu[lo + 1]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int r = row[lo];
+      if (r >= 0) {
+        const int32_t ctx = g.context_lens[lo];
+        pos = ctx + (int32_t)(t - cu[lo]);
+        const int had = (int)zl::blocks_of(ctx, g.bs), c = pos / g.bs;
+        const int64_t k = (int64_t)fresh[lo] + c - had;
+        const int32_t id = c < had ? g.seq_blocks[(int64_t)r * g.max_blocks + c] : k < g.num_new ? g.new_blocks[k] : -1;
+        if (id >= 0 && id < g.num_blocks) slot = (int64_t)id * g.bs + pos % g.bs;
+        else bad = 1;
+      }
+    }
+    g.positions[t] = pos;
+    g.slot_mapping[t] = slot;
+  }
+  if (threadIdx.x == 0 && cu[n] > g.num_tokens) bad = 1;
+  if (bad) atomicOr(g.status, ZL_DEV_OOB);
+}
+
+}  // namespace
+
+extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_rows, const int32_t* rows,
+                                    const int32_t* context_lens, const int32_t* query_lens,
+                                    const int32_t* new_blocks, int64_t num_new, int32_t* block_tables,
+                                    int32_t* cu_seqlens, int32_t* seq_lens, int32_t* positions,
+                                    int64_t* slot_mapping, int32_t* last_rows, int num_seqs, int64_t num_tokens,
+                                    int max_blocks_per_seq, int block_size, int64_t num_blocks, zl_stream stream) {
+  using namespace zl;
+  if (num_seqs < 0 || num_rows < 0 || num_new < 0 || num_tokens < 0 || max_blocks_per_seq < 0 || block_size <= 0 ||
+      num_blocks < 0)
+    return set_error(ZL_ERR_INVALID_ARG,
+                     "step_tables: bad sizes n=%d rows=%d new=%lld T=%lld max_blocks=%d bs=%d blocks=%lld", num_seqs,
+                     num_rows, (long long)num_new, (long long)num_tokens, max_blocks_per_seq, block_size,
+                     (long long)num_blocks);
+  if (num_tokens > INT32_MAX || num_blocks > INT32_MAX)
+    return set_error(ZL_ERR_INVALID_ARG, "step_tables: more than 2^31-1 token rows or blocks");
+  if (num_seqs > kMaxSeqs || (rows && num_rows > kMaxRows))
+    return set_error(ZL_ERR_UNSUPPORTED, "step_tables: at most %d requests (have %d) and %d table rows (have %d)",
+                     kMaxSeqs, num_seqs, kMaxRows, num_rows);
+  if (!rows && num_rows < num_seqs)
+    return set_error(ZL_ERR_INVALID_ARG, "step_tables: %d table rows for %d requests without `rows`", num_rows, num_seqs);
+  if (!cu_seqlens || (num_seqs && (!context_lens || !query_lens || !seq_lens || !last_rows)) ||
+      (num_seqs && max_blocks_per_seq && (!block_tables || (num_rows && !seq_blocks))) || (num_new && !new_blocks) ||
+      (num_tokens && (!positions || !slot_mapping)))
+    return set_error(ZL_ERR_INVALID_ARG, "step_tables: null pointer");
+  DeviceScope dev(ctx);
+  if (dev.status != ZL_OK) return dev.status;
+  StepArgs g{seq_blocks, rows, context_lens, query_lens, new_blocks, block_tables, cu_seqlens, seq_lens, positions,
+             slot_mapping, last_rows, num_new, num_tokens, num_blocks, num_rows, num_seqs, max_blocks_per_seq,
+             block_size, ctx->d_status};
+  const size_t smem = sizeof(int32_t) * (3 * (size_t)num_seqs + 1) + (rows ? 8 * (size_t)((num_rows + 31) / 32) : 0);
+  if (smem > 48 * 1024)
+    ZL_CUDA_TRY(cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)smem));
+  const int64_t items = (int64_t)num_seqs * ((max_blocks_per_seq + 127) / 128) * 32 + num_tokens + num_seqs + 1;
+  int64_t blocks = (items + kThreads - 1) / kThreads;
+  if (blocks > 2 * ctx->num_sms) blocks = 2 * ctx->num_sms;
+  step_tables_kernel<<<(unsigned)blocks, kThreads, smem, S(stream)>>>(g);
+  ZL_LAUNCH_CHECK(ctx);
+  return ZL_OK;
+}

@@ -57,6 +57,27 @@ inline zl_status ok() { return ZL_OK; }
 // Makes the context's device current; returns ZL_ERR_CUDA on failure.
 zl_status bind_device(zl_ctx* ctx);
 
+// Makes the context's device current for the time of a call and puts the
+// caller's back at its end. status: ZL_OK, or why the device cannot be used.
+struct DeviceScope {
+  int before = -1;
+  zl_status status;
+  explicit DeviceScope(zl_ctx* ctx) {
+    if (ctx && cudaGetDevice(&before) != cudaSuccess) before = -1;
+    if (ctx && before == ctx->device) {
+      before = -1;
+      status = ZL_OK;
+    } else {
+      status = bind_device(ctx);
+    }
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 // Grows the context workspace (stream-ordered free of the old one is not
 // needed: callers synchronise through the stream they pass).
 zl_status ensure_workspace(zl_ctx* ctx, size_t bytes);
@@ -81,6 +102,7 @@ inline cudaStream_t S(zl_stream s) { return reinterpret_cast<cudaStream_t>(s); }
     (ctx)->launches.fetch_add(1, std::memory_order_relaxed);                         \
   } while (0)
 
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline size_t dtype_size(zl_dtype t) { return t == ZL_F32 ? 4 : 2; }
 inline bool dtype_ok(zl_dtype t) { return t == ZL_F32 || t == ZL_BF16; }
 
@@ -92,6 +114,13 @@ zl_status launch_decode_generic(zl_ctx* ctx, const void* q, const void* k_pool,
                                 int B, int H, int Hkv, int d, int bs, int max_blocks,
                                 int64_t num_blocks, float scale, zl_gqa_map map,
                                 zl_dtype dtype, cudaStream_t st);
+// Decode over the blocks listed in `selected` [B][Hkv][max_selected]; the caller has checked
+// the sizes (head_dim <= 256, B*H < 2^31).
+zl_status launch_decode_selected_generic(zl_ctx* ctx, const void* q, const void* k_pool, const void* v_pool,
+                                         const int32_t* block_tables, const int32_t* seq_lens,
+                                         const int32_t* selected, void* out, int B, int H, int Hkv, int d, int bs,
+                                         int max_blocks, int64_t num_blocks, int max_selected, float scale,
+                                         zl_gqa_map map, zl_dtype dtype, cudaStream_t st);
 // Both prefill launchers check cu_seqlens on the device against total_tokens
 // (ZL_DEV_OOB and the sequence skipped when it leaves [0, total_tokens]).
 zl_status launch_prefill_generic(zl_ctx* ctx, const void* q, const void* k, const void* v,
