@@ -123,6 +123,10 @@ zl_status zl_paged_decode_selected(zl_ctx* ctx, const void* q, const void* k_poo
     return set_error(ZL_ERR_INVALID_ARG, "paged_decode_selected: null pointer");
   DeviceScope dev(ctx);
   if (dev.status != ZL_OK) return dev.status;
+  s = launch_decode_selected_fast(ctx, q, k_pool, v_pool, block_tables, seq_lens, selected, out, num_seqs, num_heads,
+                                  num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks, max_selected,
+                                  resolve_scale(scale, head_dim), gqa_map, dtype, S(stream));
+  if (s != ZL_ERR_UNSUPPORTED) return s;
   return launch_decode_selected_generic(ctx, q, k_pool, v_pool, block_tables, seq_lens, selected, out, num_seqs,
                                         num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks,
                                         max_selected, resolve_scale(scale, head_dim), gqa_map, dtype, S(stream));

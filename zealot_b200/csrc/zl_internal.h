@@ -121,6 +121,12 @@ zl_status launch_decode_selected_generic(zl_ctx* ctx, const void* q, const void*
                                          const int32_t* selected, void* out, int B, int H, int Hkv, int d, int bs,
                                          int max_blocks, int64_t num_blocks, int max_selected, float scale,
                                          zl_gqa_map map, zl_dtype dtype, cudaStream_t st);
+// The same for rows that 16-byte loads can read (selected_decode.cu); ZL_ERR_UNSUPPORTED otherwise.
+zl_status launch_decode_selected_fast(zl_ctx* ctx, const void* q, const void* k_pool, const void* v_pool,
+                                      const int32_t* block_tables, const int32_t* seq_lens,
+                                      const int32_t* selected, void* out, int B, int H, int Hkv, int d, int bs,
+                                      int max_blocks, int64_t num_blocks, int max_selected, float scale,
+                                      zl_gqa_map map, zl_dtype dtype, cudaStream_t st);
 // Both prefill launchers check cu_seqlens on the device against total_tokens
 // (ZL_DEV_OOB and the sequence skipped when it leaves [0, total_tokens]).
 zl_status launch_prefill_generic(zl_ctx* ctx, const void* q, const void* k, const void* v,
