@@ -9,19 +9,21 @@
 // cluster's distributed shared memory, in a fixed order. So a call takes no
 // workspace and no counter, and a launch for few sequences still fills the GPU.
 //
-// bf16 (selected_mma_kernel): a warp takes 32 tokens at a time straight from
-// global memory into the registers that its matrix instructions read. S = q K^T
-// has the (at most 8) query heads as the upper half of M = 16 and 8 tokens as
-// N: a lane's 16 bytes of a key row are its B operands for two steps of K = 16
-// once q is loaded in the same order, so keys need no shared memory. O^T = V^T P^T
-// has 16 elements of a value row as M and the heads as N: a lane loads 16 bytes
-// of each of four token rows and pairs two tokens' elements with a byte
-// permute. S's accumulators are P^T's operands as they stand. P enters as two
-// bf16 parts, p - bf16(p) being the second: the weights then keep 16 bits, for
-// one more instruction per tile in a kernel that waits for memory.
+// Every warp keeps a ring of small tiles of keys and values in shared memory,
+// filled by asynchronous 16-byte copies: any block size and order, and rows that
+// do not count are zeros.
 //
-// fp32 (selected_f32_kernel): eight lanes share a token's row, a warp four
-// tokens at a time, on the CUDA cores.
+// bf16 (selected_mma_kernel), tiles of 16 tokens: S = q K^T has the (at most 8) query
+// heads as the upper half of M = 16 and 8 tokens as N: a lane's 16 bytes of a key
+// row are its B operands for two steps of K = 16 once q is loaded in the same
+// order. O^T = V^T P^T has 16 elements of a value row as M and the heads as N: a
+// lane reads 16 bytes of each of four token rows and pairs two tokens' elements
+// with a byte permute. S's accumulators are P^T's operands as they stand. P enters
+// as two bf16 parts, p - bf16(p) being the second: the weights then keep 16 bits,
+// for one more instruction per tile in a kernel that waits for memory.
+//
+// fp32 (selected_f32_kernel), tiles of 8 tokens: eight lanes share a token's row,
+// on the CUDA cores.
 #include <cooperative_groups.h>
 
 #include "zl_internal.h"
@@ -34,6 +36,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kMaxCluster = 8;
 constexpr int kEntries = 512;  // list entries of a CTA that are resolved at a time
 
 struct SelArgs {
@@ -62,8 +65,9 @@ struct Job {
   }
 };
 
+// The part is one of `cluster` equal ones of max_selected entries: a list that
+// ends early leaves its last CTAs idle, and none has to read the list first.
 __device__ __forceinline__ Job find_job(const SelArgs& g, int cluster, int rank) {
-  __shared__ int first_neg;
   Job w;
   int u = blockIdx.x / cluster;
   const int sub = u % g.subs;
@@ -73,17 +77,7 @@ __device__ __forceinline__ Job find_job(const SelArgs& g, int cluster, int rank)
   w.head0 = sub * g.per_sub;
   w.heads = min(g.per_sub, g.group - w.head0);
   w.list = g.selected + (int64_t)u * g.max_selected;
-  if (threadIdx.x == 0) first_neg = g.max_selected;
-  __syncthreads();
-  int neg = g.max_selected;
-  for (int i = threadIdx.x; i < g.max_selected; i += kThreads)
-    if (w.list[i] < 0) {
-      neg = i;
-      break;
-    }
-  if (neg < g.max_selected) atomicMin(&first_neg, neg);
-  __syncthreads();
-  const int n = first_neg, step = (32 + g.bs - 1) / g.bs;  // whole tiles of 32 tokens
+  const int n = g.max_selected, step = (16 + g.bs - 1) / g.bs;  // whole tiles of 16 tokens
   int per = (n + cluster - 1) / cluster;
   per = (per + step - 1) / step * step;
   w.e0 = min(n, rank * per);
@@ -91,27 +85,40 @@ __device__ __forceinline__ Job find_job(const SelArgs& g, int cluster, int rank)
   return w;
 }
 
-// Resolves list entries [e, e + count) into shared memory.
-__device__ __forceinline__ void resolve(const SelArgs& g, const Job& w, int e, int count, Entry* sh) {
+// Resolves list entries [e, e + count) into shared memory and returns how many
+// of them come before the list's first negative entry (`end`, kept over calls).
+__device__ __forceinline__ int resolve(const SelArgs& g, const Job& w, int e, int count, Entry* sh, int* end) {
   const int32_t* table = g.tables + (int64_t)w.b * g.max_blocks;
+  if (threadIdx.x == 0 && e == w.e0) *end = g.max_selected;
+  __syncthreads();
+  int neg = g.max_selected;
   const int64_t len = g.seq_lens[w.b];
+  if (e == w.e0)  // entries of the CTAs before this one
+    for (int i = threadIdx.x; i < e; i += kThreads)
+      if (w.list[i] < 0) neg = min(neg, i);
   for (int i = threadIdx.x; i < count; i += kThreads) {
     const int j = w.list[e + i];
     Entry t{0, 0};
-    if (j >= g.max_blocks) {
-      atomicOr(g.status, ZL_DEV_OOB);
-    } else {
-      const int64_t left = len - (int64_t)j * g.bs;
-      const int32_t id = table[j];
-      if (left > 0 && id >= g.num_blocks) atomicOr(g.status, ZL_DEV_OOB);
+    if (j < 0) {
+      neg = min(neg, e + i);
+    } else if (j < g.max_blocks) {
+      const int64_t left = len - (int64_t)j * g.bs, id = table[j];
       const int64_t row = zl::pool_row(id, g.num_blocks, g.Hkv, w.kvh, g.bs, 0);
-      if (row >= 0 && left > 0) {
-        t.row = (int32_t)row;
-        t.tokens = (int32_t)min(left, (int64_t)g.bs);
+      if (left > 0) {
+        t.row = (int32_t)(row >= 0 ? row : id >= 0 ? -2 : -1);
+        t.tokens = row >= 0 ? (int32_t)min(left, (int64_t)g.bs) : 0;
       }
+    } else {
+      t.row = -2;
     }
     sh[i] = t;
   }
+  if (neg < g.max_selected) atomicMin(end, neg);
+  __syncthreads();
+  const int used = max(0, min(count, *end - e));
+  for (int i = threadIdx.x; i < used; i += kThreads)  // outside the table row or the pool
+    if (sh[i].row == -2) atomicOr(g.status, ZL_DEV_OOB);
+  return used;
 }
 
 // Joins the warps' (m, l, o) and then the cluster's, and writes the heads' outputs.
@@ -162,26 +169,74 @@ __device__ __forceinline__ void finish(const SelArgs& g, const Job& w, int clust
   if (cluster > 1) cl.sync();  // a CTA's shared memory stays until all have read it
 }
 
-__device__ __forceinline__ uint4 load16(const void* p) {
+// 16 bytes to shared memory in the background; zeros, and nothing read, where !use.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool use) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(use ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
 
-// head_dim up to DT, a multiple of 8; NT: 8-token tiles a warp takes at a time.
-template <int DT, int NT>
-__global__ void __launch_bounds__(kThreads, 2) selected_mma_kernel(SelArgs g, int cluster) {
-  constexpr int KC = DT / 32, VH = DT / 64, TOK = NT * 8;
+// Starts the copies of one tile, TOK tokens' key rows and then their value rows of ROWB
+// bytes each (what is behind the real row_bytes is zeros, as are the rows of tokens that do
+// not count), as one group; an empty group where there is no such tile. Returns which tokens
+// count. With SWIZZLE a row's 16-byte chunks lie at chunk ^ (row & 7).
+template <int ROWB, int TOK, bool SWIZZLE>
+__device__ __forceinline__ uint32_t fetch_tile(const SelArgs& g, const Entry* entries, int tile, int toks, uint32_t dst,
+                                               int row_bytes) {
+  constexpr int CPR = ROWB / 16;
+  const int lane = threadIdx.x & 31;
+  uint32_t there = 0;
+  if (tile * TOK < toks) {
+    int row = -1;
+    const int tok = tile * TOK + lane;
+    if (lane < TOK && tok < toks) {
+      const int i = tok / g.bs, t = tok - i * g.bs;
+      const Entry en = entries[i];
+      if (t < en.tokens) row = en.row + t;
+    }
+    there = __ballot_sync(0xffffffffu, row >= 0);
+#pragma unroll
+    for (int it = 0; it < TOK * CPR / 32; it++) {
+      const int r = (it * 32 + lane) / CPR, ch = (it * 32 + lane) % CPR;
+      const int from = __shfl_sync(0xffffffffu, row, r);
+      const bool use = from >= 0 && ch * 16 < row_bytes;
+      const int64_t at = use ? (int64_t)from * row_bytes + ch * 16 : 0;
+      const uint32_t to = dst + r * ROWB + ((SWIZZLE ? ch ^ (r & 7) : ch) * 16);
+      copy16(to, (const uint8_t*)g.k_pool + at, use);
+      copy16(to + TOK * ROWB, (const uint8_t*)g.v_pool + at, use);
+    }
+  }
+  copies_commit();
+  return there;
+}
+
+// Shared memory of either kernel: each warp's ring of ST tiles, which the warps' outputs
+// take over at the end.
+constexpr size_t ring_bytes(int rowb, int tok, int st) { return (size_t)kWarps * st * tok * rowb * 2; }
+
+// head_dim up to DT, a multiple of 8. Column n of the score tile i in {0, 1} is token 2 (n / 2) + i for even n and
+// 8 + i + (2 (n / 2) + 4) % 8 for odd n: the two rows that a quarter warp reads of the
+// keys then differ in bit 2 of the row, the four that it reads of the values in bits 1
+// and 2, and neither has a bank conflict.
+template <int DT, int ST>
+__global__ void __launch_bounds__(kThreads) selected_mma_kernel(SelArgs g, int cluster) {
+  constexpr int KC = DT / 32, VH = DT / 64, ROW = DT * 2;
+  constexpr uint32_t TILE = 16 * ROW;
+  extern __shared__ __align__(128) uint8_t ring[];
   __shared__ Entry entries[kEntries];
-  __shared__ __align__(16) float o_sh[kWarps * 8 * DT];
   __shared__ float m_sh[kWarps][8], l_sh[kWarps][8];
+  __shared__ int list_end;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   const int rank = blockIdx.x % cluster;
   const Job w = find_job(g, cluster, rank);
-  const __nv_bfloat16* kp = (const __nv_bfloat16*)g.k_pool;
-  const __nv_bfloat16* vp = (const __nv_bfloat16*)g.v_pool;
+  const uint32_t mine = zl::ptx::smem_u32(ring) + warp * ST * 2 * TILE;
 
   uint4 q[KC];
 #pragma unroll
@@ -189,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 2) selected_mma_kernel(SelArgs g, in
     const int e = k * 32 + c * 8;
     q[k] = make_uint4(0, 0, 0, 0);
     if (n < w.heads && e < g.d)
-      q[k] = load16((const __nv_bfloat16*)g.q + ((int64_t)w.b * g.H + w.head(g, n)) * g.d + e);
+      q[k] = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)g.q + ((int64_t)w.b * g.H + w.head(g, n)) * g.d + e);
   }
   float o[VH][4][4];
 #pragma unroll
@@ -199,107 +254,108 @@ __global__ void __launch_bounds__(kThreads, 2) selected_mma_kernel(SelArgs g, in
 #pragma unroll
       for (int x = 0; x < 4; x++) o[a][j][x] = 0.f;
   float m = -INFINITY, l = 0.f;
+  // this lane's key rows (column n of either tile) and value rows (columns 2 c, 2 c + 1)
+  const int krow = n & 1 ? 8 + ((2 * (n >> 1) + 4) & 7) : 2 * (n >> 1);
+  const int vrow[2] = {2 * c, 8 + ((2 * c + 4) & 7)};
 
   for (int e = w.e0; e < w.e1; e += kEntries) {
-    const int count = min(kEntries, w.e1 - e);
     if (e > w.e0) __syncthreads();
-    resolve(g, w, e, count, entries);
-    __syncthreads();
-    const int toks = count * g.bs;
-    for (int t0 = warp * TOK; t0 < toks; t0 += kWarps * TOK) {
-      // lane i resolves token t0 + i (the first TOK lanes)
-      int row = -1;
-      if (lane < TOK && t0 + lane < toks) {
-        const int i = (t0 + lane) / g.bs, t = t0 + lane - i * g.bs;
-        const Entry en = entries[i];
-        if (t < en.tokens) row = en.row + t;
-      }
-      uint4 kr[NT][KC], vr[NT][2][VH];
-      bool see[NT][2];
+    const int toks = resolve(g, w, e, min(kEntries, w.e1 - e), entries, &list_end) * g.bs;
+    const int tiles = (toks + 15) / 16;
+    uint32_t seen[ST];  // which of a tile's 16 tokens there are, by ring slot
+    auto fetch = [&](int tile, int slot) {
+      return fetch_tile<ROW, 16, true>(g, entries, tile, toks, mine + slot * 2 * TILE, g.d * 2);
+    };
 #pragma unroll
-      for (int i = 0; i < NT; i++) {
-        const int r = __shfl_sync(0xffffffffu, row, 8 * i + n);
+    for (int i = 0; i < ST - 1; i++) seen[i] = fetch(warp + i * kWarps, i);
+    for (int tile = warp; tile < tiles;) {
 #pragma unroll
-        for (int k = 0; k < KC; k++) {
-          kr[i][k] = make_uint4(0, 0, 0, 0);
-          if (r >= 0 && k * 32 + c * 8 < g.d) kr[i][k] = load16(kp + (int64_t)r * g.d + k * 32 + c * 8);
-        }
-      }
+      for (int slot = 0; slot < ST; slot++, tile += kWarps) {
+        if (tile >= tiles) break;
+        seen[(slot + ST - 1) % ST] = fetch(tile + (ST - 1) * kWarps, (slot + ST - 1) % ST);
+        copies_wait<ST - 1>();
+        __syncwarp();
+        const uint32_t ks = mine + slot * 2 * TILE, vs = ks + TILE;
+        float s[2][4];
 #pragma unroll
-      for (int i = 0; i < NT; i++)
+        for (int i = 0; i < 2; i++) {
+          float s2[4] = {0.f, 0.f, 0.f, 0.f};  // a second chain of products: half the latency
+          s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+          const int r = krow + i;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-          const int r = __shfl_sync(0xffffffffu, row, 8 * i + 2 * c + s);
-          see[i][s] = r >= 0;
-#pragma unroll
-          for (int a = 0; a < VH; a++) {
-            vr[i][s][a] = make_uint4(0, 0, 0, 0);
-            if (r >= 0 && a * 64 + n * 8 < g.d) vr[i][s][a] = load16(vp + (int64_t)r * g.d + a * 64 + n * 8);
+          for (int k = 0; k < KC; k++) {
+            const uint4 x = lds16(ks + r * ROW + (((k * 4 + c) ^ (r & 7)) * 16));
+            zl::ptx::mma_bf16_16816(s[i], q[k].x, 0, q[k].y, 0, x.x, x.y);
+            zl::ptx::mma_bf16_16816(s2, q[k].z, 0, q[k].w, 0, x.z, x.w);
           }
+          s[i][0] += s2[0];
+          s[i][1] += s2[1];
         }
-      float s[NT][4];
+        // row n of S: head n over this lane's tokens vrow[x] + i
+        float best = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < NT; i++) {
-        s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int k = 0; k < KC; k++) {
-          zl::ptx::mma_bf16_16816(s[i], q[k].x, 0, q[k].y, 0, kr[i][k].x, kr[i][k].y);
-          zl::ptx::mma_bf16_16816(s[i], q[k].z, 0, q[k].w, 0, kr[i][k].z, kr[i][k].w);
-        }
-      }
-      // row n of S: head n over this lane's tokens 8 i + 2 c and + 1
-      float best = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          s[i][x] = see[i][x] ? s[i][x] * g.scale2 : -INFINITY;
-          best = fmaxf(best, s[i][x]);
-        }
-      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-      if (__any_sync(0xffffffffu, best > m)) {
-        const float to = fmaxf(m, best);
-        const float a = m == -INFINITY ? 0.f : zl::ptx::ex2(m - to);
-        m = to;
-        l *= a;
-        const float a0 = __shfl_sync(0xffffffffu, a, 8 * c), a1 = __shfl_sync(0xffffffffu, a, 8 * c + 4);
-#pragma unroll
-        for (int h = 0; h < VH; h++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            o[h][j][0] *= a0;
-            o[h][j][1] *= a1;
-            o[h][j][2] *= a0;
-            o[h][j][3] *= a1;
+          for (int x = 0; x < 2; x++) {
+            s[i][x] = seen[slot] >> (vrow[x] + i) & 1 ? s[i][x] * g.scale2 : -INFINITY;
+            best = fmaxf(best, s[i][x]);
           }
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      uint32_t hi[NT], lo[NT];
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+        if (__any_sync(0xffffffffu, best > m)) {
+          const float to = fmaxf(m, best);
+          const float a = m == -INFINITY ? 0.f : zl::ptx::ex2(m - to);
+          m = to;
+          l *= a;
+          const float a0 = __shfl_sync(0xffffffffu, a, 8 * c), a1 = __shfl_sync(0xffffffffu, a, 8 * c + 4);
 #pragma unroll
-      for (int i = 0; i < NT; i++) {
-        const float p0 = zl::ptx::ex2(s[i][0] - base), p1 = zl::ptx::ex2(s[i][1] - base);
-        l += p0 + p1;
-        hi[i] = zl::ptx::pack_bf16x2(p0, p1);
-        const __nv_bfloat162 hb = *reinterpret_cast<const __nv_bfloat162*>(&hi[i]);
-        lo[i] = zl::ptx::pack_bf16x2(p0 - __low2float(hb), p1 - __high2float(hb));
-      }
-      // O^T: rows n and n + 8 of tile (a, j) are elements 64 a + 8 n + j and + 4
+          for (int h = 0; h < VH; h++)
 #pragma unroll
-      for (int i = 0; i < NT; i += 2)
+            for (int j = 0; j < 4; j++) {
+              o[h][j][0] *= a0;
+              o[h][j][1] *= a1;
+              o[h][j][2] *= a0;
+              o[h][j][3] *= a1;
+            }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const float p0 = zl::ptx::ex2(s[i][0] - base), p1 = zl::ptx::ex2(s[i][1] - base);
+          l += p0 + p1;
+          hi[i] = zl::ptx::pack_bf16x2(p0, p1);
+          const __nv_bfloat162 hb = *reinterpret_cast<const __nv_bfloat162*>(&hi[i]);
+          lo[i] = zl::ptx::pack_bf16x2(p0 - __low2float(hb), p1 - __high2float(hb));
+        }
+        // O^T: rows n and n + 8 of tile (a, j) are elements 64 a + 8 n + j and + 4
 #pragma unroll
         for (int a = 0; a < VH; a++) {
-          const uint32_t* r[4] = {&vr[i][0][a].x, &vr[i][1][a].x, &vr[i + 1][0][a].x, &vr[i + 1][1][a].x};
+          uint32_t r[4][4];
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              const int t = vrow[x] + i;
+              const uint4 y = lds16(vs + t * ROW + (((a * 8 + n) ^ (t & 7)) * 16));
+              r[2 * i + x][0] = y.x;
+              r[2 * i + x][1] = y.y;
+              r[2 * i + x][2] = y.z;
+              r[2 * i + x][3] = y.w;
+            }
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
             const uint32_t a0 = __byte_perm(r[0][j / 2], r[1][j / 2], sel), a1 = __byte_perm(r[0][2 + j / 2], r[1][2 + j / 2], sel);
             const uint32_t a2 = __byte_perm(r[2][j / 2], r[3][j / 2], sel), a3 = __byte_perm(r[2][2 + j / 2], r[3][2 + j / 2], sel);
-            zl::ptx::mma_bf16_16816(o[a][j], a0, a1, a2, a3, hi[i], hi[i + 1]);
-            zl::ptx::mma_bf16_16816(o[a][j], a0, a1, a2, a3, lo[i], lo[i + 1]);
+            zl::ptx::mma_bf16_16816(o[a][j], a0, a1, a2, a3, hi[0], hi[1]);
+            zl::ptx::mma_bf16_16816(o[a][j], a0, a1, a2, a3, lo[0], lo[1]);
           }
         }
+        __syncwarp();  // the next fetch takes this slot
+      }
     }
+    copies_wait<0>();
   }
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -307,6 +363,8 @@ __global__ void __launch_bounds__(kThreads, 2) selected_mma_kernel(SelArgs g, in
     m_sh[warp][n] = m;
     l_sh[warp][n] = l;
   }
+  __syncthreads();  // every warp is done with its ring
+  float* o_sh = reinterpret_cast<float*>(ring);
   float* ow = o_sh + warp * 8 * DT;
 #pragma unroll
   for (int a = 0; a < VH; a++)
@@ -318,18 +376,19 @@ __global__ void __launch_bounds__(kThreads, 2) selected_mma_kernel(SelArgs g, in
 }
 
 // fp32, head_dim up to 32 NV, a multiple of 4; HEADS query heads at a time.
-template <int NV, int HEADS>
-__global__ void __launch_bounds__(kThreads, 2) selected_f32_kernel(SelArgs g, int cluster) {
-  constexpr int DT = NV * 32;
+template <int NV, int HEADS, int ST>
+__global__ void __launch_bounds__(kThreads) selected_f32_kernel(SelArgs g, int cluster) {
+  constexpr int DT = NV * 32, ROW = DT * 4;
+  constexpr uint32_t TILE = 8 * ROW;
+  extern __shared__ __align__(128) uint8_t ring[];
   __shared__ Entry entries[kEntries];
-  __shared__ __align__(16) float o_sh[kWarps * HEADS * DT];
   __shared__ __align__(16) float q_sh[HEADS * DT];
   __shared__ float m_sh[kWarps][HEADS], l_sh[kWarps][HEADS];
+  __shared__ int list_end;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tg = lane >> 3, li = lane & 7;
   const int rank = blockIdx.x % cluster;
   const Job w = find_job(g, cluster, rank);
-  const float* kp = (const float*)g.k_pool;
-  const float* vp = (const float*)g.v_pool;
+  const uint32_t mine = zl::ptx::smem_u32(ring) + warp * ST * 2 * TILE;
   for (int i = threadIdx.x; i < HEADS * DT; i += kThreads) {
     const int h = i / DT, e = i - h * DT;
     q_sh[i] = h < w.heads && e < g.d ? ((const float*)g.q)[((int64_t)w.b * g.H + w.head(g, h)) * g.d + e] * g.scale2 : 0.f;
@@ -343,55 +402,77 @@ __global__ void __launch_bounds__(kThreads, 2) selected_f32_kernel(SelArgs g, in
 #pragma unroll
     for (int v = 0; v < NV; v++) o[h][v] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  auto row4 = [](uint32_t a) {
+    const uint4 x = lds16(a);
+    return make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+  };
   for (int e = w.e0; e < w.e1; e += kEntries) {
-    const int count = min(kEntries, w.e1 - e);
     if (e > w.e0) __syncthreads();
-    resolve(g, w, e, count, entries);
-    __syncthreads();
-    const int toks = count * g.bs;
-    for (int t0 = warp * 4; t0 < toks; t0 += kWarps * 4) {
-      int row = -1;
-      if (t0 + tg < toks) {
-        const int i = (t0 + tg) / g.bs, t = t0 + tg - i * g.bs;
-        const Entry en = entries[i];
-        if (t < en.tokens) row = en.row + t;
-      }
-      float4 kr[NV], vr[NV];
+    const int toks = resolve(g, w, e, min(kEntries, w.e1 - e), entries, &list_end) * g.bs;
+    const int tiles = (toks + 7) / 8;
+    uint32_t seen[ST];
+    auto fetch = [&](int tile, int slot) {
+      return fetch_tile<ROW, 8, false>(g, entries, tile, toks, mine + slot * 2 * TILE, g.d * 4);
+    };
 #pragma unroll
-      for (int v = 0; v < NV; v++) {
-        const int x = v * 32 + li * 4;
-        kr[v] = vr[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (row >= 0 && x < g.d) {
-          kr[v] = __ldg(reinterpret_cast<const float4*>(kp + (int64_t)row * g.d + x));
-          vr[v] = __ldg(reinterpret_cast<const float4*>(vp + (int64_t)row * g.d + x));
-        }
-      }
+    for (int i = 0; i < ST - 1; i++) seen[i] = fetch(warp + i * kWarps, i);
+    for (int tile = warp; tile < tiles;) {
 #pragma unroll
-      for (int h = 0; h < HEADS; h++) {
-        float s = 0.f;
+      for (int slot = 0; slot < ST; slot++, tile += kWarps) {
+        if (tile >= tiles) break;
+        seen[(slot + ST - 1) % ST] = fetch(tile + (ST - 1) * kWarps, (slot + ST - 1) % ST);
+        copies_wait<ST - 1>();
+        __syncwarp();
+        // this lane's elements of rows tg and 4 + tg
+        const uint32_t ks = mine + slot * 2 * TILE + tg * ROW + li * 16, vs = ks + TILE;
+        float s[HEADS][2];
+#pragma unroll
+        for (int h = 0; h < HEADS; h++) s[h][0] = s[h][1] = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-          const float4 qv = *reinterpret_cast<const float4*>(&q_sh[h * DT + v * 32 + li * 4]);
-          s = fmaf(qv.x, kr[v].x, fmaf(qv.y, kr[v].y, fmaf(qv.z, kr[v].z, fmaf(qv.w, kr[v].w, s))));
+          const float4 k0 = row4(ks + v * 128), k1 = row4(ks + 4 * ROW + v * 128);
+#pragma unroll
+          for (int h = 0; h < HEADS; h++) {
+            const float4 x = *reinterpret_cast<const float4*>(&q_sh[h * DT + v * 32 + li * 4]);
+            s[h][0] = fmaf(x.x, k0.x, fmaf(x.y, k0.y, fmaf(x.z, k0.z, fmaf(x.w, k0.w, s[h][0]))));
+            s[h][1] = fmaf(x.x, k1.x, fmaf(x.y, k1.y, fmaf(x.z, k1.z, fmaf(x.w, k1.w, s[h][1]))));
+          }
         }
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        s += __shfl_xor_sync(0xffffffffu, s, 2);
-        s += __shfl_xor_sync(0xffffffffu, s, 4);
-        if (row < 0) s = -INFINITY;
-        const float to = fmaxf(m[h], s), base = to == -INFINITY ? 0.f : to;
-        const float a = m[h] == -INFINITY ? 0.f : exp2f(m[h] - base), p = exp2f(s - base);
-        m[h] = to;
-        l[h] = fmaf(l[h], a, p);
+        float a[HEADS];
+#pragma unroll
+        for (int h = 0; h < HEADS; h++) {
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            s[h][u] += __shfl_xor_sync(0xffffffffu, s[h][u], 1);
+            s[h][u] += __shfl_xor_sync(0xffffffffu, s[h][u], 2);
+            s[h][u] += __shfl_xor_sync(0xffffffffu, s[h][u], 4);
+            if (!(seen[slot] >> (4 * u + tg) & 1)) s[h][u] = -INFINITY;
+          }
+          const float to = fmaxf(m[h], fmaxf(s[h][0], s[h][1])), base = to == -INFINITY ? 0.f : to;
+          a[h] = m[h] == -INFINITY ? 0.f : exp2f(m[h] - base);
+          s[h][0] = exp2f(s[h][0] - base);
+          s[h][1] = exp2f(s[h][1] - base);
+          m[h] = to;
+          l[h] = fmaf(l[h], a[h], s[h][0] + s[h][1]);
+        }
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-          o[h][v].x = fmaf(o[h][v].x, a, p * vr[v].x);
-          o[h][v].y = fmaf(o[h][v].y, a, p * vr[v].y);
-          o[h][v].z = fmaf(o[h][v].z, a, p * vr[v].z);
-          o[h][v].w = fmaf(o[h][v].w, a, p * vr[v].w);
+          const float4 v0 = row4(vs + v * 128), v1 = row4(vs + 4 * ROW + v * 128);
+#pragma unroll
+          for (int h = 0; h < HEADS; h++) {
+            o[h][v].x = fmaf(o[h][v].x, a[h], fmaf(s[h][0], v0.x, s[h][1] * v1.x));
+            o[h][v].y = fmaf(o[h][v].y, a[h], fmaf(s[h][0], v0.y, s[h][1] * v1.y));
+            o[h][v].z = fmaf(o[h][v].z, a[h], fmaf(s[h][0], v0.z, s[h][1] * v1.z));
+            o[h][v].w = fmaf(o[h][v].w, a[h], fmaf(s[h][0], v0.w, s[h][1] * v1.w));
+          }
         }
+        __syncwarp();  // the next fetch takes this slot
       }
     }
+    copies_wait<0>();
   }
+  __syncthreads();  // every warp is done with its ring
+  float* o_sh = reinterpret_cast<float*>(ring);
   // join the warp's four token groups
 #pragma unroll
   for (int h = 0; h < HEADS; h++) {
@@ -420,12 +501,15 @@ __global__ void __launch_bounds__(kThreads, 2) selected_f32_kernel(SelArgs g, in
   finish<float, HEADS, DT>(g, w, cluster, rank, o_sh, m_sh, l_sh);
 }
 
-zl_status launch(zl_ctx* ctx, void (*kernel)(SelArgs, int), const SelArgs& g, int64_t jobs, int cluster,
+zl_status launch(zl_ctx* ctx, void (*kernel)(SelArgs, int), size_t smem, const SelArgs& g, int64_t jobs, int cluster,
                  cudaStream_t st) {
   using namespace zl;
+  if (smem > 48 * 1024)
+    ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(jobs * cluster));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -459,17 +543,19 @@ zl_status launch_decode_selected_fast(zl_ctx* ctx, const void* q, const void* k_
   SelArgs g{q, k_pool, v_pool, block_tables, seq_lens, selected, out, H, Hkv, d, bs, max_blocks, max_selected,
             num_blocks, scale * 1.4426950408889634f, map == ZL_GQA_MODULO, group, subs, per_sub, ctx->d_status};
   const int64_t jobs = (int64_t)B * Hkv * subs;
-  // CTAs per list
+  // CTAs per list: as many as one wave of the GPU has room for (two to an SM), while each
+  // warp has a tile of its own
   const int64_t tokens = (int64_t)max_selected * bs;
   int cluster = 1;
-  while (cluster < 8 && jobs * cluster < 4 * ctx->num_sms && tokens / (2 * cluster) >= 128) cluster *= 2;
+  while (cluster < kMaxCluster && jobs * cluster <= ctx->num_sms && tokens >= cluster * 128) cluster *= 2;
   if (jobs * cluster > INT32_MAX) return ZL_ERR_UNSUPPORTED;
-  void (*kernel)(SelArgs, int);
   if (dtype == ZL_BF16)
-    kernel = d <= 64 ? selected_mma_kernel<64, 4> : d <= 128 ? selected_mma_kernel<128, 4> : selected_mma_kernel<256, 2>;
-  else
-    kernel = d <= 64 ? selected_f32_kernel<2, 4> : d <= 128 ? selected_f32_kernel<4, 4> : selected_f32_kernel<8, 2>;
-  return launch(ctx, kernel, g, jobs, cluster, st);
+    return d <= 64    ? launch(ctx, selected_mma_kernel<64, 4>, ring_bytes(128, 16, 4), g, jobs, cluster, st)
+           : d <= 128 ? launch(ctx, selected_mma_kernel<128, 3>, ring_bytes(256, 16, 3), g, jobs, cluster, st)
+                      : launch(ctx, selected_mma_kernel<256, 3>, ring_bytes(512, 16, 3), g, jobs, cluster, st);
+  return d <= 64    ? launch(ctx, selected_f32_kernel<2, 4, 4>, ring_bytes(256, 8, 4), g, jobs, cluster, st)
+         : d <= 128 ? launch(ctx, selected_f32_kernel<4, 4, 3>, ring_bytes(512, 8, 3), g, jobs, cluster, st)
+                    : launch(ctx, selected_f32_kernel<8, 2, 3>, ring_bytes(1024, 8, 3), g, jobs, cluster, st);
 }
 
 }  // namespace zl
