@@ -15,6 +15,7 @@
 // as attention over all blocks would be.
 #include "zl_internal.h"
 #include "zl_pages.h"
+#include "zl_ptx.cuh"
 
 namespace {
 
@@ -97,6 +98,109 @@ bounds_elem_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __r
   }
 }
 
+// Elementwise min and max of four 32-bit words of T, NaN where an operand is.
+template <typename T> __device__ __forceinline__ uint32_t word_min(uint32_t a, uint32_t b);
+template <typename T> __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t word_min<float>(uint32_t a, uint32_t b) {
+  return __float_as_uint(min_nan(__uint_as_float(a), __uint_as_float(b)));
+}
+template <> __device__ __forceinline__ uint32_t word_max<float>(uint32_t a, uint32_t b) {
+  return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+}
+template <> __device__ __forceinline__ uint32_t word_min<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t word_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void merge(uint4& lo, uint4& hi, const uint4& a, const uint4& b) {
+  lo.x = word_min<T>(lo.x, a.x);
+  lo.y = word_min<T>(lo.y, a.y);
+  lo.z = word_min<T>(lo.z, a.z);
+  lo.w = word_min<T>(lo.w, a.w);
+  hi.x = word_max<T>(hi.x, b.x);
+  hi.y = word_max<T>(hi.y, b.y);
+  hi.z = word_max<T>(hi.z, b.z);
+  hi.w = word_max<T>(hi.w, b.w);
+}
+
+// Rows of 16-byte chunks, up to 32 CH of them: one warp per block and kv head, LPR
+// lanes to a row (a power of two), CH chunks to a lane, 32 / LPR rows at a time and
+// eight such loads in flight. The lanes of all sequences' heads run through the
+// blocks together: head h of block j is unit j * Hkv + h, so a step that touches one
+// block per sequence keeps the warps of one CTA busy.
+template <typename T, int LPR, int CH>
+__global__ void __launch_bounds__(256, 4)
+bounds_vec_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __restrict__ tok_begin,
+                  T* __restrict__ bounds) {
+  constexpr int RPL = 32 / LPR, DEPTH = CH == 1 ? 8 : 4, VEC = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, sub = lane / LPR, ch = lane % LPR;
+  const int chunks = g.d / VEC;
+  for (int b = blockIdx.y; b < g.B; b += gridDim.y) {
+    const int64_t len = seq_len(g, b), n = zl::blocks_of(len, g.bs);
+    const int64_t first = tok_begin ? max(tok_begin[b], 0) / g.bs : 0;
+    for (int64_t u = first * g.Hkv + blockIdx.x * 8 + (threadIdx.x >> 5); u < n * g.Hkv; u += (int64_t)gridDim.x * 8) {
+      const int64_t j = u / g.Hkv;
+      const int h = (int)(u - j * g.Hkv);
+      const int64_t id = block_id(g, b, j);
+      if (id < 0) continue;
+      const uint4* rows = reinterpret_cast<const uint4*>(k_pool) + zl::pool_row(id, g.num_blocks, g.Hkv, h, g.bs, 0) * chunks;
+      const int toks = (int)min((int64_t)g.bs, len - j * g.bs);
+      uint4* out = reinterpret_cast<uint4*>(bounds) + (id * g.Hkv + h) * 2 * chunks;
+      uint4 lo[CH], hi[CH];
+      // every lane starts from a row of its own, or from row 0 where the block has fewer
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const int x = ch + c * LPR;
+        lo[c] = make_uint4(0, 0, 0, 0);
+        if (x < chunks) lo[c] = __ldg(rows + (int64_t)(sub < toks ? sub : 0) * chunks + x);
+        hi[c] = lo[c];
+      }
+      for (int t = RPL; t < toks; t += RPL * DEPTH) {
+        uint4 v[DEPTH][CH];
+#pragma unroll
+        for (int k = 0; k < DEPTH; k++)
+#pragma unroll
+          for (int c = 0; c < CH; c++) {
+            const int r = t + k * RPL + sub, x = ch + c * LPR;
+            v[k][c] = lo[c];  // no new row: merging lo into lo, and hi with it, changes nothing
+            if (r < toks && x < chunks) v[k][c] = __ldg(rows + (int64_t)r * chunks + x);
+          }
+#pragma unroll
+        for (int k = 0; k < DEPTH; k++)
+#pragma unroll
+          for (int c = 0; c < CH; c++) merge<T>(lo[c], hi[c], v[k][c], v[k][c]);
+      }
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+#pragma unroll
+        for (int o = LPR; o < 32; o <<= 1) {
+          uint4 a, z;
+          a.x = __shfl_xor_sync(0xffffffffu, lo[c].x, o);
+          a.y = __shfl_xor_sync(0xffffffffu, lo[c].y, o);
+          a.z = __shfl_xor_sync(0xffffffffu, lo[c].z, o);
+          a.w = __shfl_xor_sync(0xffffffffu, lo[c].w, o);
+          z.x = __shfl_xor_sync(0xffffffffu, hi[c].x, o);
+          z.y = __shfl_xor_sync(0xffffffffu, hi[c].y, o);
+          z.z = __shfl_xor_sync(0xffffffffu, hi[c].z, o);
+          z.w = __shfl_xor_sync(0xffffffffu, hi[c].w, o);
+          merge<T>(lo[c], hi[c], a, z);
+        }
+        const int x = ch + c * LPR;
+        if (x < chunks && sub == 0) {
+          out[x] = lo[c];
+          out[chunks + x] = hi[c];
+        }
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------- scores
 
 // One warp per (sequence, kv head, block), one element per lane and pass.
@@ -131,46 +235,288 @@ scores_elem_kernel(PagedArgs g, const T* __restrict__ q, const T* __restrict__ b
   }
 }
 
+// Bounds rows that 16-byte loads can read.
+//
+// bf16: a warp scores 16 blocks with matrix instructions: the blocks are M = 16, the
+// (at most 8) query heads N, and the 2 d products of a block's two rows with min(q, 0)
+// and max(q, 0) the sum. A lane loads 16 bytes of its two blocks' rows straight into
+// the operands of two steps of K = 16, q in the same order, all of a tile's loads
+// (8 KB at d = 128) in flight at once; products of bf16 are exact in fp32.
+template <int DT>
+__global__ void __launch_bounds__(256) scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
+                                                         const __nv_bfloat16* __restrict__ bounds, float scale,
+                                                         float* __restrict__ scores) {
+  constexpr int KC = DT / 32;
+  const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
+  const int group = g.H / g.Hkv;
+  const int64_t u = blockIdx.x / parts;
+  const int part = (int)(blockIdx.x - u * parts);
+  const int b = (int)(u / g.Hkv), h = (int)(u - (int64_t)b * g.Hkv);
+  uint4 x[KC];
+#pragma unroll
+  for (int k = 0; k < KC; k++) {
+    x[k] = make_uint4(0, 0, 0, 0);
+    if (n < group && k * 32 + c * 8 < g.d) {
+      const int head = g.modulo ? n * g.Hkv + h : h * group + n;
+      x[k] = __ldg(reinterpret_cast<const uint4*>(q + ((int64_t)b * g.H + head) * g.d + k * 32 + c * 8));
+    }
+  }
+  const int nb = (int)zl::blocks_of(seq_len(g, b), g.bs), tiles = (g.max_blocks + 15) / 16;
+  float* out = scores + u * g.max_blocks;
+  for (int tile = part * 8 + (threadIdx.x >> 5); tile < tiles; tile += parts * 8) {
+    uint4 v[2][2][KC];  // [row n, n + 8][lo, hi]
+    bool there[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const int j = tile * 16 + n + 8 * r;
+      const int64_t id = j < nb ? block_id(g, b, j) : -1;
+      there[r] = id >= 0;
+      const __nv_bfloat16* row = bounds + (there[r] ? (id * g.Hkv + h) * 2 * g.d : 0);
+#pragma unroll
+      for (int z = 0; z < 2; z++)
+#pragma unroll
+        for (int k = 0; k < KC; k++) {
+          v[r][z][k] = make_uint4(0, 0, 0, 0);
+          if (there[r] && k * 32 + c * 8 < g.d)
+            v[r][z][k] = __ldg(reinterpret_cast<const uint4*>(row + z * g.d + k * 32 + c * 8));
+        }
+    }
+    float s[2][4];
+#pragma unroll
+    for (int z = 0; z < 2; z++) {
+      s[z][0] = s[z][1] = s[z][2] = s[z][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KC; k++) {
+        auto side = [&](uint32_t a) { return z ? word_max<__nv_bfloat16>(a, 0u) : word_min<__nv_bfloat16>(a, 0u); };
+        zl::ptx::mma_bf16_16816(s[z], v[0][z][k].x, v[1][z][k].x, v[0][z][k].y, v[1][z][k].y, side(x[k].x), side(x[k].y));
+        zl::ptx::mma_bf16_16816(s[z], v[0][z][k].z, v[1][z][k].z, v[0][z][k].w, v[1][z][k].w, side(x[k].z), side(x[k].w));
+      }
+    }
+    // rows n and n + 8, heads 2 c and 2 c + 1
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      float best = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (2 * c + i < group) best = max_nan(best, (s[0][2 * r + i] + s[1][2 * r + i]) * scale);
+      best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 1));
+      best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 2));
+      const int j = tile * 16 + n + 8 * r;
+      if (c == r && j < g.max_blocks) out[j] = there[r] ? best : -INFINITY;
+    }
+  }
+}
+
+// fp32 (and bf16 with more than 8 query heads to a kv head): eight lanes share a
+// block's rows, a warp scores four blocks at a time on the CUDA cores; q's two sides
+// are in shared memory, 8 heads at a time.
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts, const T* __restrict__ q,
+                                                         const T* __restrict__ bounds, float scale,
+                                                         float* __restrict__ scores) {
+  constexpr int VEC = 16 / sizeof(T), DT = NV * 8 * VEC;
+  __shared__ __align__(16) float sides[2][8][DT];
+  const int lane = threadIdx.x & 31, tg = lane >> 3, li = lane & 7;
+  const int group = g.H / g.Hkv;
+  const int64_t u = blockIdx.x / parts;
+  const int part = (int)(blockIdx.x - u * parts);
+  const int b = (int)(u / g.Hkv), h = (int)(u - (int64_t)b * g.Hkv);
+  const int nb = (int)zl::blocks_of(seq_len(g, b), g.bs), tiles = (g.max_blocks + 3) / 4;
+  float* out = scores + u * g.max_blocks;
+  for (int h0 = 0; h0 < group; h0 += 8) {
+    const int heads = min(8, group - h0);
+    if (h0) __syncthreads();
+    for (int i = threadIdx.x; i < heads * DT; i += 256) {
+      const int k = i / DT, e = i - k * DT;
+      const int head = g.modulo ? (h0 + k) * g.Hkv + h : h * group + h0 + k;
+      const float f = e < g.d ? to_f(q[((int64_t)b * g.H + head) * g.d + e]) : 0.f;
+      sides[0][k][e] = min_nan(f, 0.f);
+      sides[1][k][e] = max_nan(f, 0.f);
+    }
+    __syncthreads();
+    for (int tile = part * 8 + (threadIdx.x >> 5); tile < tiles; tile += parts * 8) {
+      const int j = tile * 4 + tg;
+      const int64_t id = j < nb ? block_id(g, b, j) : -1;
+      uint4 v[2][NV];
+#pragma unroll
+      for (int z = 0; z < 2; z++)
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+          v[z][k] = make_uint4(0, 0, 0, 0);
+          if (id >= 0 && (k * 8 + li) * VEC < g.d)
+            v[z][k] = __ldg(reinterpret_cast<const uint4*>(bounds + ((id * g.Hkv + h) * 2 + z) * g.d + (k * 8 + li) * VEC));
+        }
+      float best = -INFINITY;
+      for (int i = 0; i < heads; i++) {
+        float s = 0.f;
+#pragma unroll
+        for (int z = 0; z < 2; z++)
+#pragma unroll
+          for (int k = 0; k < NV; k++) {
+            const T* e = reinterpret_cast<const T*>(&v[z][k]);
+            const float* f = &sides[z][i][(k * 8 + li) * VEC];
+#pragma unroll
+            for (int y = 0; y < VEC; y++) s = fmaf(f[y], to_f(e[y]), s);
+          }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        s += __shfl_xor_sync(0xffffffffu, s, 4);
+        best = max_nan(best, s * scale);
+      }
+      if (li == 0 && j < g.max_blocks) {
+        if (id < 0) best = -INFINITY;
+        out[j] = h0 ? max_nan(out[j], best) : best;
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- selection
 
 // The `top` blocks of one (sequence, kv head), ascending: the first `nf`, the
 // last `nl` and the best of those between, equal scores by the lower index.
 // With m = top - (nf + nl) still to choose from the middle, the threshold is
-// the largest key that at least m middle keys reach; it is found bit by bit by
-// counting, which needs no atomics and costs the same for every distribution
-// of the scores.
-constexpr int kSelThreads = 256;
+// the largest key that at least m middle keys reach; it is found from the top bit
+// down by counting, which needs no atomics and costs the same for every
+// distribution of the scores. A key's place in the output is the number of keys
+// above the threshold before it and of equal ones, of which the first few count.
+struct SelectArgs {
+  const float* scores;
+  const int32_t* seq_lens;
+  int32_t* selected;
+  int Hkv, max_blocks, bs, top, first, last;
+  int* status;
+};
+
+// The parts of a row that need no search; returns whether that was all. [lo, hi): the
+// middle blocks, of which m are to be chosen.
+template <int THREADS>
+__device__ __forceinline__ bool select_ends(const SelectArgs& g, int64_t row, int& lo, int& hi, int& m) {
+  const int tid = threadIdx.x;
+  int32_t* out = g.selected + row * g.top;
+  const int64_t want = zl::blocks_of(g.seq_lens[row / g.Hkv], g.bs);
+  if (want > g.max_blocks && tid == 0) atomicOr(g.status, ZL_DEV_OOB);
+  const int n = (int)min(want, (int64_t)g.max_blocks);
+  lo = g.first;
+  hi = n - g.last;
+  m = g.top - g.first - g.last;
+  if (n <= g.top) {
+    for (int j = tid; j < g.top; j += THREADS) out[j] = j < n ? j : -1;
+    return true;
+  }
+  // n > top >= first + last: the three parts do not meet
+  for (int j = tid; j < g.first; j += THREADS) out[j] = j;
+  for (int j = tid; j < g.last; j += THREADS) out[g.top - g.last + j] = hi + j;
+  return m == 0;
+}
+
+// Tables of up to THREADS R blocks: each thread keeps R keys, R <= 31, key i of
+// thread t being block i * THREADS + t. Two bits of the threshold a pass: the counts
+// for the three larger values of the next digit are summed over a warp as 10-bit
+// fields of one word.
+template <int THREADS, int R>
+__global__ void __launch_bounds__(THREADS) select_reg_kernel(SelectArgs g) {
+  constexpr int W = THREADS / 32;
+  __shared__ __align__(16) int4 part[2][W];
+  __shared__ uint32_t before[R * W];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x;
+  const float* sc = g.scores + row * g.max_blocks;
+  int32_t* out = g.selected + row * g.top;
+  uint32_t key[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) {  // loaded before the length is known
+    const int j = i * THREADS + tid;
+    key[i] = j < g.max_blocks ? __float_as_uint(__ldg(sc + j)) : 0;
+  }
+  int lo, hi, m;
+  if (select_ends<THREADS>(g, row, lo, hi, m)) return;
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int j = i * THREADS + tid;
+    key[i] = j >= lo && j < hi ? zl::score_key(key[i]) : 0;  // 0 is no score's key (-inf has 0x007fffff)
+  }
+  uint32_t limit = 0;
+  for (int bit = 30, p = 0; bit >= 0; bit -= 2, p ^= 1) {
+    const uint32_t c1 = limit | 1u << bit, c2 = limit | 2u << bit, c3 = limit | 3u << bit;
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < R; i++) c += (key[i] >= c1) + ((key[i] >= c2) << 10) + ((key[i] >= c3) << 20);
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) part[p][warp] = make_int4(c & 1023, c >> 10 & 1023, c >> 20, 0);
+    __syncthreads();
+    int s1 = 0, s2 = 0, s3 = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      const int4 x = part[p][w];
+      s1 += x.x;
+      s2 += x.y;
+      s3 += x.z;
+    }
+    if (s3 >= m) limit = c3;
+    else if (s2 >= m) limit = c2;
+    else if (s1 >= m) limit = c1;
+  }
+  // counts of each warp's keys above (low half) and at the limit (high half), by index order
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const uint32_t gt = __popc(__ballot_sync(0xffffffffu, key[i] > limit));
+    const uint32_t eq = __popc(__ballot_sync(0xffffffffu, key[i] == limit));
+    if (lane == 0) before[i * W + warp] = gt | eq << 16;
+  }
+  __syncthreads();
+  if (warp == 0) {  // exclusive sums of both halves; no total passes 31 * 1024
+    constexpr int PER = (R * W + 31) / 32;
+    uint32_t mine[PER], sum = 0;
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int at = lane * PER + k;
+      mine[k] = at < R * W ? before[at] : 0;
+      sum += mine[k];
+    }
+    uint32_t incl = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    uint32_t at = incl - sum;
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      if (lane * PER + k < R * W) before[lane * PER + k] = at;
+      at += mine[k];
+    }
+    if (lane == 31) part[0][0].x = (int)(incl & 0xffff);  // all keys above the limit
+  }
+  __syncthreads();
+  const int ties = m - part[0][0].x;
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const uint32_t gts = __ballot_sync(0xffffffffu, key[i] > limit), eqs = __ballot_sync(0xffffffffu, key[i] == limit);
+    const uint32_t below = (1u << lane) - 1, b = before[i * W + warp];
+    const int gt = (int)(b & 0xffff) + __popc(gts & below), eq = (int)(b >> 16) + __popc(eqs & below);
+    if (key[i] > limit || (key[i] == limit && eq < ties)) out[lo + gt + min(eq, ties)] = i * THREADS + tid;
+  }
+}
+
+// Longer tables: the keys are read again, from L2, in every pass.
+constexpr int kSelThreads = 1024;
 
 __device__ __forceinline__ int block_count(int c, int* red) {  // sum over the CTA, to every thread
   c = __reduce_add_sync(0xffffffffu, c);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = c;
   __syncthreads();
-  int s = 0;
-  for (int w = 0; w < kSelThreads / 32; w++) s += red[w];
-  return s;
+  return __reduce_add_sync(0xffffffffu, red[threadIdx.x & 31]);
 }
 
-__global__ void __launch_bounds__(kSelThreads)
-select_kernel(const float* __restrict__ scores, const int32_t* __restrict__ seq_lens, int Hkv, int max_blocks, int bs,
-              int top, int num_first, int num_last, int32_t* __restrict__ selected, int* status) {
+__global__ void __launch_bounds__(kSelThreads) select_kernel(SelectArgs g) {
   __shared__ int red[kSelThreads / 32];
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const float* sc = scores + row * max_blocks;
-  int32_t* out = selected + row * top;
-  const int64_t want = zl::blocks_of(seq_lens[row / Hkv], bs);
-  if (want > max_blocks && tid == 0) atomicOr(status, ZL_DEV_OOB);
-  const int n = (int)min(want, (int64_t)max_blocks);
-  if (n <= top) {
-    for (int j = tid; j < top; j += kSelThreads) out[j] = j < n ? j : -1;
-    return;
-  }
-  // n > top >= num_first + num_last: the three parts do not meet
-  const int lo = num_first, hi = n - num_last, m = top - num_first - num_last;
-  for (int j = tid; j < num_first; j += kSelThreads) out[j] = j;
-  for (int j = tid; j < num_last; j += kSelThreads) out[top - num_last + j] = hi + j;
-  if (m == 0) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float* sc = g.scores + row * g.max_blocks;
+  int32_t* out = g.selected + row * g.top;
+  int lo, hi, m;
+  if (select_ends<kSelThreads>(g, row, lo, hi, m)) return;
   auto key = [&](int j) { return zl::score_key(__float_as_uint(sc[j])); };
   uint32_t limit = 0;
   for (int bit = 31; bit >= 0; bit--) {
@@ -182,35 +528,22 @@ select_kernel(const float* __restrict__ scores, const int32_t* __restrict__ seq_
   int above = 0;
   for (int j = lo + tid; j < hi; j += kSelThreads) above += key(j) > limit;
   int ties = m - block_count(above, red);  // of the keys equal to the limit, the first so many
-  // write in index order: each pass handles one index per thread
-  int at = num_first;
-  for (int base = lo; base < hi; base += kSelThreads) {
-    const int j = base + tid;
-    const uint32_t kj = j < hi ? key(j) : 0;
-    const int eq = j < hi && kj == limit;
-    // equal keys before this one in the pass
-    const unsigned eqs = __ballot_sync(0xffffffffu, eq);
+  // write in index order, one index per thread and pass
+  int at = lo;
+  for (int64_t base = lo; base < hi; base += kSelThreads) {
+    const int64_t j = base + tid;
+    const uint32_t kj = j < hi ? key((int)j) : 0;
+    const unsigned gts = __ballot_sync(0xffffffffu, kj > limit), eqs = __ballot_sync(0xffffffffu, kj == limit);
     __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = __popc(eqs);
+    if (lane == 0) red[warp] = __popc(gts) | __popc(eqs) << 16;
     __syncthreads();
-    int before = __popc(eqs & ((1u << (tid & 31)) - 1)), all = 0;
-    for (int w = 0; w < kSelThreads / 32; w++) {
-      before += w < (tid >> 5) ? red[w] : 0;
-      all += red[w];
-    }
-    const int take = j < hi && (kj > limit || (eq && before < ties));
-    ties -= min(ties, all);
-    const unsigned takes = __ballot_sync(0xffffffffu, take);
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = __popc(takes);
-    __syncthreads();
-    int place = __popc(takes & ((1u << (tid & 31)) - 1)), total = 0;
-    for (int w = 0; w < kSelThreads / 32; w++) {
-      place += w < (tid >> 5) ? red[w] : 0;
-      total += red[w];
-    }
-    if (take) out[at + place] = j;
-    at += total;
+    const int mine = red[lane];
+    const int all = __reduce_add_sync(0xffffffffu, mine), pre = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+    const int gt = (pre & 0xffff) + __popc(gts & ((1u << lane) - 1)), eq = (pre >> 16) + __popc(eqs & ((1u << lane) - 1));
+    if (kj > limit || (j < hi && kj == limit && eq < ties)) out[at + gt + min(eq, ties)] = (int)j;
+    const int used = min(ties, all >> 16);
+    at += (all & 0xffff) + used;
+    ties -= used;
   }
 }
 
@@ -230,6 +563,34 @@ zl_status check_paged(const char* who, int B, int H, int Hkv, int d, int bs, int
 dim3 grid_of(int64_t units, int64_t blocks) {
   const int64_t y = units < 65535 ? units : 65535, x = (blocks + 7) / 8;
   return dim3((unsigned)(x < 1 ? 1 : x > 4096 ? 4096 : x), (unsigned)y);
+}
+
+template <typename T>
+void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* tok_begin, void* bounds, int num_sms,
+                       cudaStream_t st) {
+  const int chunks = g.d * (int)sizeof(T) / 16;
+  // Every block of long prompts, or the few that a step's tokens touched: with
+  // tok_begin the grid is one that an idle GPU starts at once, and its CTAs go on
+  // from block to block where there are more.
+  int64_t x = ((int64_t)g.max_blocks * g.Hkv + 7) / 8;
+  const int64_t few = (16 * (int64_t)num_sms + g.B - 1) / g.B;
+  if (tok_begin && x > few) x = few;
+  if (x > INT32_MAX) x = INT32_MAX;
+  const dim3 grid((unsigned)x, (unsigned)(g.B < 65535 ? g.B : 65535));
+  const T* k = (const T*)k_pool;
+  T* o = (T*)bounds;
+  if (chunks <= 8) bounds_vec_kernel<T, 8, 1><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
+  else if (chunks <= 16) bounds_vec_kernel<T, 16, 1><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
+  else if (chunks <= 32) bounds_vec_kernel<T, 32, 1><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
+  else bounds_vec_kernel<T, 32, 2><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
+}
+
+// CTAs of 8 warps for each of `rows` rows of `tiles` tiles: some 8 to an SM in all,
+// each warp then taking several tiles of long rows with one load of q.
+int scores_parts(int64_t rows, int64_t tiles, int num_sms) {
+  int64_t x = (8 * (int64_t)num_sms + rows - 1) / rows;
+  if (x > (tiles + 7) / 8) x = (tiles + 7) / 8;
+  return (int)(x < 1 ? 1 : x);
 }
 
 }  // namespace
@@ -252,12 +613,18 @@ zl_status zl_block_bounds(zl_ctx* ctx, const void* k_pool, const int32_t* block_
   if (dev.status != ZL_OK) return dev.status;
   PagedArgs g{block_tables, seq_lens, num_seqs, num_kv_heads, num_kv_heads, head_dim, block_size,
               max_blocks_per_seq, num_blocks, 0, ctx->d_status};
-  const dim3 grid = grid_of((int64_t)num_seqs * num_kv_heads, max_blocks_per_seq);
-  if (dtype == ZL_F32)
-    bounds_elem_kernel<float><<<grid, 256, 0, S(stream)>>>(g, (const float*)k_pool, tok_begin, (float*)bounds);
-  else
-    bounds_elem_kernel<__nv_bfloat16><<<grid, 256, 0, S(stream)>>>(g, (const __nv_bfloat16*)k_pool, tok_begin,
-                                                                   (__nv_bfloat16*)bounds);
+  const cudaStream_t st = S(stream);
+  if (head_dim * dtype_size(dtype) % 16 == 0 && head_dim <= 256 && aligned16(k_pool) && aligned16(bounds)) {
+    if (dtype == ZL_F32) launch_bounds_vec<float>(g, k_pool, tok_begin, bounds, ctx->num_sms, st);
+    else launch_bounds_vec<__nv_bfloat16>(g, k_pool, tok_begin, bounds, ctx->num_sms, st);
+  } else {
+    const dim3 grid = grid_of((int64_t)num_seqs * num_kv_heads, max_blocks_per_seq);
+    if (dtype == ZL_F32)
+      bounds_elem_kernel<float><<<grid, 256, 0, st>>>(g, (const float*)k_pool, tok_begin, (float*)bounds);
+    else
+      bounds_elem_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(g, (const __nv_bfloat16*)k_pool, tok_begin,
+                                                              (__nv_bfloat16*)bounds);
+  }
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }
@@ -276,13 +643,32 @@ zl_status zl_block_scores(zl_ctx* ctx, const void* q, const void* bounds, const 
   if (dev.status != ZL_OK) return dev.status;
   PagedArgs g{block_tables, seq_lens, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
               max_blocks_per_seq, num_blocks, gqa_map == ZL_GQA_MODULO, ctx->d_status};
-  const dim3 grid = grid_of((int64_t)num_seqs * num_kv_heads, max_blocks_per_seq);
   const float sc = resolve_scale(scale, head_dim);
-  if (dtype == ZL_F32)
-    scores_elem_kernel<float><<<grid, 256, 0, S(stream)>>>(g, (const float*)q, (const float*)bounds, sc, scores);
-  else
-    scores_elem_kernel<__nv_bfloat16><<<grid, 256, 0, S(stream)>>>(g, (const __nv_bfloat16*)q,
-                                                                   (const __nv_bfloat16*)bounds, sc, scores);
+  const cudaStream_t st = S(stream);
+  const int64_t rows = (int64_t)num_seqs * num_kv_heads;
+  const int p16 = scores_parts(rows, (max_blocks_per_seq + 15) / 16, ctx->num_sms),
+            p4 = scores_parts(rows, (max_blocks_per_seq + 3) / 4, ctx->num_sms);
+  const bool vec = head_dim * dtype_size(dtype) % 16 == 0 && head_dim <= 256 && aligned16(q) && aligned16(bounds) &&
+                   rows * p4 <= INT32_MAX;
+  const unsigned n16 = (unsigned)(rows * p16), n4 = (unsigned)(rows * p4);
+  const auto *qb = (const __nv_bfloat16*)q, *bb = (const __nv_bfloat16*)bounds;
+  const auto *qf = (const float*)q, *bf = (const float*)bounds;
+  if (vec && dtype == ZL_BF16 && num_heads / num_kv_heads <= 8) {
+    if (head_dim <= 64) scores_mma_kernel<64><<<n16, 256, 0, st>>>(g, p16, qb, bb, sc, scores);
+    else if (head_dim <= 128) scores_mma_kernel<128><<<n16, 256, 0, st>>>(g, p16, qb, bb, sc, scores);
+    else scores_mma_kernel<256><<<n16, 256, 0, st>>>(g, p16, qb, bb, sc, scores);
+  } else if (vec && dtype == ZL_BF16) {
+    if (head_dim <= 128) scores_vec_kernel<__nv_bfloat16, 2><<<n4, 256, 0, st>>>(g, p4, qb, bb, sc, scores);
+    else scores_vec_kernel<__nv_bfloat16, 4><<<n4, 256, 0, st>>>(g, p4, qb, bb, sc, scores);
+  } else if (vec) {
+    if (head_dim <= 64) scores_vec_kernel<float, 2><<<n4, 256, 0, st>>>(g, p4, qf, bf, sc, scores);
+    else if (head_dim <= 128) scores_vec_kernel<float, 4><<<n4, 256, 0, st>>>(g, p4, qf, bf, sc, scores);
+    else scores_vec_kernel<float, 8><<<n4, 256, 0, st>>>(g, p4, qf, bf, sc, scores);
+  } else {
+    const dim3 grid = grid_of(rows, max_blocks_per_seq);
+    if (dtype == ZL_F32) scores_elem_kernel<float><<<grid, 256, 0, st>>>(g, qf, bf, sc, scores);
+    else scores_elem_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(g, qb, bb, sc, scores);
+  }
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }
@@ -303,9 +689,15 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
     return set_error(ZL_ERR_INVALID_ARG, "select_blocks: null pointer");
   DeviceScope dev(ctx);
   if (dev.status != ZL_OK) return dev.status;
-  select_kernel<<<(unsigned)rows, kSelThreads, 0, S(stream)>>>(scores, seq_lens, num_kv_heads, max_blocks_per_seq,
-                                                               block_size, max_selected, num_first, num_last, selected,
-                                                               ctx->d_status);
+  const SelectArgs g{scores, seq_lens, selected, num_kv_heads, max_blocks_per_seq, block_size, max_selected,
+                     num_first, num_last, ctx->d_status};
+  const unsigned n = (unsigned)rows;
+  const cudaStream_t st = S(stream);
+  if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4><<<n, 128, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 2048) select_reg_kernel<256, 8><<<n, 256, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 8192) select_reg_kernel<512, 16><<<n, 512, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24><<<n, 1024, 0, st>>>(g);
+  else select_kernel<<<n, kSelThreads, 0, st>>>(g);
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }
