@@ -153,12 +153,12 @@ bounds_vec_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __re
       const int toks = (int)min((int64_t)g.bs, len - j * g.bs);
       uint4* out = reinterpret_cast<uint4*>(bounds) + (id * g.Hkv + h) * 2 * chunks;
       uint4 lo[CH], hi[CH];
-      // every lane starts from a row of its own, or from row 0 where the block has fewer
+      // every lane starts from a row of its own, or from the last where the block has fewer
 #pragma unroll
       for (int c = 0; c < CH; c++) {
         const int x = ch + c * LPR;
         lo[c] = make_uint4(0, 0, 0, 0);
-        if (x < chunks) lo[c] = __ldg(rows + (int64_t)(sub < toks ? sub : 0) * chunks + x);
+        if (x < chunks) lo[c] = __ldg(rows + (int64_t)min(sub, toks - 1) * chunks + x);
         hi[c] = lo[c];
       }
       for (int t = RPL; t < toks; t += RPL * DEPTH) {
@@ -167,9 +167,8 @@ bounds_vec_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __re
         for (int k = 0; k < DEPTH; k++)
 #pragma unroll
           for (int c = 0; c < CH; c++) {
-            const int r = t + k * RPL + sub, x = ch + c * LPR;
-            v[k][c] = lo[c];  // no new row: merging lo into lo, and hi with it, changes nothing
-            if (r < toks && x < chunks) v[k][c] = __ldg(rows + (int64_t)r * chunks + x);
+            const int r = min(t + k * RPL + sub, toks - 1), x = ch + c * LPR;  // a row twice changes nothing
+            v[k][c] = x < chunks ? __ldg(rows + (int64_t)r * chunks + x) : make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
         for (int k = 0; k < DEPTH; k++)
@@ -239,19 +238,61 @@ scores_elem_kernel(PagedArgs g, const T* __restrict__ q, const T* __restrict__ b
 //
 // bf16: a warp scores 16 blocks with matrix instructions: the blocks are M = 16, the
 // (at most 8) query heads N, and the 2 d products of a block's two rows with min(q, 0)
-// and max(q, 0) the sum. A lane loads 16 bytes of its two blocks' rows straight into
-// the operands of two steps of K = 16, q in the same order, all of a tile's loads
-// (8 KB at d = 128) in flight at once; products of bf16 are exact in fp32.
-template <int DT>
-__global__ void __launch_bounds__(256) scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
-                                                         const __nv_bfloat16* __restrict__ bounds, float scale,
-                                                         float* __restrict__ scores) {
-  constexpr int KC = DT / 32;
-  const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
+// and max(q, 0) the sum. A lane's 16 bytes of its two blocks' rows are its operands for
+// two steps of K = 16, q loaded in the same order; products of bf16 are exact in fp32.
+// Each warp keeps a ring of ST tiles (16 blocks' bounds) in shared memory, filled by
+// asynchronous copies, and the block ids of one tile more. Chunk ch of row r lies at
+// ch ^ swz(r), so that the two rows that a quarter warp reads do not meet in a bank.
+constexpr int kScoreWarps = 4;
+template <int DT, int ST>
+__global__ void __launch_bounds__(kScoreWarps * 32)
+scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
+                  const __nv_bfloat16* __restrict__ bounds, float scale, float* __restrict__ scores) {
+  constexpr int KC = DT / 32, CPR = DT / 4, ROW = DT * 4;  // a row: lo and hi side by side, DT elements each
+  extern __shared__ __align__(128) uint8_t ring[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   const int group = g.H / g.Hkv;
   const int64_t u = blockIdx.x / parts;
   const int part = (int)(blockIdx.x - u * parts);
   const int b = (int)(u / g.Hkv), h = (int)(u - (int64_t)b * g.Hkv);
+  const uint32_t mine = zl::ptx::smem_u32(ring) + warp * ST * 16 * ROW;
+  const int32_t* table = g.tables + (int64_t)b * g.max_blocks;
+  auto swz = [](int r) { return (r & 1) << 2 | (r >> 1 & 3); };
+  const int nb = (int)zl::blocks_of(seq_len(g, b), g.bs), tiles = (g.max_blocks + 15) / 16, some = (nb + 15) / 16;
+  const int t0 = part * kScoreWarps + warp, step = parts * kScoreWarps;
+  auto load_ids = [&](int tile) {  // lane i < 16: the id of the tile's block i
+    const int j = tile * 16 + lane;
+    return lane < 16 && j < nb ? table[j] : -1;
+  };
+  auto fetch = [&](int tile, int slot, int32_t id) {  // which of the 16 blocks there are
+    uint32_t there = 0;
+    if (tile < some) {
+      if (id >= g.num_blocks) {
+        atomicOr(g.status, ZL_DEV_OOB);
+        id = -1;
+      }
+      there = __ballot_sync(0xffffffffu, id >= 0);
+#pragma unroll
+      for (int it = 0; it < 16 * CPR / 32; it++) {
+        const int r = (it * 32 + lane) / CPR, ch = (it * 32 + lane) % CPR;
+        const int64_t from = __shfl_sync(0xffffffffu, id, r);
+        const int z = ch / (CPR / 2), e = (ch - z * (CPR / 2)) * 8;
+        const bool use = from >= 0 && e < g.d;
+        const __nv_bfloat16* src = bounds + (use ? ((from * g.Hkv + h) * 2 + z) * g.d + e : 0);
+        zl::ptx::copy16(mine + (slot * 16 + r) * ROW + (ch ^ swz(r)) * 16, src, use);
+      }
+    }
+    zl::ptx::copies_commit();
+    return there;
+  };
+  int32_t id = load_ids(t0);
+  uint32_t seen[ST];
+#pragma unroll
+  for (int i = 0; i < ST - 1; i++) {
+    const int32_t next = load_ids(t0 + (i + 1) * step);
+    seen[i] = fetch(t0 + i * step, i, id);
+    id = next;
+  }
   uint4 x[KC];
 #pragma unroll
   for (int k = 0; k < KC; k++) {
@@ -261,50 +302,49 @@ __global__ void __launch_bounds__(256) scores_mma_kernel(PagedArgs g, int parts,
       x[k] = __ldg(reinterpret_cast<const uint4*>(q + ((int64_t)b * g.H + head) * g.d + k * 32 + c * 8));
     }
   }
-  const int nb = (int)zl::blocks_of(seq_len(g, b), g.bs), tiles = (g.max_blocks + 15) / 16;
   float* out = scores + u * g.max_blocks;
-  for (int tile = part * 8 + (threadIdx.x >> 5); tile < tiles; tile += parts * 8) {
-    uint4 v[2][2][KC];  // [row n, n + 8][lo, hi]
-    bool there[2];
+  for (int tile = t0; tile < some;) {
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const int j = tile * 16 + n + 8 * r;
-      const int64_t id = j < nb ? block_id(g, b, j) : -1;
-      there[r] = id >= 0;
-      const __nv_bfloat16* row = bounds + (there[r] ? (id * g.Hkv + h) * 2 * g.d : 0);
+    for (int slot = 0; slot < ST; slot++, tile += step) {
+      if (tile >= some) break;
+      const int32_t next = load_ids(tile + ST * step);
+      seen[(slot + ST - 1) % ST] = fetch(tile + (ST - 1) * step, (slot + ST - 1) % ST, id);
+      id = next;
+      zl::ptx::copies_wait<ST - 1>();
+      __syncwarp();
+      const uint32_t rows = mine + (slot * 16 + n) * ROW;
+      float s[2][4];
 #pragma unroll
-      for (int z = 0; z < 2; z++)
+      for (int z = 0; z < 2; z++) {
+        s[z][0] = s[z][1] = s[z][2] = s[z][3] = 0.f;
 #pragma unroll
         for (int k = 0; k < KC; k++) {
-          v[r][z][k] = make_uint4(0, 0, 0, 0);
-          if (there[r] && k * 32 + c * 8 < g.d)
-            v[r][z][k] = __ldg(reinterpret_cast<const uint4*>(row + z * g.d + k * 32 + c * 8));
+          auto side = [&](uint32_t a) { return z ? word_max<__nv_bfloat16>(a, 0u) : word_min<__nv_bfloat16>(a, 0u); };
+          const uint32_t at = rows + ((z * (CPR / 2) + k * 4 + c) ^ swz(n)) * 16;  // swz(n + 8) is the same
+          const uint4 v = zl::ptx::lds16(at), w = zl::ptx::lds16(at + 8 * ROW);
+          zl::ptx::mma_bf16_16816(s[z], v.x, w.x, v.y, w.y, side(x[k].x), side(x[k].y));
+          zl::ptx::mma_bf16_16816(s[z], v.z, w.z, v.w, w.w, side(x[k].z), side(x[k].w));
         }
-    }
-    float s[2][4];
-#pragma unroll
-    for (int z = 0; z < 2; z++) {
-      s[z][0] = s[z][1] = s[z][2] = s[z][3] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KC; k++) {
-        auto side = [&](uint32_t a) { return z ? word_max<__nv_bfloat16>(a, 0u) : word_min<__nv_bfloat16>(a, 0u); };
-        zl::ptx::mma_bf16_16816(s[z], v[0][z][k].x, v[1][z][k].x, v[0][z][k].y, v[1][z][k].y, side(x[k].x), side(x[k].y));
-        zl::ptx::mma_bf16_16816(s[z], v[0][z][k].z, v[1][z][k].z, v[0][z][k].w, v[1][z][k].w, side(x[k].z), side(x[k].w));
       }
-    }
-    // rows n and n + 8, heads 2 c and 2 c + 1
+      // rows n and n + 8, heads 2 c and 2 c + 1
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-      float best = -INFINITY;
+      for (int r = 0; r < 2; r++) {
+        float best = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 2; i++)
-        if (2 * c + i < group) best = max_nan(best, (s[0][2 * r + i] + s[1][2 * r + i]) * scale);
-      best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 1));
-      best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 2));
-      const int j = tile * 16 + n + 8 * r;
-      if (c == r && j < g.max_blocks) out[j] = there[r] ? best : -INFINITY;
+        for (int i = 0; i < 2; i++)
+          if (2 * c + i < group) best = max_nan(best, (s[0][2 * r + i] + s[1][2 * r + i]) * scale);
+        best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 1));
+        best = max_nan(best, __shfl_xor_sync(0xffffffffu, best, 2));
+        const int j = tile * 16 + n + 8 * r;
+        if (c == r && j < g.max_blocks) out[j] = seen[slot] >> (n + 8 * r) & 1 ? best : -INFINITY;
+      }
+      __syncwarp();  // the next fetch takes this slot
     }
   }
+  zl::ptx::copies_wait<0>();
+  // after the sequence's last tile
+  for (int tile = some + t0; tile < tiles; tile += step)
+    if (lane < 16 && tile * 16 + lane < g.max_blocks) out[tile * 16 + lane] = -INFINITY;
 }
 
 // fp32 (and bf16 with more than 8 query heads to a kv head): eight lanes share a
@@ -410,32 +450,14 @@ __device__ __forceinline__ bool select_ends(const SelectArgs& g, int64_t row, in
   return m == 0;
 }
 
-// Tables of up to THREADS R blocks: each thread keeps R keys, R <= 31, key i of
-// thread t being block i * THREADS + t. Two bits of the threshold a pass: the counts
-// for the three larger values of the next digit are summed over a warp as 10-bit
-// fields of one word.
+// The threshold among keys in registers, by counting: two bits a pass, the counts for
+// the three larger values of the next digit being summed over a warp as 10-bit fields of
+// one word (R <= 31). No atomics; for few keys a thread.
 template <int THREADS, int R>
-__global__ void __launch_bounds__(THREADS) select_reg_kernel(SelectArgs g) {
+__device__ __forceinline__ uint32_t limit_by_counts(const uint32_t (&key)[R], int m) {
   constexpr int W = THREADS / 32;
   __shared__ __align__(16) int4 part[2][W];
-  __shared__ uint32_t before[R * W];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x;
-  const float* sc = g.scores + row * g.max_blocks;
-  int32_t* out = g.selected + row * g.top;
-  uint32_t key[R];
-#pragma unroll
-  for (int i = 0; i < R; i++) {  // loaded before the length is known
-    const int j = i * THREADS + tid;
-    key[i] = j < g.max_blocks ? __float_as_uint(__ldg(sc + j)) : 0;
-  }
-  int lo, hi, m;
-  if (select_ends<THREADS>(g, row, lo, hi, m)) return;
-#pragma unroll
-  for (int i = 0; i < R; i++) {
-    const int j = i * THREADS + tid;
-    key[i] = j >= lo && j < hi ? zl::score_key(key[i]) : 0;  // 0 is no score's key (-inf has 0x007fffff)
-  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t limit = 0;
   for (int bit = 30, p = 0; bit >= 0; bit -= 2, p ^= 1) {
     const uint32_t c1 = limit | 1u << bit, c2 = limit | 2u << bit, c3 = limit | 3u << bit;
@@ -457,6 +479,99 @@ __global__ void __launch_bounds__(THREADS) select_reg_kernel(SelectArgs g) {
     else if (s2 >= m) limit = c2;
     else if (s1 >= m) limit = c1;
   }
+  return limit;
+}
+
+// The same for many keys: three digits of 11, 11 and 10 bits, a histogram in shared
+// memory for each over the keys that share the digits before it. A warp whose keys all
+// fall into one bin adds them with one atomic.
+template <int THREADS, int R>
+__device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], int m) {
+  constexpr int BINS = 2048, PER = BINS / THREADS, W = THREADS / 32;
+  static_assert(PER * THREADS == BINS, "");
+  __shared__ int hist[BINS];
+  __shared__ int sums[W];
+  __shared__ int found[2];  // the digit, and how many keys of its bin are still to be chosen
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t limit = 0, mask = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; pass++) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
+#pragma unroll
+    for (int k = 0; k < PER; k++) hist[k * THREADS + tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const bool in = key[i] != 0 && (key[i] & mask) == limit;
+      const int bin = key[i] >> shift & ((1 << width) - 1);
+      const unsigned who = __ballot_sync(0xffffffffu, in);
+      if (!who) continue;
+      const int one = __shfl_sync(0xffffffffu, bin, __ffs(who) - 1);
+      if (__all_sync(0xffffffffu, !in || bin == one)) {
+        if (lane == 0) atomicAdd(&hist[one], __popc(who));
+      } else if (in) {
+        atomicAdd(&hist[bin], 1);
+      }
+    }
+    __syncthreads();
+    // sums from the top bin down: this thread has bins [top - PER + 1, top]
+    const int top = BINS - 1 - tid * PER;
+    int own = 0;
+#pragma unroll
+    for (int k = 0; k < PER; k++) own += hist[top - k];
+    int incl = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    const int s = lane < W ? sums[lane] : 0;
+    int above = incl - own + __reduce_add_sync(0xffffffffu, lane < warp ? s : 0);
+#pragma unroll
+    for (int k = 0; k < PER; k++) {  // one bin holds the m-th key from the top
+      const int c = hist[top - k];
+      if (above < m && m <= above + c) {
+        found[0] = top - k;
+        found[1] = m - above;
+      }
+      above += c;
+    }
+    __syncthreads();
+    limit |= (uint32_t)found[0] << shift;
+    m = found[1];
+    mask |= ((1u << width) - 1) << shift;
+  }
+  return limit;
+}
+
+// Tables of up to THREADS R blocks: each thread keeps R keys, key i of thread t being
+// block i * THREADS + t.
+template <int THREADS, int R, bool DIGITS>
+__global__ void __launch_bounds__(THREADS) select_reg_kernel(SelectArgs g) {
+  constexpr int W = THREADS / 32;
+  __shared__ uint32_t before[R * W];
+  __shared__ int total_above;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x;
+  const float* sc = g.scores + row * g.max_blocks;
+  int32_t* out = g.selected + row * g.top;
+  uint32_t key[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) {  // loaded before the length is known
+    const int j = i * THREADS + tid;
+    key[i] = j < g.max_blocks ? __float_as_uint(__ldg(sc + j)) : 0;
+  }
+  int lo, hi, m;
+  if (select_ends<THREADS>(g, row, lo, hi, m)) return;
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int j = i * THREADS + tid;
+    key[i] = j >= lo && j < hi ? zl::score_key(key[i]) : 0;  // 0 is no score's key (-inf has 0x007fffff)
+  }
+  uint32_t limit;
+  if constexpr (DIGITS) limit = limit_by_digits<THREADS, R>(key, m);
+  else limit = limit_by_counts<THREADS, R>(key, m);
   // counts of each warp's keys above (low half) and at the limit (high half), by index order
 #pragma unroll
   for (int i = 0; i < R; i++) {
@@ -485,10 +600,10 @@ __global__ void __launch_bounds__(THREADS) select_reg_kernel(SelectArgs g) {
       if (lane * PER + k < R * W) before[lane * PER + k] = at;
       at += mine[k];
     }
-    if (lane == 31) part[0][0].x = (int)(incl & 0xffff);  // all keys above the limit
+    if (lane == 31) total_above = (int)(incl & 0xffff);
   }
   __syncthreads();
-  const int ties = m - part[0][0].x;
+  const int ties = m - total_above;
 #pragma unroll
   for (int i = 0; i < R; i++) {
     const uint32_t gts = __ballot_sync(0xffffffffu, key[i] > limit), eqs = __ballot_sync(0xffffffffu, key[i] == limit);
@@ -585,12 +700,22 @@ void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* to
   else bounds_vec_kernel<T, 32, 2><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
 }
 
-// CTAs of 8 warps for each of `rows` rows of `tiles` tiles: some 8 to an SM in all,
-// each warp then taking several tiles of long rows with one load of q.
-int scores_parts(int64_t rows, int64_t tiles, int num_sms) {
-  int64_t x = (8 * (int64_t)num_sms + rows - 1) / rows;
-  if (x > (tiles + 7) / 8) x = (tiles + 7) / 8;
+// CTAs for each of `rows` rows of `tiles` tiles, `warps` tiles at a time: some `waves` CTAs
+// to an SM in all, each warp then taking several tiles of long rows with one load of q.
+int scores_parts(int64_t rows, int64_t tiles, int warps, int waves, int num_sms) {
+  int64_t x = (waves * (int64_t)num_sms + rows - 1) / rows;
+  if (x > (tiles + warps - 1) / warps) x = (tiles + warps - 1) / warps;
   return (int)(x < 1 ? 1 : x);
+}
+
+template <int DT, int ST>
+zl_status launch_scores_mma(const PagedArgs& g, int parts, unsigned grid, const __nv_bfloat16* q,
+                            const __nv_bfloat16* bounds, float scale, float* scores, cudaStream_t st) {
+  using namespace zl;
+  constexpr int smem = kScoreWarps * ST * 16 * DT * 4;
+  ZL_CUDA_TRY(cudaFuncSetAttribute(scores_mma_kernel<DT, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  scores_mma_kernel<DT, ST><<<grid, kScoreWarps * 32, smem, st>>>(g, parts, q, bounds, scale, scores);
+  return ZL_OK;
 }
 
 }  // namespace
@@ -646,17 +771,18 @@ zl_status zl_block_scores(zl_ctx* ctx, const void* q, const void* bounds, const 
   const float sc = resolve_scale(scale, head_dim);
   const cudaStream_t st = S(stream);
   const int64_t rows = (int64_t)num_seqs * num_kv_heads;
-  const int p16 = scores_parts(rows, (max_blocks_per_seq + 15) / 16, ctx->num_sms),
-            p4 = scores_parts(rows, (max_blocks_per_seq + 3) / 4, ctx->num_sms);
+  const int p16 = scores_parts(rows, (max_blocks_per_seq + 15) / 16, kScoreWarps, 6, ctx->num_sms),
+            p4 = scores_parts(rows, (max_blocks_per_seq + 3) / 4, 8, 8, ctx->num_sms);
   const bool vec = head_dim * dtype_size(dtype) % 16 == 0 && head_dim <= 256 && aligned16(q) && aligned16(bounds) &&
-                   rows * p4 <= INT32_MAX;
+                   rows * p4 <= INT32_MAX && rows * p16 <= INT32_MAX;
   const unsigned n16 = (unsigned)(rows * p16), n4 = (unsigned)(rows * p4);
   const auto *qb = (const __nv_bfloat16*)q, *bb = (const __nv_bfloat16*)bounds;
   const auto *qf = (const float*)q, *bf = (const float*)bounds;
   if (vec && dtype == ZL_BF16 && num_heads / num_kv_heads <= 8) {
-    if (head_dim <= 64) scores_mma_kernel<64><<<n16, 256, 0, st>>>(g, p16, qb, bb, sc, scores);
-    else if (head_dim <= 128) scores_mma_kernel<128><<<n16, 256, 0, st>>>(g, p16, qb, bb, sc, scores);
-    else scores_mma_kernel<256><<<n16, 256, 0, st>>>(g, p16, qb, bb, sc, scores);
+    s = head_dim <= 64    ? launch_scores_mma<64, 4>(g, p16, n16, qb, bb, sc, scores, st)
+        : head_dim <= 128 ? launch_scores_mma<128, 3>(g, p16, n16, qb, bb, sc, scores, st)
+                          : launch_scores_mma<256, 3>(g, p16, n16, qb, bb, sc, scores, st);
+    if (s != ZL_OK) return s;
   } else if (vec && dtype == ZL_BF16) {
     if (head_dim <= 128) scores_vec_kernel<__nv_bfloat16, 2><<<n4, 256, 0, st>>>(g, p4, qb, bb, sc, scores);
     else scores_vec_kernel<__nv_bfloat16, 4><<<n4, 256, 0, st>>>(g, p4, qb, bb, sc, scores);
@@ -693,10 +819,10 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
                      num_first, num_last, ctx->d_status};
   const unsigned n = (unsigned)rows;
   const cudaStream_t st = S(stream);
-  if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4><<<n, 128, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 2048) select_reg_kernel<256, 8><<<n, 256, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 8192) select_reg_kernel<512, 16><<<n, 512, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24><<<n, 1024, 0, st>>>(g);
+  if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4, false><<<n, 128, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 2048) select_reg_kernel<256, 8, false><<<n, 256, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 8192) select_reg_kernel<512, 16, true><<<n, 512, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24, true><<<n, 1024, 0, st>>>(g);
   else select_kernel<<<n, kSelThreads, 0, st>>>(g);
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;

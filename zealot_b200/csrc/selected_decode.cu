@@ -169,20 +169,6 @@ __device__ __forceinline__ void finish(const SelArgs& g, const Job& w, int clust
   if (cluster > 1) cl.sync();  // a CTA's shared memory stays until all have read it
 }
 
-// 16 bytes to shared memory in the background; zeros, and nothing read, where !use.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool use) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(use ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-
 // Starts the copies of one tile, TOK tokens' key rows and then their value rows of ROWB
 // bytes each (what is behind the real row_bytes is zeros, as are the rows of tokens that do
 // not count), as one group; an empty group where there is no such tile. Returns which tokens
@@ -209,11 +195,11 @@ __device__ __forceinline__ uint32_t fetch_tile(const SelArgs& g, const Entry* en
       const bool use = from >= 0 && ch * 16 < row_bytes;
       const int64_t at = use ? (int64_t)from * row_bytes + ch * 16 : 0;
       const uint32_t to = dst + r * ROWB + ((SWIZZLE ? ch ^ (r & 7) : ch) * 16);
-      copy16(to, (const uint8_t*)g.k_pool + at, use);
-      copy16(to + TOK * ROWB, (const uint8_t*)g.v_pool + at, use);
+      zl::ptx::copy16(to, (const uint8_t*)g.k_pool + at, use);
+      zl::ptx::copy16(to + TOK * ROWB, (const uint8_t*)g.v_pool + at, use);
     }
   }
-  copies_commit();
+  zl::ptx::copies_commit();
   return there;
 }
 
@@ -273,7 +259,7 @@ __global__ void __launch_bounds__(kThreads) selected_mma_kernel(SelArgs g, int c
       for (int slot = 0; slot < ST; slot++, tile += kWarps) {
         if (tile >= tiles) break;
         seen[(slot + ST - 1) % ST] = fetch(tile + (ST - 1) * kWarps, (slot + ST - 1) % ST);
-        copies_wait<ST - 1>();
+        zl::ptx::copies_wait<ST - 1>();
         __syncwarp();
         const uint32_t ks = mine + slot * 2 * TILE, vs = ks + TILE;
         float s[2][4];
@@ -284,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) selected_mma_kernel(SelArgs g, int c
           const int r = krow + i;
 #pragma unroll
           for (int k = 0; k < KC; k++) {
-            const uint4 x = lds16(ks + r * ROW + (((k * 4 + c) ^ (r & 7)) * 16));
+            const uint4 x = zl::ptx::lds16(ks + r * ROW + (((k * 4 + c) ^ (r & 7)) * 16));
             zl::ptx::mma_bf16_16816(s[i], q[k].x, 0, q[k].y, 0, x.x, x.y);
             zl::ptx::mma_bf16_16816(s2, q[k].z, 0, q[k].w, 0, x.z, x.w);
           }
@@ -337,7 +323,7 @@ __global__ void __launch_bounds__(kThreads) selected_mma_kernel(SelArgs g, int c
 #pragma unroll
             for (int x = 0; x < 2; x++) {
               const int t = vrow[x] + i;
-              const uint4 y = lds16(vs + t * ROW + (((a * 8 + n) ^ (t & 7)) * 16));
+              const uint4 y = zl::ptx::lds16(vs + t * ROW + (((a * 8 + n) ^ (t & 7)) * 16));
               r[2 * i + x][0] = y.x;
               r[2 * i + x][1] = y.y;
               r[2 * i + x][2] = y.z;
@@ -355,7 +341,7 @@ __global__ void __launch_bounds__(kThreads) selected_mma_kernel(SelArgs g, int c
         __syncwarp();  // the next fetch takes this slot
       }
     }
-    copies_wait<0>();
+    zl::ptx::copies_wait<0>();
   }
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -403,7 +389,7 @@ __global__ void __launch_bounds__(kThreads) selected_f32_kernel(SelArgs g, int c
     for (int v = 0; v < NV; v++) o[h][v] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   auto row4 = [](uint32_t a) {
-    const uint4 x = lds16(a);
+    const uint4 x = zl::ptx::lds16(a);
     return make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
   };
   for (int e = w.e0; e < w.e1; e += kEntries) {
@@ -421,7 +407,7 @@ __global__ void __launch_bounds__(kThreads) selected_f32_kernel(SelArgs g, int c
       for (int slot = 0; slot < ST; slot++, tile += kWarps) {
         if (tile >= tiles) break;
         seen[(slot + ST - 1) % ST] = fetch(tile + (ST - 1) * kWarps, (slot + ST - 1) % ST);
-        copies_wait<ST - 1>();
+        zl::ptx::copies_wait<ST - 1>();
         __syncwarp();
         // this lane's elements of rows tg and 4 + tg
         const uint32_t ks = mine + slot * 2 * TILE + tg * ROW + li * 16, vs = ks + TILE;
@@ -469,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) selected_f32_kernel(SelArgs g, int c
         __syncwarp();  // the next fetch takes this slot
       }
     }
-    copies_wait<0>();
+    zl::ptx::copies_wait<0>();
   }
   __syncthreads();  // every warp is done with its ring
   float* o_sh = reinterpret_cast<float*>(ring);
