@@ -144,10 +144,13 @@ bounds_vec_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __re
   for (int b = blockIdx.y; b < g.B; b += gridDim.y) {
     const int64_t len = seq_len(g, b), n = zl::blocks_of(len, g.bs);
     const int64_t first = tok_begin ? max(tok_begin[b], 0) / g.bs : 0;
-    for (int64_t u = first * g.Hkv + blockIdx.x * 8 + (threadIdx.x >> 5); u < n * g.Hkv; u += (int64_t)gridDim.x * 8) {
+    const int64_t step = (int64_t)gridDim.x * 8;
+    int64_t u = first * g.Hkv + blockIdx.x * 8 + (threadIdx.x >> 5);
+    int64_t id = u < n * g.Hkv ? block_id(g, b, u / g.Hkv) : -1, next;
+    for (; u < n * g.Hkv; u += step, id = next) {
       const int64_t j = u / g.Hkv;
       const int h = (int)(u - j * g.Hkv);
-      const int64_t id = block_id(g, b, j);
+      next = u + step < n * g.Hkv ? block_id(g, b, (u + step) / g.Hkv) : -1;
       if (id < 0) continue;
       const uint4* rows = reinterpret_cast<const uint4*>(k_pool) + zl::pool_row(id, g.num_blocks, g.Hkv, h, g.bs, 0) * chunks;
       const int toks = (int)min((int64_t)g.bs, len - j * g.bs);
@@ -243,18 +246,19 @@ scores_elem_kernel(PagedArgs g, const T* __restrict__ q, const T* __restrict__ b
 // Each warp keeps a ring of ST tiles (16 blocks' bounds) in shared memory, filled by
 // asynchronous copies, and the block ids of one tile more. Chunk ch of row r lies at
 // ch ^ swz(r), so that the two rows that a quarter warp reads do not meet in a bank.
-constexpr int kScoreWarps = 4;
+constexpr int kScoreWarps = 4, kScoreCtas = 3;
 template <int DT, int ST>
 __global__ void __launch_bounds__(kScoreWarps * 32)
 scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
                   const __nv_bfloat16* __restrict__ bounds, float scale, float* __restrict__ scores) {
-  constexpr int KC = DT / 32, CPR = DT / 4, ROW = DT * 4;  // a row: lo and hi side by side, DT elements each
+  constexpr int KC = DT / 32, ROW = DT * 4;  // a row: lo and hi side by side, DT elements each
+  constexpr int CPR = DT / 4;                // its 16-byte chunks
   extern __shared__ __align__(128) uint8_t ring[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   const int group = g.H / g.Hkv;
-  const int64_t u = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x - u * parts);
-  const int b = (int)(u / g.Hkv), h = (int)(u - (int64_t)b * g.Hkv);
+  // the heads of the same blocks, whose bounds lie side by side, run at the same time
+  const int h = (int)(blockIdx.x % g.Hkv), part = (int)(blockIdx.x / g.Hkv % parts), b = (int)(blockIdx.x / g.Hkv / parts);
+  const int64_t u = (int64_t)b * g.Hkv + h;
   const uint32_t mine = zl::ptx::smem_u32(ring) + warp * ST * 16 * ROW;
   const int32_t* table = g.tables + (int64_t)b * g.max_blocks;
   auto swz = [](int r) { return (r & 1) << 2 | (r >> 1 & 3); };
@@ -264,6 +268,11 @@ scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
     const int j = tile * 16 + lane;
     return lane < 16 && j < nb ? table[j] : -1;
   };
+  // copy `it` of a lane: chunk ch of the tile's row r; a row of 64 chunks takes two copies
+  const int z0 = lane % CPR / (CPR / 2), e0 = (lane % CPR - z0 * (CPR / 2)) * 8;
+  const bool used = e0 < g.d;
+  const uint8_t* mine_src = reinterpret_cast<const uint8_t*>(bounds + (used ? z0 * g.d + e0 : 0));
+  const int64_t row_bytes = 4 * g.d;
   auto fetch = [&](int tile, int slot, int32_t id) {  // which of the 16 blocks there are
     uint32_t there = 0;
     if (tile < some) {
@@ -272,13 +281,13 @@ scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
         id = -1;
       }
       there = __ballot_sync(0xffffffffu, id >= 0);
+      const int row = id < 0 ? -1 : id * g.Hkv + h;
 #pragma unroll
       for (int it = 0; it < 16 * CPR / 32; it++) {
         const int r = (it * 32 + lane) / CPR, ch = (it * 32 + lane) % CPR;
-        const int64_t from = __shfl_sync(0xffffffffu, id, r);
-        const int z = ch / (CPR / 2), e = (ch - z * (CPR / 2)) * 8;
-        const bool use = from >= 0 && e < g.d;
-        const __nv_bfloat16* src = bounds + (use ? ((from * g.Hkv + h) * 2 + z) * g.d + e : 0);
+        const int from = __shfl_sync(0xffffffffu, row, r);
+        const bool use = from >= 0 && used;
+        const uint8_t* src = mine_src + (use ? from : 0) * row_bytes + (CPR == 64 && it % 2 && used ? 2 * g.d : 0);
         zl::ptx::copy16(mine + (slot * 16 + r) * ROW + (ch ^ swz(r)) * 16, src, use);
       }
     }
@@ -358,9 +367,9 @@ __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts,
   __shared__ __align__(16) float sides[2][8][DT];
   const int lane = threadIdx.x & 31, tg = lane >> 3, li = lane & 7;
   const int group = g.H / g.Hkv;
-  const int64_t u = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x - u * parts);
-  const int b = (int)(u / g.Hkv), h = (int)(u - (int64_t)b * g.Hkv);
+  // the heads of the same blocks, whose bounds lie side by side, run at the same time
+  const int h = (int)(blockIdx.x % g.Hkv), part = (int)(blockIdx.x / g.Hkv % parts), b = (int)(blockIdx.x / g.Hkv / parts);
+  const int64_t u = (int64_t)b * g.Hkv + h;
   const int nb = (int)zl::blocks_of(seq_len(g, b), g.bs), tiles = (g.max_blocks + 3) / 4;
   float* out = scores + u * g.max_blocks;
   for (int h0 = 0; h0 < group; h0 += 8) {
@@ -680,6 +689,7 @@ dim3 grid_of(int64_t units, int64_t blocks) {
   return dim3((unsigned)(x < 1 ? 1 : x > 4096 ? 4096 : x), (unsigned)y);
 }
 
+constexpr int kBoundsWaves = 32;
 template <typename T>
 void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* tok_begin, void* bounds, int num_sms,
                        cudaStream_t st) {
@@ -688,8 +698,8 @@ void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* to
   // tok_begin the grid is one that an idle GPU starts at once, and its CTAs go on
   // from block to block where there are more.
   int64_t x = ((int64_t)g.max_blocks * g.Hkv + 7) / 8;
-  const int64_t few = (16 * (int64_t)num_sms + g.B - 1) / g.B;
-  if (tok_begin && x > few) x = few;
+  const int64_t few = ((tok_begin ? 4 : kBoundsWaves) * (int64_t)num_sms + g.B - 1) / g.B;
+  if (x > few) x = few;
   if (x > INT32_MAX) x = INT32_MAX;
   const dim3 grid((unsigned)x, (unsigned)(g.B < 65535 ? g.B : 65535));
   const T* k = (const T*)k_pool;
@@ -700,10 +710,11 @@ void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* to
   else bounds_vec_kernel<T, 32, 2><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
 }
 
-// CTAs for each of `rows` rows of `tiles` tiles, `warps` tiles at a time: some `waves` CTAs
-// to an SM in all, each warp then taking several tiles of long rows with one load of q.
-int scores_parts(int64_t rows, int64_t tiles, int warps, int waves, int num_sms) {
-  int64_t x = (waves * (int64_t)num_sms + rows - 1) / rows;
+// CTAs for each of `rows` rows of `tiles` tiles, `warps` tiles at a time: not more than
+// `ctas` in all where that leaves one for each row, each warp then taking several tiles of
+// long rows with one load of q.
+int scores_parts(int64_t rows, int64_t tiles, int warps, int64_t ctas) {
+  int64_t x = ctas / rows;
   if (x > (tiles + warps - 1) / warps) x = (tiles + warps - 1) / warps;
   return (int)(x < 1 ? 1 : x);
 }
@@ -771,17 +782,18 @@ zl_status zl_block_scores(zl_ctx* ctx, const void* q, const void* bounds, const 
   const float sc = resolve_scale(scale, head_dim);
   const cudaStream_t st = S(stream);
   const int64_t rows = (int64_t)num_seqs * num_kv_heads;
-  const int p16 = scores_parts(rows, (max_blocks_per_seq + 15) / 16, kScoreWarps, 6, ctx->num_sms),
-            p4 = scores_parts(rows, (max_blocks_per_seq + 3) / 4, 8, 8, ctx->num_sms);
+  const int p16 = scores_parts(rows, (max_blocks_per_seq + 15) / 16, kScoreWarps, kScoreCtas * ctx->num_sms),
+            p4 = scores_parts(rows, (max_blocks_per_seq + 3) / 4, 8, 8 * ctx->num_sms);
   const bool vec = head_dim * dtype_size(dtype) % 16 == 0 && head_dim <= 256 && aligned16(q) && aligned16(bounds) &&
-                   rows * p4 <= INT32_MAX && rows * p16 <= INT32_MAX;
+                   rows * p4 <= INT32_MAX && rows * p16 <= INT32_MAX &&
+                   (double)num_blocks * num_kv_heads <= INT32_MAX;
   const unsigned n16 = (unsigned)(rows * p16), n4 = (unsigned)(rows * p4);
   const auto *qb = (const __nv_bfloat16*)q, *bb = (const __nv_bfloat16*)bounds;
   const auto *qf = (const float*)q, *bf = (const float*)bounds;
   if (vec && dtype == ZL_BF16 && num_heads / num_kv_heads <= 8) {
     s = head_dim <= 64    ? launch_scores_mma<64, 4>(g, p16, n16, qb, bb, sc, scores, st)
-        : head_dim <= 128 ? launch_scores_mma<128, 3>(g, p16, n16, qb, bb, sc, scores, st)
-                          : launch_scores_mma<256, 3>(g, p16, n16, qb, bb, sc, scores, st);
+        : head_dim <= 128 ? launch_scores_mma<128, 2>(g, p16, n16, qb, bb, sc, scores, st)
+                          : launch_scores_mma<256, 2>(g, p16, n16, qb, bb, sc, scores, st);
     if (s != ZL_OK) return s;
   } else if (vec && dtype == ZL_BF16) {
     if (head_dim <= 128) scores_vec_kernel<__nv_bfloat16, 2><<<n4, 256, 0, st>>>(g, p4, qb, bb, sc, scores);
@@ -820,7 +832,7 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
   const unsigned n = (unsigned)rows;
   const cudaStream_t st = S(stream);
   if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4, false><<<n, 128, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 2048) select_reg_kernel<256, 8, false><<<n, 256, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 2048) select_reg_kernel<256, 8, true><<<n, 256, 0, st>>>(g);
   else if (max_blocks_per_seq <= 8192) select_reg_kernel<512, 16, true><<<n, 512, 0, st>>>(g);
   else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24, true><<<n, 1024, 0, st>>>(g);
   else select_kernel<<<n, kSelThreads, 0, st>>>(g);

@@ -121,6 +121,161 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(RopeArgs g) {
   }
 }
 
+// Four elements, as 8 (bf16) or 16 (fp32) bytes.
+struct Quad {
+  float x[4];
+};
+__device__ __forceinline__ Quad load4(const float* p) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  return {{v.x, v.y, v.z, v.w}};
+}
+__device__ __forceinline__ Quad load4(const __nv_bfloat16* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
+  return {{a.x, a.y, b.x, b.y}};
+}
+__device__ __forceinline__ void store4(float* p, const Quad& q) {
+  *reinterpret_cast<float4*>(p) = make_float4(q.x[0], q.x[1], q.x[2], q.x[3]);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const Quad& q) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(q.x[0], q.x[1]), b = __floats2bfloat162_rn(q.x[2], q.x[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// Rotates a lane's 8 elements by the angles of its pairs 4 u .. 4 u + 3.
+__device__ __forceinline__ void rotate(Quad& a, Quad& b, const float2* cs, bool interleaved) {
+  const float4 c01 = reinterpret_cast<const float4*>(cs)[0], c23 = reinterpret_cast<const float4*>(cs)[1];
+  const float c[4] = {c01.x, c01.z, c23.x, c23.z}, s[4] = {c01.y, c01.w, c23.y, c23.w};
+  if (interleaved) {  // pairs (a0, a1), (a2, a3), (b0, b1), (b2, b3)
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+      Quad& q = x < 2 ? a : b;
+      const int i = 2 * (x & 1);
+      const float y = q.x[i], z = q.x[i + 1];
+      q.x[i] = y * c[x] - z * s[x];
+      q.x[i + 1] = z * c[x] + y * s[x];
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+      const float y = a.x[x], z = b.x[x];
+      a.x[x] = y * c[x] - z * s[x];
+      b.x[x] = z * c[x] + y * s[x];
+    }
+  }
+}
+
+// head_dim and rotary_dim multiples of 8, rows that 4-element loads can read. HBM-bound
+// for many tokens. LG lanes (a power of two, at least d / 8) share a row; a lane has 8
+// elements of it, two runs of four: pairs 4 u .. 4 u + 3, whose elements lie in the two
+// halves of the rotated part (or, interleaved, side by side), so that a rotation needs no
+// exchange between lanes. A CTA takes `per` tokens: their angles, once for all heads, and
+// their cache rows go to shared memory. A lane group keeps to one head (of q, then k, then
+// v) over U tokens at a time, all of whose loads are in flight at once, with that head's
+// pointers and weight in registers; gridDim.y CTAs share the heads of few tokens.
+constexpr int kTokens = 8;
+template <typename T, int LG, int U>
+__global__ void __launch_bounds__(256) rope_vec_kernel(RopeArgs g, int per) {
+  __shared__ __align__(16) float2 cs[kTokens * kMaxDim / 2];
+  __shared__ int64_t cache[kTokens];  // row of kv head 0, -1 for none
+  constexpr int NG = 256 / LG;
+  const int tid = threadIdx.x, u = tid % LG;
+  const int64_t t0 = (int64_t)blockIdx.x * per;
+  const int tokens = (int)min((int64_t)per, g.tokens - t0), heads = g.H + 2 * g.Hkv;
+  const int half = g.rot / 2;
+  const bool mine = u * 8 < g.d, turned = u * 8 < g.rot;
+  const int e0 = turned && !g.interleaved ? 4 * u : 8 * u, e1 = turned && !g.interleaved ? half + 4 * u : 8 * u + 4;
+  bool angles = false;  // whether this CTA's angles are there
+  // every group of a CTA goes through the loop equally often (the barrier inside)
+  for (int h0 = blockIdx.y * NG; h0 < heads; h0 += gridDim.y * NG) {
+    const int h = h0 + tid / LG;
+    const bool isq = h < g.H, isk = !isq && h < g.H + g.Hkv;
+    const int hh = isq ? h : isk ? h - g.H : h - g.H - g.Hkv;
+    const int64_t stride = isq ? g.q_stride : isk ? g.k_stride : g.v_stride;
+    T* out = (T*)(isq ? g.q_out : isk ? g.k_out : g.v_out);
+    T* pool = (T*)(isq ? nullptr : isk ? g.k_pool : g.v_pool);
+    const T* w = (const T*)(isq ? g.q_weight : isk ? g.k_weight : nullptr);
+    const bool use = mine && h < heads && (out || pool);
+    const T* src = (const T*)(isq ? g.q : isk ? g.k : g.v) + (use ? t0 * stride + (int64_t)hh * g.d : 0);
+    const int64_t out_stride = (int64_t)(isq ? g.H : g.Hkv) * g.d;
+    if (out) out += t0 * out_stride + (int64_t)hh * g.d;
+    if (pool) pool += (int64_t)hh * g.bs * g.d;
+    for (int c0 = 0; c0 < tokens; c0 += U) {
+      Quad a[U], b[U];
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        a[k] = b[k] = {{0.f, 0.f, 0.f, 0.f}};
+        if (use && c0 + k < tokens) {
+          a[k] = load4(src + (c0 + k) * stride + e0);
+          b[k] = load4(src + (c0 + k) * stride + e1);
+        }
+      }
+      if (!angles) {  // while the first rows are on their way
+        for (int i = tid; i < tokens * half; i += 256) {
+          const int t = i / half;
+          cs[i] = turn(g.positions[t0 + t], g.inv_freq[i - t * half]);
+        }
+        if (tid < tokens) cache[tid] = cache_row(g, t0 + tid, 0);
+        __syncthreads();
+        angles = true;
+      }
+      Quad wa{}, wb{};
+      if (w && use) {
+        wa = load4(w + e0);
+        wb = load4(w + e1);
+      }
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        float ss = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) ss = fmaf(a[k].x[x], a[k].x[x], fmaf(b[k].x[x], b[k].x[x], ss));
+#pragma unroll
+        for (int o = LG / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (!use || c0 + k >= tokens) continue;
+        if (w) {
+          const float y = ss / g.d + g.eps, r = rsqrtf(y);
+          const float inv = r * fmaf(-0.5f * y * r, r, 1.5f);  // a Newton step: within half a step of fp32 or so
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            a[k].x[x] = a[k].x[x] * inv * wa.x[x];
+            b[k].x[x] = b[k].x[x] * inv * wb.x[x];
+          }
+        }
+        if ((isq || isk) && turned) rotate(a[k], b[k], &cs[(c0 + k) * half + 4 * u], g.interleaved);
+        if (out) {
+          store4(out + (c0 + k) * out_stride + e0, a[k]);
+          store4(out + (c0 + k) * out_stride + e1, b[k]);
+        }
+        if (pool && cache[c0 + k] >= 0) {
+          store4(pool + cache[c0 + k] * g.d + e0, a[k]);
+          store4(pool + cache[c0 + k] * g.d + e1, b[k]);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int LG>
+void launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
+  constexpr int NG = 256 / LG;
+  // one token to a CTA, and the heads over several, while there are few tokens
+  int64_t per = g.tokens / (4 * (int64_t)num_sms);
+  per = per < 1 ? 1 : per > kTokens ? kTokens : per;
+  const unsigned x = (unsigned)((g.tokens + per - 1) / per);
+  const unsigned y = per > 1 ? 1 : (unsigned)((g.H + 2 * g.Hkv + NG - 1) / NG);
+  const dim3 grid(x, y < 65535 ? y : 65535);
+  if (per >= 4) rope_vec_kernel<T, LG, 4><<<grid, 256, 0, st>>>(g, (int)per);
+  else rope_vec_kernel<T, LG, 1><<<grid, 256, 0, st>>>(g, (int)per);
+}
+
+template <typename T>
+void launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
+  if (g.d <= 64) launch_rope_vec<T, 8>(g, num_sms, st);
+  else if (g.d <= 128) launch_rope_vec<T, 16>(g, num_sms, st);
+  else launch_rope_vec<T, 32>(g, num_sms, st);
+}
+
 }  // namespace
 
 extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, const void* v, int64_t q_stride,
@@ -156,11 +311,22 @@ extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, 
   RopeArgs g{q, k, v, q_stride, k_stride, v_stride, q_weight, k_weight, eps, positions, inv_freq, rotary_dim,
              interleaved, q_out, k_out, v_out, k_pool, v_pool, k_pool ? slot_mapping : nullptr, block_size,
              num_blocks, num_tokens, num_heads, num_kv_heads, head_dim, ctx->d_status};
-  const int64_t units = num_tokens * (num_heads + 2 * (int64_t)num_kv_heads);
-  int64_t blocks = (units + 7) / 8;
-  if (blocks > (int64_t)ctx->num_sms * 32) blocks = (int64_t)ctx->num_sms * 32;
-  if (dtype == ZL_F32) rope_elem_kernel<float><<<(unsigned)blocks, 256, 0, S(stream)>>>(g);
-  else rope_elem_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, S(stream)>>>(g);
+  const size_t quad = 4 * dtype_size(dtype);
+  auto fits = [quad](const void* p) { return reinterpret_cast<uintptr_t>(p) % quad == 0; };
+  const bool vec = head_dim % 8 == 0 && rotary_dim % 8 == 0 && fits(q) && fits(k) && fits(v) && fits(q_out) &&
+                   fits(k_out) && fits(v_out) && fits(k_pool) && fits(v_pool) &&
+                   (num_tokens == 1 || (q_stride % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0)) &&
+                   num_tokens <= INT32_MAX && (num_heads + 2 * (int64_t)num_kv_heads) <= 1 << 20;
+  if (vec) {
+    if (dtype == ZL_F32) launch_rope_vec<float>(g, ctx->num_sms, S(stream));
+    else launch_rope_vec<__nv_bfloat16>(g, ctx->num_sms, S(stream));
+  } else {
+    const int64_t units = num_tokens * (num_heads + 2 * (int64_t)num_kv_heads);
+    int64_t blocks = (units + 7) / 8;
+    if (blocks > (int64_t)ctx->num_sms * 32) blocks = (int64_t)ctx->num_sms * 32;
+    if (dtype == ZL_F32) rope_elem_kernel<float><<<(unsigned)blocks, 256, 0, S(stream)>>>(g);
+    else rope_elem_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, S(stream)>>>(g);
+  }
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }
