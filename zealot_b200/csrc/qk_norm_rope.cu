@@ -16,6 +16,7 @@
 // off by 0.06 radians.
 #include "zl_internal.h"
 #include "zl_pages.h"
+#include "zl_ptx.cuh"
 
 namespace {
 
@@ -34,6 +35,7 @@ struct RopeArgs {
   int bs;
   int64_t num_blocks, tokens;
   int H, Hkv, d;
+  float inv_d;
   int* status;
 };
 
@@ -166,114 +168,197 @@ __device__ __forceinline__ void rotate(Quad& a, Quad& b, const float2* cs, bool 
   }
 }
 
-// head_dim and rotary_dim multiples of 8, rows that 4-element loads can read. HBM-bound
-// for many tokens. LG lanes (a power of two, at least d / 8) share a row; a lane has 8
-// elements of it, two runs of four: pairs 4 u .. 4 u + 3, whose elements lie in the two
-// halves of the rotated part (or, interleaved, side by side), so that a rotation needs no
-// exchange between lanes. A CTA takes `per` tokens: their angles, once for all heads, and
-// their cache rows go to shared memory. A lane group keeps to one head (of q, then k, then
-// v) over U tokens at a time, all of whose loads are in flight at once, with that head's
-// pointers and weight in registers; gridDim.y CTAs share the heads of few tokens.
-constexpr int kTokens = 8;
-template <typename T, int LG, int U>
-__global__ void __launch_bounds__(256) rope_vec_kernel(RopeArgs g, int per) {
-  __shared__ __align__(16) float2 cs[kTokens * kMaxDim / 2];
-  __shared__ int64_t cache[kTokens];  // row of kv head 0, -1 for none
-  constexpr int NG = 256 / LG;
-  const int tid = threadIdx.x, u = tid % LG;
-  const int64_t t0 = (int64_t)blockIdx.x * per;
-  const int tokens = (int)min((int64_t)per, g.tokens - t0), heads = g.H + 2 * g.Hkv;
-  const int half = g.rot / 2;
-  const bool mine = u * 8 < g.d, turned = u * 8 < g.rot;
-  const int e0 = turned && !g.interleaved ? 4 * u : 8 * u, e1 = turned && !g.interleaved ? half + 4 * u : 8 * u + 4;
-  bool angles = false;  // whether this CTA's angles are there
-  // every group of a CTA goes through the loop equally often (the barrier inside)
-  for (int h0 = blockIdx.y * NG; h0 < heads; h0 += gridDim.y * NG) {
-    const int h = h0 + tid / LG;
+// head_dim and rotary_dim multiples of 8, rows that 4-element loads can read. LG lanes (a
+// power of two, at least d / 8) share a row; a lane has 8 elements of it, two runs of four:
+// pairs 4 u .. 4 u + 3, whose elements lie in the two halves of the rotated part (or,
+// interleaved, side by side), so that a rotation needs no exchange between lanes. A CTA takes
+// `per` tokens; their angles, once for all heads, and their cache rows go to shared memory.
+// A lane group keeps to one head (of q, then k, then v) over all its tokens, then takes the
+// next. HeadRows is that head: where its rows come from and go to.
+template <typename T>
+struct HeadRows {
+  const T* src;  // this lane's group's row of the CTA's first token
+  T *out, *pool;
+  const T* w;
+  int64_t stride, out_stride;
+  bool use, turn;
+  __device__ __forceinline__ HeadRows(const RopeArgs& g, int h, int64_t t0, bool mine, bool turned) {
     const bool isq = h < g.H, isk = !isq && h < g.H + g.Hkv;
     const int hh = isq ? h : isk ? h - g.H : h - g.H - g.Hkv;
-    const int64_t stride = isq ? g.q_stride : isk ? g.k_stride : g.v_stride;
-    T* out = (T*)(isq ? g.q_out : isk ? g.k_out : g.v_out);
-    T* pool = (T*)(isq ? nullptr : isk ? g.k_pool : g.v_pool);
-    const T* w = (const T*)(isq ? g.q_weight : isk ? g.k_weight : nullptr);
-    const bool use = mine && h < heads && (out || pool);
-    const T* src = (const T*)(isq ? g.q : isk ? g.k : g.v) + (use ? t0 * stride + (int64_t)hh * g.d : 0);
-    const int64_t out_stride = (int64_t)(isq ? g.H : g.Hkv) * g.d;
+    out = (T*)(isq ? g.q_out : isk ? g.k_out : g.v_out);
+    pool = (T*)(isq ? nullptr : isk ? g.k_pool : g.v_pool);
+    w = (const T*)(isq ? g.q_weight : isk ? g.k_weight : nullptr);
+    use = mine && h < g.H + 2 * g.Hkv && (out || pool);
+    turn = turned && (isq || isk);
+    stride = isq ? g.q_stride : isk ? g.k_stride : g.v_stride;
+    out_stride = (int64_t)(isq ? g.H : g.Hkv) * g.d;
+    src = (const T*)(isq ? g.q : isk ? g.k : g.v);
+    if (use) src += t0 * stride + (int64_t)hh * g.d;
     if (out) out += t0 * out_stride + (int64_t)hh * g.d;
     if (pool) pool += (int64_t)hh * g.bs * g.d;
-    for (int c0 = 0; c0 < tokens; c0 += U) {
-      Quad a[U], b[U];
+  }
+};
+
+template <typename T, int LG>
+struct Lane {  // a lane's place in its row
+  int u, e0, e1;
+  bool mine, turned;
+  __device__ __forceinline__ explicit Lane(const RopeArgs& g) {
+    u = threadIdx.x % LG;
+    mine = u * 8 < g.d;
+    turned = u * 8 < g.rot;
+    const bool halves = turned && !g.interleaved;
+    e0 = halves ? 4 * u : 8 * u;
+    e1 = halves ? g.rot / 2 + 4 * u : 8 * u + 4;
+  }
+};
+
+// Norms and rotates one row and stores it: token c of the CTA, whose angles are cs and
+// whose pool rows start at element `at` (-1: none).
+template <typename T, int LG>
+__device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<T, LG>& ln, const HeadRows<T>& r, int c,
+                                           Quad a, Quad b, const float2* cs, int64_t at) {
+  float ss = 0.f, s2 = 0.f;
 #pragma unroll
-      for (int k = 0; k < U; k++) {
-        a[k] = b[k] = {{0.f, 0.f, 0.f, 0.f}};
-        if (use && c0 + k < tokens) {
-          a[k] = load4(src + (c0 + k) * stride + e0);
-          b[k] = load4(src + (c0 + k) * stride + e1);
-        }
-      }
-      if (!angles) {  // while the first rows are on their way
-        for (int i = tid; i < tokens * half; i += 256) {
-          const int t = i / half;
-          cs[i] = turn(g.positions[t0 + t], g.inv_freq[i - t * half]);
-        }
-        if (tid < tokens) cache[tid] = cache_row(g, t0 + tid, 0);
-        __syncthreads();
-        angles = true;
-      }
-      Quad wa{}, wb{};
-      if (w && use) {
-        wa = load4(w + e0);
-        wb = load4(w + e1);
-      }
+  for (int x = 0; x < 4; x++) {
+    ss = fmaf(a.x[x], a.x[x], ss);
+    s2 = fmaf(b.x[x], b.x[x], s2);
+  }
+  ss += s2;
 #pragma unroll
-      for (int k = 0; k < U; k++) {
-        float ss = 0.f;
+  for (int o = LG / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (!r.use) return;
+  if (r.w) {
+    const Quad wa = load4(r.w + ln.e0), wb = load4(r.w + ln.e1);
+    const float y = ss * g.inv_d + g.eps, q = rsqrtf(y);
+    const float inv = q * fmaf(-0.5f * y * q, q, 1.5f);  // a Newton step: right to fp32's last place or so
 #pragma unroll
-        for (int x = 0; x < 4; x++) ss = fmaf(a[k].x[x], a[k].x[x], fmaf(b[k].x[x], b[k].x[x], ss));
-#pragma unroll
-        for (int o = LG / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!use || c0 + k >= tokens) continue;
-        if (w) {
-          const float y = ss / g.d + g.eps, r = rsqrtf(y);
-          const float inv = r * fmaf(-0.5f * y * r, r, 1.5f);  // a Newton step: within half a step of fp32 or so
-#pragma unroll
-          for (int x = 0; x < 4; x++) {
-            a[k].x[x] = a[k].x[x] * inv * wa.x[x];
-            b[k].x[x] = b[k].x[x] * inv * wb.x[x];
-          }
-        }
-        if ((isq || isk) && turned) rotate(a[k], b[k], &cs[(c0 + k) * half + 4 * u], g.interleaved);
-        if (out) {
-          store4(out + (c0 + k) * out_stride + e0, a[k]);
-          store4(out + (c0 + k) * out_stride + e1, b[k]);
-        }
-        if (pool && cache[c0 + k] >= 0) {
-          store4(pool + cache[c0 + k] * g.d + e0, a[k]);
-          store4(pool + cache[c0 + k] * g.d + e1, b[k]);
-        }
-      }
+    for (int x = 0; x < 4; x++) {
+      a.x[x] = a.x[x] * inv * wa.x[x];
+      b.x[x] = b.x[x] * inv * wb.x[x];
     }
+  }
+  if (r.turn) rotate(a, b, cs + 4 * ln.u, g.interleaved);
+  if (r.out) {
+    T* to = r.out + c * r.out_stride;
+    store4(to + ln.e0, a);
+    store4(to + ln.e1, b);
+  }
+  if (r.pool && at >= 0) {
+    store4(r.pool + at + ln.e0, a);
+    store4(r.pool + at + ln.e1, b);
   }
 }
 
+// The CTA's angles and, in elements, the pool rows of its tokens' kv head 0.
+__device__ __forceinline__ void token_tables(const RopeArgs& g, int64_t t0, int tokens, float2* cs, int64_t* cache) {
+  const int half = g.rot / 2;
+  for (int i = threadIdx.x; i < tokens * half; i += 256) {
+    const int t = i / half;
+    cs[i] = turn(g.positions[t0 + t], g.inv_freq[i - t * half]);
+  }
+  if (threadIdx.x < tokens) {
+    const int64_t row = cache_row(g, t0 + threadIdx.x, 0);
+    cache[threadIdx.x] = row < 0 ? -1 : row * g.d;
+  }
+}
+
+// Few tokens: one to a CTA, and its heads over gridDim.y of them.
 template <typename T, int LG>
-void launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
+__global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
+  __shared__ __align__(16) float2 cs[kMaxDim / 2];
+  __shared__ int64_t cache[1];
+  const Lane<T, LG> ln(g);
+  const int64_t t0 = blockIdx.x;
+  bool tables = false;
+  // every group of a CTA goes through the loop equally often (the barrier inside)
+  for (int h0 = blockIdx.y * (256 / LG); h0 < g.H + 2 * g.Hkv; h0 += gridDim.y * (256 / LG)) {
+    const HeadRows<T> r(g, h0 + threadIdx.x / LG, t0, ln.mine, ln.turned);
+    Quad a{}, b{};
+    if (r.use) {
+      a = load4(r.src + ln.e0);
+      b = load4(r.src + ln.e1);
+    }
+    if (!tables) {  // while the row is on its way
+      token_tables(g, t0, 1, cs, cache);
+      __syncthreads();
+      tables = true;
+    }
+    finish_row(g, ln, r, 0, a, b, cs, cache[0]);
+  }
+}
+
+// Many tokens: HBM-bound. Every thread copies its own two runs of the rows that it will need
+// kAhead steps from now into its own slots of shared memory, in the background: bytes on their
+// way without registers, and without a barrier, since each thread waits for its own.
+constexpr int kTokens = 16, kAhead = 8;
+template <typename T, int LG>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) rope_tokens_kernel(RopeArgs g, int per) {
+  constexpr int RUN = 4 * sizeof(T);
+  extern __shared__ __align__(16) uint8_t dyn[];  // [kAhead][256][2 RUN], then the angles
+  __shared__ int64_t cache[kTokens];
+  float2* cs = reinterpret_cast<float2*>(dyn + kAhead * 256 * 2 * RUN);
+  const Lane<T, LG> ln(g);
+  const int64_t t0 = (int64_t)blockIdx.x * per;
+  const int tokens = (int)min((int64_t)per, g.tokens - t0), half = g.rot / 2, group = threadIdx.x / LG;
+  const int blocks = (g.H + 2 * g.Hkv + 256 / LG - 1) / (256 / LG), steps = blocks * tokens;
+  const uint32_t slots = zl::ptx::smem_u32(dyn) + threadIdx.x * 2 * RUN;
+  HeadRows<T> ahead(g, group, t0, ln.mine, ln.turned), r = ahead;
+  int hb = 0, c2 = 0;  // head block and token of the next copy
+  auto fetch = [&](int slot) {
+    if (hb < blocks && ahead.use) {
+      const uint32_t to = slots + slot * 256 * 2 * RUN;
+      zl::ptx::copy_async<RUN>(to, ahead.src + ln.e0);
+      zl::ptx::copy_async<RUN>(to + RUN, ahead.src + ln.e1);
+    }
+    zl::ptx::copies_commit();
+    ahead.src += ahead.stride;
+    if (++c2 == tokens) {
+      c2 = 0;
+      if (++hb < blocks) ahead = HeadRows<T>(g, hb * (256 / LG) + group, t0, ln.mine, ln.turned);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead - 1; i++) fetch(i);
+  token_tables(g, t0, tokens, cs, cache);
+  __syncthreads();
+  for (int s = 0, h = 0, c = 0; s < steps; s++) {
+    fetch((s + kAhead - 1) % kAhead);
+    zl::ptx::copies_wait<kAhead - 1>();
+    const T* slot = reinterpret_cast<const T*>(dyn + ((s % kAhead) * 256 + threadIdx.x) * 2 * RUN);
+    finish_row(g, ln, r, c, load4(slot), load4(slot + 4), cs + c * half, cache[c]);
+    if (++c == tokens) {
+      c = 0;
+      h++;
+      r = HeadRows<T>(g, h * (256 / LG) + group, t0, ln.mine, ln.turned);
+    }
+  }
+  zl::ptx::copies_wait<0>();
+}
+
+template <typename T, int LG>
+zl_status launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
+  using namespace zl;
   constexpr int NG = 256 / LG;
-  // one token to a CTA, and the heads over several, while there are few tokens
   int64_t per = g.tokens / (4 * (int64_t)num_sms);
-  per = per < 1 ? 1 : per > kTokens ? kTokens : per;
-  const unsigned x = (unsigned)((g.tokens + per - 1) / per);
-  const unsigned y = per > 1 ? 1 : (unsigned)((g.H + 2 * g.Hkv + NG - 1) / NG);
-  const dim3 grid(x, y < 65535 ? y : 65535);
-  if (per >= 4) rope_vec_kernel<T, LG, 4><<<grid, 256, 0, st>>>(g, (int)per);
-  else rope_vec_kernel<T, LG, 1><<<grid, 256, 0, st>>>(g, (int)per);
+  if (per < 4) {
+    const unsigned y = (unsigned)((g.H + 2 * g.Hkv + NG - 1) / NG);
+    rope_token_kernel<T, LG><<<dim3((unsigned)g.tokens, y < 65535 ? y : 65535), 256, 0, st>>>(g);
+    return ZL_OK;
+  }
+  if (per > kTokens) per = kTokens;
+  const size_t smem = (size_t)kAhead * 256 * 8 * sizeof(T) + per * (g.rot / 2) * sizeof(float2);
+  if (smem > 48 * 1024)
+    ZL_CUDA_TRY(cudaFuncSetAttribute(rope_tokens_kernel<T, LG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  rope_tokens_kernel<T, LG><<<(unsigned)((g.tokens + per - 1) / per), 256, smem, st>>>(g, (int)per);
+  return ZL_OK;
 }
 
 template <typename T>
-void launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
-  if (g.d <= 64) launch_rope_vec<T, 8>(g, num_sms, st);
-  else if (g.d <= 128) launch_rope_vec<T, 16>(g, num_sms, st);
-  else launch_rope_vec<T, 32>(g, num_sms, st);
+zl_status launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
+  return g.d <= 64    ? launch_rope_vec<T, 8>(g, num_sms, st)
+         : g.d <= 128 ? launch_rope_vec<T, 16>(g, num_sms, st)
+                      : launch_rope_vec<T, 32>(g, num_sms, st);
 }
 
 }  // namespace
@@ -310,7 +395,7 @@ extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, 
   if (dev.status != ZL_OK) return dev.status;
   RopeArgs g{q, k, v, q_stride, k_stride, v_stride, q_weight, k_weight, eps, positions, inv_freq, rotary_dim,
              interleaved, q_out, k_out, v_out, k_pool, v_pool, k_pool ? slot_mapping : nullptr, block_size,
-             num_blocks, num_tokens, num_heads, num_kv_heads, head_dim, ctx->d_status};
+             num_blocks, num_tokens, num_heads, num_kv_heads, head_dim, 1.f / head_dim, ctx->d_status};
   const size_t quad = 4 * dtype_size(dtype);
   auto fits = [quad](const void* p) { return reinterpret_cast<uintptr_t>(p) % quad == 0; };
   const bool vec = head_dim % 8 == 0 && rotary_dim % 8 == 0 && fits(q) && fits(k) && fits(v) && fits(q_out) &&
@@ -318,8 +403,9 @@ extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, 
                    (num_tokens == 1 || (q_stride % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0)) &&
                    num_tokens <= INT32_MAX && (num_heads + 2 * (int64_t)num_kv_heads) <= 1 << 20;
   if (vec) {
-    if (dtype == ZL_F32) launch_rope_vec<float>(g, ctx->num_sms, S(stream));
-    else launch_rope_vec<__nv_bfloat16>(g, ctx->num_sms, S(stream));
+    const zl_status s = dtype == ZL_F32 ? launch_rope_vec<float>(g, ctx->num_sms, S(stream))
+                                        : launch_rope_vec<__nv_bfloat16>(g, ctx->num_sms, S(stream));
+    if (s != ZL_OK) return s;
   } else {
     const int64_t units = num_tokens * (num_heads + 2 * (int64_t)num_kv_heads);
     int64_t blocks = (units + 7) / 8;
