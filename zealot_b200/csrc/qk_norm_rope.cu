@@ -11,9 +11,8 @@
 // asked for, into packed rows for zl_prefill_varlen; values are copied.
 //
 // Everything is kept in fp32 and rounded once, at the store. The angle is
-// p f_i in 64 bits, taken off its whole turns in 64 bits too (Cody and Waite's
-// reduction with 2 pi in two parts): at p = 10^6 the product in fp32 would be
-// off by 0.06 radians.
+// p f_i in 64 bits, and its whole turns are taken off in 64 bits too: at p = 10^6
+// the product in fp32 would be off by 0.06 radians.
 #include "zl_internal.h"
 #include "zl_pages.h"
 #include "zl_ptx.cuh"
@@ -44,14 +43,13 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// cos and sin of position * frequency.
+// cos and sin of position * frequency: the angle in turns, with 1 / (2 pi) in two parts, less
+// its whole turns.
 __device__ __forceinline__ float2 turn(int32_t pos, double freq) {
-  const double a = (double)pos * freq;
-  const double k = rint(a * 0.15915494309189533577);
-  double r = fma(-k, 6.283185307179586232, a);
-  r = fma(-k, 2.449293598294706539e-16, r);
+  const double a = (double)pos * freq, t = a * 0.15915494309189535;
+  const double rest = fma(a, -9.839338337591243e-18, fma(a, 0.15915494309189535, -t));  // what the product lost
   float s, c;
-  sincosf((float)r, &s, &c);
+  sincospif((float)(2. * ((t - rint(t)) + rest)), &s, &c);
   return make_float2(c, s);
 }
 
@@ -123,61 +121,80 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(RopeArgs g) {
   }
 }
 
-// Four elements, as 8 (bf16) or 16 (fp32) bytes.
-struct Quad {
-  float x[4];
+// E elements: 16 bytes, or 8 for four of bf16.
+template <int E>
+struct Run {
+  float x[E];
 };
-__device__ __forceinline__ Quad load4(const float* p) {
+__device__ __forceinline__ Run<4> load_run(const float* p, Run<4>) {
   const float4 v = *reinterpret_cast<const float4*>(p);
   return {{v.x, v.y, v.z, v.w}};
 }
-__device__ __forceinline__ Quad load4(const __nv_bfloat16* p) {
+__device__ __forceinline__ Run<4> load_run(const __nv_bfloat16* p, Run<4>) {
   const uint2 v = *reinterpret_cast<const uint2*>(p);
   const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
   const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
   return {{a.x, a.y, b.x, b.y}};
 }
-__device__ __forceinline__ void store4(float* p, const Quad& q) {
+__device__ __forceinline__ Run<8> load_run(const __nv_bfloat16* p, Run<8>) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  Run<8> r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 f = __bfloat1622float2(h[i]);
+    r.x[2 * i] = f.x;
+    r.x[2 * i + 1] = f.y;
+  }
+  return r;
+}
+__device__ __forceinline__ void store_run(float* p, const Run<4>& q) {
   *reinterpret_cast<float4*>(p) = make_float4(q.x[0], q.x[1], q.x[2], q.x[3]);
 }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const Quad& q) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(q.x[0], q.x[1]), b = __floats2bfloat162_rn(q.x[2], q.x[3]);
-  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+__device__ __forceinline__ void store_run(__nv_bfloat16* p, const Run<4>& q) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(zl::ptx::pack_bf16x2(q.x[0], q.x[1]), zl::ptx::pack_bf16x2(q.x[2], q.x[3]));
+}
+__device__ __forceinline__ void store_run(__nv_bfloat16* p, const Run<8>& q) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(zl::ptx::pack_bf16x2(q.x[0], q.x[1]), zl::ptx::pack_bf16x2(q.x[2], q.x[3]),
+                 zl::ptx::pack_bf16x2(q.x[4], q.x[5]), zl::ptx::pack_bf16x2(q.x[6], q.x[7]));
 }
 
-// Rotates a lane's 8 elements by the angles of its pairs 4 u .. 4 u + 3.
-__device__ __forceinline__ void rotate(Quad& a, Quad& b, const float2* cs, bool interleaved) {
-  const float4 c01 = reinterpret_cast<const float4*>(cs)[0], c23 = reinterpret_cast<const float4*>(cs)[1];
-  const float c[4] = {c01.x, c01.z, c23.x, c23.z}, s[4] = {c01.y, c01.w, c23.y, c23.w};
-  if (interleaved) {  // pairs (a0, a1), (a2, a3), (b0, b1), (b2, b3)
+// Rotates a lane's two runs by the angles of its E pairs. Two pairs' angles are 16 bytes, and
+// those of neighbouring lanes lie side by side: `lanes` such pieces, then the next two pairs'.
+template <int E>
+__device__ __forceinline__ void rotate(Run<E>& a, Run<E>& b, const float4* cs, int lanes, bool interleaved) {
 #pragma unroll
-    for (int x = 0; x < 4; x++) {
-      Quad& q = x < 2 ? a : b;
-      const int i = 2 * (x & 1);
-      const float y = q.x[i], z = q.x[i + 1];
-      q.x[i] = y * c[x] - z * s[x];
-      q.x[i + 1] = z * c[x] + y * s[x];
-    }
-  } else {
-#pragma unroll
-    for (int x = 0; x < 4; x++) {
-      const float y = a.x[x], z = b.x[x];
-      a.x[x] = y * c[x] - z * s[x];
-      b.x[x] = z * c[x] + y * s[x];
+  for (int x = 0; x < E; x += 2) {
+    const float4 t = cs[x / 2 * lanes];
+    if (interleaved) {  // 2 x, 2 x + 1 and 2 x + 2, 2 x + 3 of the 2 E elements in a row
+      Run<E>& q = x < E / 2 ? a : b;
+      const int i = 2 * (x % (E / 2));
+      const float y0 = q.x[i], z0 = q.x[i + 1], y1 = q.x[i + 2], z1 = q.x[i + 3];
+      q.x[i] = y0 * t.x - z0 * t.y;
+      q.x[i + 1] = z0 * t.x + y0 * t.y;
+      q.x[i + 2] = y1 * t.z - z1 * t.w;
+      q.x[i + 3] = z1 * t.z + y1 * t.w;
+    } else {
+      const float y0 = a.x[x], z0 = b.x[x], y1 = a.x[x + 1], z1 = b.x[x + 1];
+      a.x[x] = y0 * t.x - z0 * t.y;
+      b.x[x] = z0 * t.x + y0 * t.y;
+      a.x[x + 1] = y1 * t.z - z1 * t.w;
+      b.x[x + 1] = z1 * t.z + y1 * t.w;
     }
   }
 }
 
-// head_dim and rotary_dim multiples of 8, rows that 4-element loads can read. LG lanes (a
-// power of two, at least d / 8) share a row; a lane has 8 elements of it, two runs of four:
-// pairs 4 u .. 4 u + 3, whose elements lie in the two halves of the rotated part (or,
+// Rows that loads of E elements can read, head_dim and rotary_dim multiples of 2 E. LG lanes
+// (a power of two, at least d / (2 E)) share a row; a lane has two runs of E of its elements,
+// the pairs E u .. E u + E - 1, whose elements lie in the two halves of the rotated part (or,
 // interleaved, side by side), so that a rotation needs no exchange between lanes. A CTA takes
 // `per` tokens; their angles, once for all heads, and their cache rows go to shared memory.
-// A lane group keeps to one head (of q, then k, then v) over all its tokens, then takes the
-// next. HeadRows is that head: where its rows come from and go to.
+// A lane group keeps to one head (of q, then k, then v) over its tokens, then takes the next.
+// HeadRows is that head: where its rows come from and go to.
 template <typename T>
 struct HeadRows {
-  const T* src;  // this lane's group's row of the CTA's first token
+  const T* src;  // the head's row of the CTA's first token
   T *out, *pool;
   const T* w;
   int64_t stride, out_stride;
@@ -199,28 +216,28 @@ struct HeadRows {
   }
 };
 
-template <typename T, int LG>
+template <int LG, int E>
 struct Lane {  // a lane's place in its row
   int u, e0, e1;
   bool mine, turned;
   __device__ __forceinline__ explicit Lane(const RopeArgs& g) {
     u = threadIdx.x % LG;
-    mine = u * 8 < g.d;
-    turned = u * 8 < g.rot;
+    mine = u * 2 * E < g.d;
+    turned = u * 2 * E < g.rot;
     const bool halves = turned && !g.interleaved;
-    e0 = halves ? 4 * u : 8 * u;
-    e1 = halves ? g.rot / 2 + 4 * u : 8 * u + 4;
+    e0 = halves ? E * u : 2 * E * u;
+    e1 = halves ? g.rot / 2 + E * u : 2 * E * u + E;
   }
 };
 
 // Norms and rotates one row and stores it: token c of the CTA, whose angles are cs and
 // whose pool rows start at element `at` (-1: none).
-template <typename T, int LG>
-__device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<T, LG>& ln, const HeadRows<T>& r, int c,
-                                           Quad a, Quad b, const float2* cs, int64_t at) {
+template <typename T, int LG, int E>
+__device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>& ln, const HeadRows<T>& r, int c,
+                                           Run<E> a, Run<E> b, const float2* cs, int64_t at) {
   float ss = 0.f, s2 = 0.f;
 #pragma unroll
-  for (int x = 0; x < 4; x++) {
+  for (int x = 0; x < E; x++) {
     ss = fmaf(a.x[x], a.x[x], ss);
     s2 = fmaf(b.x[x], b.x[x], s2);
   }
@@ -229,33 +246,34 @@ __device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<T, LG>&
   for (int o = LG / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (!r.use) return;
   if (r.w) {
-    const Quad wa = load4(r.w + ln.e0), wb = load4(r.w + ln.e1);
+    const Run<E> wa = load_run(r.w + ln.e0, Run<E>{}), wb = load_run(r.w + ln.e1, Run<E>{});
     const float y = ss * g.inv_d + g.eps, q = rsqrtf(y);
     const float inv = q * fmaf(-0.5f * y * q, q, 1.5f);  // a Newton step: right to fp32's last place or so
 #pragma unroll
-    for (int x = 0; x < 4; x++) {
+    for (int x = 0; x < E; x++) {
       a.x[x] = a.x[x] * inv * wa.x[x];
       b.x[x] = b.x[x] * inv * wb.x[x];
     }
   }
-  if (r.turn) rotate(a, b, cs + 4 * ln.u, g.interleaved);
+  if (r.turn) rotate(a, b, reinterpret_cast<const float4*>(cs) + ln.u, g.rot / (2 * E), g.interleaved);
   if (r.out) {
     T* to = r.out + c * r.out_stride;
-    store4(to + ln.e0, a);
-    store4(to + ln.e1, b);
+    store_run(to + ln.e0, a);
+    store_run(to + ln.e1, b);
   }
   if (r.pool && at >= 0) {
-    store4(r.pool + at + ln.e0, a);
-    store4(r.pool + at + ln.e1, b);
+    store_run(r.pool + at + ln.e0, a);
+    store_run(r.pool + at + ln.e1, b);
   }
 }
 
-// The CTA's angles and, in elements, the pool rows of its tokens' kv head 0.
+// The CTA's angles, in rotate()'s order, and, in elements, the pool rows of its tokens' kv head 0.
+template <int E>
 __device__ __forceinline__ void token_tables(const RopeArgs& g, int64_t t0, int tokens, float2* cs, int64_t* cache) {
   const int half = g.rot / 2;
   for (int i = threadIdx.x; i < tokens * half; i += 256) {
-    const int t = i / half;
-    cs[i] = turn(g.positions[t0 + t], g.inv_freq[i - t * half]);
+    const int t = i / half, p = i - t * half, u = p / E, x = p % E;  // pair x of lane u
+    cs[t * half + (x / 2 * (half / E) + u) * 2 + x % 2] = turn(g.positions[t0 + t], g.inv_freq[p]);
   }
   if (threadIdx.x < tokens) {
     const int64_t row = cache_row(g, t0 + threadIdx.x, 0);
@@ -264,23 +282,23 @@ __device__ __forceinline__ void token_tables(const RopeArgs& g, int64_t t0, int 
 }
 
 // Few tokens: one to a CTA, and its heads over gridDim.y of them.
-template <typename T, int LG>
+template <typename T, int LG, int E>
 __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
   __shared__ __align__(16) float2 cs[kMaxDim / 2];
   __shared__ int64_t cache[1];
-  const Lane<T, LG> ln(g);
+  const Lane<LG, E> ln(g);
   const int64_t t0 = blockIdx.x;
   bool tables = false;
   // every group of a CTA goes through the loop equally often (the barrier inside)
   for (int h0 = blockIdx.y * (256 / LG); h0 < g.H + 2 * g.Hkv; h0 += gridDim.y * (256 / LG)) {
     const HeadRows<T> r(g, h0 + threadIdx.x / LG, t0, ln.mine, ln.turned);
-    Quad a{}, b{};
+    Run<E> a{}, b{};
     if (r.use) {
-      a = load4(r.src + ln.e0);
-      b = load4(r.src + ln.e1);
+      a = load_run(r.src + ln.e0, a);
+      b = load_run(r.src + ln.e1, b);
     }
     if (!tables) {  // while the row is on its way
-      token_tables(g, t0, 1, cs, cache);
+      token_tables<E>(g, t0, 1, cs, cache);
       __syncthreads();
       tables = true;
     }
@@ -289,76 +307,91 @@ __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
 }
 
 // Many tokens: HBM-bound. Every thread copies its own two runs of the rows that it will need
-// kAhead steps from now into its own slots of shared memory, in the background: bytes on their
-// way without registers, and without a barrier, since each thread waits for its own.
-constexpr int kTokens = 16, kAhead = 8;
-template <typename T, int LG>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) rope_tokens_kernel(RopeArgs g, int per) {
-  constexpr int RUN = 4 * sizeof(T);
-  extern __shared__ __align__(16) uint8_t dyn[];  // [kAhead][256][2 RUN], then the angles
+// kAhead - 1 steps from now into its own slots of shared memory, in the background: bytes on
+// their way without registers, and without a barrier, since each thread waits for its own.
+// The groups are shared out as `hpb` heads by `slices` parts of the tokens.
+constexpr int kTokens = 16, kAhead = 4, kFew = 2;
+template <typename T> constexpr int kResident = sizeof(T) == 2 ? 3 : 4;  // CTAs to an SM
+template <typename T, int LG, int E>
+__global__ void __launch_bounds__(256, kResident<T>) rope_tokens_kernel(RopeArgs g, int per, int hpb, int slices) {
+  constexpr int RUN = E * sizeof(T);
+  extern __shared__ __align__(16) uint8_t dyn[];  // [kAhead][2][256] runs, then the angles
   __shared__ int64_t cache[kTokens];
   float2* cs = reinterpret_cast<float2*>(dyn + kAhead * 256 * 2 * RUN);
-  const Lane<T, LG> ln(g);
+  const Lane<LG, E> ln(g);
   const int64_t t0 = (int64_t)blockIdx.x * per;
   const int tokens = (int)min((int64_t)per, g.tokens - t0), half = g.rot / 2, group = threadIdx.x / LG;
-  const int blocks = (g.H + 2 * g.Hkv + 256 / LG - 1) / (256 / LG), steps = blocks * tokens;
-  const uint32_t slots = zl::ptx::smem_u32(dyn) + threadIdx.x * 2 * RUN;
-  HeadRows<T> ahead(g, group, t0, ln.mine, ln.turned), r = ahead;
-  int hb = 0, c2 = 0;  // head block and token of the next copy
+  const int slice = group / hpb, heads = slice < slices ? g.H + 2 * g.Hkv : 0;  // a group that is left over: none
+  const uint32_t slots = zl::ptx::smem_u32(dyn) + threadIdx.x * RUN;
+  int h2 = group - slice * hpb, c2 = slice;  // head and token of the next copy
+  if (c2 >= tokens) h2 = heads;
+  HeadRows<T> ahead(g, h2, t0, ln.mine, ln.turned), r = ahead;
+  int h = h2, c = c2;
   auto fetch = [&](int slot) {
-    if (hb < blocks && ahead.use) {
-      const uint32_t to = slots + slot * 256 * 2 * RUN;
-      zl::ptx::copy_async<RUN>(to, ahead.src + ln.e0);
-      zl::ptx::copy_async<RUN>(to + RUN, ahead.src + ln.e1);
+    if (h2 < heads) {
+      if (ahead.use) {
+        const uint32_t to = slots + slot * 256 * 2 * RUN;
+        const T* src = ahead.src + c2 * ahead.stride;
+        zl::ptx::copy_async<RUN>(to, src + ln.e0);
+        zl::ptx::copy_async<RUN>(to + 256 * RUN, src + ln.e1);
+      }
+      if ((c2 += slices) >= tokens) {
+        c2 = slice;
+        h2 += hpb;
+        ahead = HeadRows<T>(g, h2, t0, ln.mine, ln.turned);
+      }
     }
     zl::ptx::copies_commit();
-    ahead.src += ahead.stride;
-    if (++c2 == tokens) {
-      c2 = 0;
-      if (++hb < blocks) ahead = HeadRows<T>(g, hb * (256 / LG) + group, t0, ln.mine, ln.turned);
-    }
   };
 #pragma unroll
   for (int i = 0; i < kAhead - 1; i++) fetch(i);
-  token_tables(g, t0, tokens, cs, cache);
+  token_tables<E>(g, t0, tokens, cs, cache);
   __syncthreads();
-  for (int s = 0, h = 0, c = 0; s < steps; s++) {
+  // a warp's groups take their last steps together: the sum over lanes needs them all
+  int s = 0;
+  while (__any_sync(0xffffffffu, h < heads)) {
     fetch((s + kAhead - 1) % kAhead);
     zl::ptx::copies_wait<kAhead - 1>();
-    const T* slot = reinterpret_cast<const T*>(dyn + ((s % kAhead) * 256 + threadIdx.x) * 2 * RUN);
-    finish_row(g, ln, r, c, load4(slot), load4(slot + 4), cs + c * half, cache[c]);
-    if (++c == tokens) {
-      c = 0;
-      h++;
-      r = HeadRows<T>(g, h * (256 / LG) + group, t0, ln.mine, ln.turned);
+    const T* slot = reinterpret_cast<const T*>(dyn + (s % kAhead * 2 * 256 + threadIdx.x) * RUN);
+    r.use = r.use && h < heads;
+    finish_row(g, ln, r, c, load_run(slot, Run<E>{}), load_run(slot + 256 * E, Run<E>{}), cs + c * half, cache[c]);
+    if (h < heads && (c += slices) >= tokens) {
+      c = slice;
+      h += hpb;
+      r = HeadRows<T>(g, h, t0, ln.mine, ln.turned);
     }
+    s++;
   }
   zl::ptx::copies_wait<0>();
 }
 
-template <typename T, int LG>
+template <typename T, int LG, int E>
 zl_status launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
   using namespace zl;
   constexpr int NG = 256 / LG;
-  int64_t per = g.tokens / (4 * (int64_t)num_sms);
-  if (per < 4) {
-    const unsigned y = (unsigned)((g.H + 2 * g.Hkv + NG - 1) / NG);
-    rope_token_kernel<T, LG><<<dim3((unsigned)g.tokens, y < 65535 ? y : 65535), 256, 0, st>>>(g);
+  const int heads = g.H + 2 * g.Hkv, blocks = (heads + NG - 1) / NG;
+  // CTAs that the GPU has room for at once, and tokens to a CTA that fill whole rounds of them
+  const int64_t room = kResident<T> * (int64_t)num_sms, rounds = (g.tokens + room * kTokens - 1) / (room * kTokens);
+  const int64_t per = (g.tokens + room * rounds - 1) / (room * rounds);
+  if (per < kFew) {
+    rope_token_kernel<T, LG, E><<<dim3((unsigned)g.tokens, blocks < 65535 ? blocks : 65535), 256, 0, st>>>(g);
     return ZL_OK;
   }
-  if (per > kTokens) per = kTokens;
-  const size_t smem = (size_t)kAhead * 256 * 8 * sizeof(T) + per * (g.rot / 2) * sizeof(float2);
-  if (smem > 48 * 1024)
-    ZL_CUDA_TRY(cudaFuncSetAttribute(rope_tokens_kernel<T, LG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  rope_tokens_kernel<T, LG><<<(unsigned)((g.tokens + per - 1) / per), 256, smem, st>>>(g, (int)per);
+  const int hpb = (heads + blocks - 1) / blocks, slices = NG / hpb;
+  const size_t smem = (size_t)kAhead * 256 * 2 * E * sizeof(T) + per * (g.rot / 2) * sizeof(float2);
+  const auto kernel = rope_tokens_kernel<T, LG, E>;
+  ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<(unsigned)((g.tokens + per - 1) / per), 256, smem, st>>>(g, (int)per, hpb, slices);
   return ZL_OK;
 }
 
-template <typename T>
+template <typename T, int E>
 zl_status launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
-  return g.d <= 64    ? launch_rope_vec<T, 8>(g, num_sms, st)
-         : g.d <= 128 ? launch_rope_vec<T, 16>(g, num_sms, st)
-                      : launch_rope_vec<T, 32>(g, num_sms, st);
+  const int lanes = g.d / (2 * E);
+  return lanes <= 4    ? launch_rope_vec<T, 4, E>(g, num_sms, st)
+         : lanes <= 8  ? launch_rope_vec<T, 8, E>(g, num_sms, st)
+         : lanes <= 16 ? launch_rope_vec<T, 16, E>(g, num_sms, st)
+                       : launch_rope_vec<T, 32, E>(g, num_sms, st);
 }
 
 }  // namespace
@@ -396,22 +429,28 @@ extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, 
   RopeArgs g{q, k, v, q_stride, k_stride, v_stride, q_weight, k_weight, eps, positions, inv_freq, rotary_dim,
              interleaved, q_out, k_out, v_out, k_pool, v_pool, k_pool ? slot_mapping : nullptr, block_size,
              num_blocks, num_tokens, num_heads, num_kv_heads, head_dim, 1.f / head_dim, ctx->d_status};
-  const size_t quad = 4 * dtype_size(dtype);
-  auto fits = [quad](const void* p) { return reinterpret_cast<uintptr_t>(p) % quad == 0; };
-  const bool vec = head_dim % 8 == 0 && rotary_dim % 8 == 0 && fits(q) && fits(k) && fits(v) && fits(q_out) &&
-                   fits(k_out) && fits(v_out) && fits(k_pool) && fits(v_pool) &&
-                   (num_tokens == 1 || (q_stride % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0)) &&
-                   num_tokens <= INT32_MAX && (num_heads + 2 * (int64_t)num_kv_heads) <= 1 << 20;
+  // rows of runs of `n` elements
+  auto runs = [&](int n) {
+    const size_t bytes = n * dtype_size(dtype);
+    for (const void* p : {q, k, v, q_weight, k_weight, (const void*)q_out, (const void*)k_out, (const void*)v_out,
+                          (const void*)k_pool, (const void*)v_pool})
+      if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
+    return head_dim % (2 * n) == 0 && rotary_dim % (2 * n) == 0 &&
+           (num_tokens == 1 || (q_stride % n == 0 && k_stride % n == 0 && v_stride % n == 0));
+  };
+  const bool vec = num_tokens <= INT32_MAX && num_heads + 2 * (int64_t)num_kv_heads <= 1 << 20 && runs(4);
+  const cudaStream_t st = S(stream);
   if (vec) {
-    const zl_status s = dtype == ZL_F32 ? launch_rope_vec<float>(g, ctx->num_sms, S(stream))
-                                        : launch_rope_vec<__nv_bfloat16>(g, ctx->num_sms, S(stream));
+    const zl_status s = dtype == ZL_F32 ? launch_rope_vec<float, 4>(g, ctx->num_sms, st)
+                        : runs(8)       ? launch_rope_vec<__nv_bfloat16, 8>(g, ctx->num_sms, st)
+                                        : launch_rope_vec<__nv_bfloat16, 4>(g, ctx->num_sms, st);
     if (s != ZL_OK) return s;
   } else {
     const int64_t units = num_tokens * (num_heads + 2 * (int64_t)num_kv_heads);
     int64_t blocks = (units + 7) / 8;
     if (blocks > (int64_t)ctx->num_sms * 32) blocks = (int64_t)ctx->num_sms * 32;
-    if (dtype == ZL_F32) rope_elem_kernel<float><<<(unsigned)blocks, 256, 0, S(stream)>>>(g);
-    else rope_elem_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, S(stream)>>>(g);
+    if (dtype == ZL_F32) rope_elem_kernel<float><<<(unsigned)blocks, 256, 0, st>>>(g);
+    else rope_elem_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, st>>>(g);
   }
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
