@@ -20,7 +20,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxSeqs = 8192;      // requests of one step: 12 bytes of shared memory each
+constexpr int kMaxSeqs = 8192;      // requests of one step: 16 bytes of shared memory each
 constexpr int kMaxRows = 1 << 18;   // rows of the persistent table: 2 bits of shared memory each
 
 struct StepArgs {
@@ -79,27 +79,77 @@ __device__ void scan2(int32_t* a, int32_t* b, int n) {
   if (threadIdx.x == kThreads - 1) a[n] = ea;
 }
 
+// Columns [c, c + N) of request i's table row: r is its row of seq_blocks or -1, `had` and
+// `has` its blocks before and after, `fresh` the place of its first new id.
+template <int N>
+__device__ __forceinline__ bool table_columns(const StepArgs& g, int i, int c, int r, int had, int has, int fresh) {
+  int32_t id[N];
+  bool bad = false;
+  int32_t* old = g.seq_blocks + (int64_t)(r < 0 ? 0 : r) * g.max_blocks + c;
+#pragma unroll
+  for (int k = 0; k < N; k++) id[k] = -1;
+  if (c < had) {
+    if constexpr (N == 4) {
+      const int4 v = *reinterpret_cast<const int4*>(old);
+      id[0] = v.x;
+      id[1] = v.y;
+      id[2] = v.z;
+      id[3] = v.w;
+    } else {
+      id[0] = *old;
+    }
+  }
+  if (c < has) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      if (c + k >= has) {
+        id[k] = -1;
+        continue;
+      }
+      const int64_t at = (int64_t)fresh + c + k - had;
+      if (c + k >= had) id[k] = at < g.num_new ? g.new_blocks[at] : -1;
+      if (id[k] < 0 || id[k] >= g.num_blocks) {
+        id[k] = -1;
+        bad = true;
+      }
+      if (c + k >= had) old[k] = id[k];
+    }
+  }
+  int32_t* to = g.block_tables + (int64_t)i * g.max_blocks + c;
+  if constexpr (N == 4) *reinterpret_cast<int4*>(to) = make_int4(id[0], id[1], id[2], id[3]);
+  else *to = id[0];
+  return bad;
+}
+
+// A CTA takes units: N columns per thread and step of a table row's stretch of kStretch
+// columns, then stretches of kThreads token rows.
+constexpr int kStretch = 4096;
+template <int N>
 __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
   extern __shared__ int32_t sh[];
   const int n = g.num_seqs;
   int32_t* cu = sh;                                             // [n + 1] first token row
   int32_t* fresh = cu + n + 1;                                  // [n] first new id
   int32_t* row = fresh + n;                                     // [n] row of seq_blocks, -1: nothing to serve
-  uint32_t* once = reinterpret_cast<uint32_t*>(row + n);        // rows seen
+  int32_t* ctx = row + n;                                       // [n] context length
+  uint32_t* once = reinterpret_cast<uint32_t*>(ctx + n);        // rows seen
   const int words = g.rows ? (g.num_rows + 31) / 32 : 0;
   uint32_t* twice = once + words;                               // rows seen again
-  int bad = 0;
+  bool bad = false;
 
   for (int w = threadIdx.x; w < 2 * words; w += kThreads) once[w] = 0;
-  __syncthreads();
+  if (words) __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int r = g.rows ? g.rows[i] : i;
-    const zl::StepRequest q = zl::step_request(g.context_lens[i], g.query_lens[i], g.bs, g.max_blocks);
+    const int32_t c = g.context_lens[i];
+    const zl::StepRequest q = zl::step_request(c, g.query_lens[i], g.bs, g.max_blocks);
+    const bool ok = r >= 0 && r < g.num_rows && q.ok;
     cu[i] = q.tokens;
     fresh[i] = r < 0 ? 0 : q.need;
-    row[i] = r >= 0 && r < g.num_rows && q.ok ? r : -1;
-    bad |= r >= 0 && row[i] < 0;
-    if (g.rows && row[i] >= 0) {
+    row[i] = ok ? r : -1;
+    ctx[i] = c;
+    bad |= r >= 0 && !ok;
+    if (g.rows && ok) {
       const uint32_t bit = 1u << (r & 31);
       if (atomicOr(once + (r >> 5), bit) & bit) atomicOr(twice + (r >> 5), bit);
     }
@@ -112,49 +162,38 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
     // every request of a row that is listed twice, or whose tokens do not fit
     if (r >= 0 && ((g.rows && (twice[r >> 5] >> (r & 31) & 1)) || cu[i + 1] > g.num_tokens)) {
       row[i] = -1;
-      bad = 1;
+      bad = true;
     }
   }
   __syncthreads();
 
-  const int gtid = blockIdx.x * kThreads + threadIdx.x, gsize = gridDim.x * kThreads;
   const int32_t cap = (int32_t)(g.num_tokens < 0x7fffffff ? g.num_tokens : 0x7fffffff);
-  for (int i = gtid; i <= n; i += gsize) {
-    const int32_t c = min(cu[i], cap);
-    g.cu_seqlens[i] = c;
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i <= n; i += gridDim.x * kThreads) {
+    g.cu_seqlens[i] = min(cu[i], cap);
     if (i < n) {
-      g.seq_lens[i] = row[i] < 0 ? 0 : g.context_lens[i] + g.query_lens[i];
+      g.seq_lens[i] = row[i] < 0 ? 0 : ctx[i] + cu[i + 1] - cu[i];
       g.last_rows[i] = max(min(cu[i + 1], cap) - 1, 0);
     }
   }
-  // table rows: a warp per row and 128 columns
-  const int segs = (g.max_blocks + 127) / 128;
-  for (int64_t u = gtid >> 5; u < (int64_t)n * segs; u += gsize >> 5) {
-    const int i = (int)(u / segs), c0 = (int)(u - (int64_t)i * segs) * 128 + (threadIdx.x & 31);
-    const int r = row[i];
-    int had = 0, has = 0;
-    if (r >= 0) {
-      const zl::StepRequest q = zl::step_request(g.context_lens[i], g.query_lens[i], g.bs, g.max_blocks);
-      had = q.had;
-      has = q.had + q.need;
-    }
-    for (int c = c0; c < min(c0 + 128, g.max_blocks); c += 32) {
-      int32_t id = -1;
-      if (c < has) {
-        int32_t* at = g.seq_blocks + (int64_t)r * g.max_blocks + c;
-        const int64_t k = (int64_t)fresh[i] + c - had;
-        id = c < had ? *at : k < g.num_new ? g.new_blocks[k] : -1;
-        if (id < 0 || id >= g.num_blocks) {
-          id = -1;
-          bad = 1;
-        }
-        if (c >= had) *at = id;
+  const int stretches = (g.max_blocks + kStretch - 1) / kStretch;
+  const int64_t tables = (int64_t)n * stretches, units = tables + (g.num_tokens + kThreads - 1) / kThreads;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    if (u < tables) {
+      const int i = (int)(u / stretches), c0 = (int)(u - (int64_t)i * stretches) * kStretch;
+      const int r = row[i];
+      int had = 0, has = 0;
+      if (r >= 0) {
+        had = (int)zl::blocks_of(ctx[i], g.bs);
+        has = (int)zl::blocks_of((int64_t)ctx[i] + cu[i + 1] - cu[i], g.bs);
       }
-      g.block_tables[(int64_t)i * g.max_blocks + c] = id;
+      const int end = min(c0 + kStretch, g.max_blocks);
+#pragma unroll 4
+      for (int c = c0 + threadIdx.x * N; c < end; c += kThreads * N)
+        bad |= table_columns<N>(g, i, c, r, had, has, fresh[i]);
+      continue;
     }
-  }
-  // token rows
-  for (int64_t t = gtid; t < g.num_tokens; t += gsize) {
+    const int64_t t = (u - tables) * kThreads + threadIdx.x;
+    if (t >= g.num_tokens) continue;
     int32_t pos = 0;
     int64_t slot = -1;
     if (t < cu[n]) {
@@ -166,19 +205,18 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
       }
       const int r = row[lo];
       if (r >= 0) {
-        const int32_t ctx = g.context_lens[lo];
-        pos = ctx + (int32_t)(t - cu[lo]);
-        const int had = (int)zl::blocks_of(ctx, g.bs), c = pos / g.bs;
+        pos = ctx[lo] + (int32_t)(t - cu[lo]);
+        const int had = (int)zl::blocks_of(ctx[lo], g.bs), c = pos / g.bs;
         const int64_t k = (int64_t)fresh[lo] + c - had;
         const int32_t id = c < had ? g.seq_blocks[(int64_t)r * g.max_blocks + c] : k < g.num_new ? g.new_blocks[k] : -1;
         if (id >= 0 && id < g.num_blocks) slot = (int64_t)id * g.bs + pos % g.bs;
-        else bad = 1;
+        else bad = true;
       }
     }
     g.positions[t] = pos;
     g.slot_mapping[t] = slot;
   }
-  if (threadIdx.x == 0 && cu[n] > g.num_tokens) bad = 1;
+  if (threadIdx.x == 0 && cu[n] > g.num_tokens) bad = true;
   if (bad) atomicOr(g.status, ZL_DEV_OOB);
 }
 
@@ -213,14 +251,15 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   StepArgs g{seq_blocks, rows, context_lens, query_lens, new_blocks, block_tables, cu_seqlens, seq_lens, positions,
              slot_mapping, last_rows, num_new, num_tokens, num_blocks, num_rows, num_seqs, max_blocks_per_seq,
              block_size, ctx->d_status};
-  const size_t smem = sizeof(int32_t) * (3 * (size_t)num_seqs + 1) + (rows ? 8 * (size_t)((num_rows + 31) / 32) : 0);
+  const size_t smem = sizeof(int32_t) * (4 * (size_t)num_seqs + 1) + (rows ? 8 * (size_t)((num_rows + 31) / 32) : 0);
+  const bool vec = max_blocks_per_seq % 4 == 0 && aligned16(seq_blocks) && aligned16(block_tables);
+  const auto kernel = vec ? step_tables_kernel<4> : step_tables_kernel<1>;
   if (smem > 32 * 1024)  // with the static part it may pass 48 KB
-    ZL_CUDA_TRY(cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)smem));
-  const int64_t items = (int64_t)num_seqs * ((max_blocks_per_seq + 127) / 128) * 32 + num_tokens + num_seqs + 1;
-  int64_t blocks = (items + kThreads - 1) / kThreads;
-  if (blocks > 2 * ctx->num_sms) blocks = 2 * ctx->num_sms;
-  step_tables_kernel<<<(unsigned)blocks, kThreads, smem, S(stream)>>>(g);
+    ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  int64_t blocks = (int64_t)num_seqs * ((max_blocks_per_seq + kStretch - 1) / kStretch) + (num_tokens + kThreads - 1) / kThreads;
+  const int64_t most = 4 * ctx->num_sms;
+  blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
+  kernel<<<(unsigned)blocks, kThreads, smem, S(stream)>>>(g);
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }
