@@ -15,6 +15,7 @@ SOURCE = """
 #include "zl_pages.h"
 extern "C" {
 int64_t blocks_of(int64_t t, int bs) { return zl::blocks_of(t, bs); }
+int32_t blocks_of32(uint32_t t, int bs) { return zl::blocks_of32(t, bs); }
 int64_t pool_row(int64_t id, int64_t nb, int hkv, int h, int bs, int t) { return zl::pool_row(id, nb, hkv, h, bs, t); }
 int step_request(int64_t c, int64_t q, int bs, int64_t mb, int32_t* out) {
   zl::StepRequest r = zl::step_request(c, q, bs, mb);
@@ -37,6 +38,7 @@ def pages(tmp_path_factory):
     lib = ctypes.CDLL(str(so))
     i64 = ctypes.c_int64
     lib.blocks_of.restype, lib.blocks_of.argtypes = i64, [i64, ctypes.c_int]
+    lib.blocks_of32.argtypes = [ctypes.c_uint32, ctypes.c_int]
     lib.pool_row.restype = i64
     lib.pool_row.argtypes = [i64, i64] + [ctypes.c_int] * 4
     lib.step_request.argtypes = [i64, i64, ctypes.c_int, i64, ctypes.POINTER(ctypes.c_int32)]
@@ -48,6 +50,9 @@ def pages(tmp_path_factory):
 def test_blocks_of(pages, bs):
     for t in (-5, 0, 1, bs - 1, bs, bs + 1, 2**31 - 1):
         assert pages.blocks_of(t, bs) == (0 if t <= 0 else -(-t // bs))
+        if t >= 0:
+            assert pages.blocks_of32(t, bs) == -(-t // bs)
+    assert pages.blocks_of32(2**31 - 1, 2**31 - 1) == 1 and pages.blocks_of32(1, 2**31 - 1) == 1
 
 
 def test_pool_row_bad_ids(pages):

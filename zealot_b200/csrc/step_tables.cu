@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kMaxSeqs = 8192;      // requests of one step: 16 bytes of shared memory each
 constexpr int kMaxRows = 1 << 18;   // rows of the persistent table: 2 bits of shared memory each
 
@@ -79,51 +79,57 @@ __device__ void scan2(int32_t* a, int32_t* b, int n) {
   if (threadIdx.x == kThreads - 1) a[n] = ea;
 }
 
-// Columns [c, c + N) of request i's table row: r is its row of seq_blocks or -1, `had` and
-// `has` its blocks before and after, `fresh` the place of its first new id.
+// N table entries, as one load or store.
 template <int N>
-__device__ __forceinline__ bool table_columns(const StepArgs& g, int i, int c, int r, int had, int has, int fresh) {
-  int32_t id[N];
-  bool bad = false;
-  int32_t* old = g.seq_blocks + (int64_t)(r < 0 ? 0 : r) * g.max_blocks + c;
-#pragma unroll
-  for (int k = 0; k < N; k++) id[k] = -1;
-  if (c < had) {
-    if constexpr (N == 4) {
-      const int4 v = *reinterpret_cast<const int4*>(old);
-      id[0] = v.x;
-      id[1] = v.y;
-      id[2] = v.z;
-      id[3] = v.w;
-    } else {
-      id[0] = *old;
-    }
+struct Ids {
+  int32_t x[N];
+};
+template <int N>
+__device__ __forceinline__ Ids<N> load_ids(const int32_t* p) {
+  Ids<N> r;
+  if constexpr (N == 4) {
+    const int4 v = *reinterpret_cast<const int4*>(p);
+    r.x[0] = v.x;
+    r.x[1] = v.y;
+    r.x[2] = v.z;
+    r.x[3] = v.w;
+  } else {
+    r.x[0] = *p;
   }
-  if (c < has) {
+  return r;
+}
+
+// Columns [c, c + N) of request i's table row from its old ones `id`: r is its row of
+// seq_blocks, `had` and `has` its blocks before and after, `fresh` the place of its first new id.
+template <int N>
+__device__ __forceinline__ bool table_columns(const StepArgs& g, int i, int c, int r, int had, int has, int fresh,
+                                              Ids<N> id) {
+  bool bad = false;
+  if (c + N > had) {  // past the old blocks: new ones, then nothing
 #pragma unroll
     for (int k = 0; k < N; k++) {
-      if (c + k >= has) {
-        id[k] = -1;
-        continue;
-      }
+      if (c + k < had) continue;
       const int64_t at = (int64_t)fresh + c + k - had;
-      if (c + k >= had) id[k] = at < g.num_new ? g.new_blocks[at] : -1;
-      if (id[k] < 0 || id[k] >= g.num_blocks) {
-        id[k] = -1;
-        bad = true;
-      }
-      if (c + k >= had) old[k] = id[k];
+      id.x[k] = c + k < has && at < g.num_new ? g.new_blocks[at] : -1;
+      if ((uint32_t)id.x[k] >= (uint32_t)g.num_blocks) id.x[k] = -1;
+      if (c + k < has) g.seq_blocks[(int64_t)r * g.max_blocks + c + k] = id.x[k];
     }
   }
+#pragma unroll
+  for (int k = 0; k < N; k++)
+    if ((uint32_t)id.x[k] >= (uint32_t)g.num_blocks) {
+      id.x[k] = -1;
+      bad |= c + k < has;
+    }
   int32_t* to = g.block_tables + (int64_t)i * g.max_blocks + c;
-  if constexpr (N == 4) *reinterpret_cast<int4*>(to) = make_int4(id[0], id[1], id[2], id[3]);
-  else *to = id[0];
+  if constexpr (N == 4) *reinterpret_cast<int4*>(to) = make_int4(id.x[0], id.x[1], id.x[2], id.x[3]);
+  else *to = id.x[0];
   return bad;
 }
 
 // A CTA takes units: N columns per thread and step of a table row's stretch of kStretch
 // columns, then stretches of kThreads token rows.
-constexpr int kStretch = 4096;
+constexpr int kStretch = 8192;
 template <int N>
 __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
   extern __shared__ int32_t sh[];
@@ -176,23 +182,32 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
     }
   }
   const int stretches = (g.max_blocks + kStretch - 1) / kStretch;
-  const int64_t tables = (int64_t)n * stretches, units = tables + (g.num_tokens + kThreads - 1) / kThreads;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+  // fewer than 2^32: at most 2^13 requests of 2^18 stretches (a table row of fewer than 2^30 columns),
+  // and fewer than 2^24 stretches of tokens
+  const uint32_t tables = (uint32_t)n * stretches, units = tables + (uint32_t)((g.num_tokens + kThreads - 1) / kThreads);
+  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
     if (u < tables) {
-      const int i = (int)(u / stretches), c0 = (int)(u - (int64_t)i * stretches) * kStretch;
+      const int i = (int)(u / stretches), c0 = (int)(u - (uint32_t)i * stretches) * kStretch;
       const int r = row[i];
       int had = 0, has = 0;
       if (r >= 0) {
-        had = (int)zl::blocks_of(ctx[i], g.bs);
-        has = (int)zl::blocks_of((int64_t)ctx[i] + cu[i + 1] - cu[i], g.bs);
+        had = zl::blocks_of32(ctx[i], g.bs);
+        has = zl::blocks_of32(ctx[i] + cu[i + 1] - cu[i], g.bs);
       }
+      constexpr int STEP = kThreads * N, DEPTH = 4;
       const int end = min(c0 + kStretch, g.max_blocks);
-#pragma unroll 4
-      for (int c = c0 + threadIdx.x * N; c < end; c += kThreads * N)
-        bad |= table_columns<N>(g, i, c, r, had, has, fresh[i]);
+      for (int c = c0 + threadIdx.x * N; c < end; c += STEP * DEPTH) {
+        Ids<N> old[DEPTH];  // all loads before the first store
+#pragma unroll
+        for (int k = 0; k < DEPTH; k++)
+          if (c + k * STEP < min(had, end)) old[k] = load_ids<N>(g.seq_blocks + (int64_t)r * g.max_blocks + c + k * STEP);
+#pragma unroll
+        for (int k = 0; k < DEPTH; k++)
+          if (c + k * STEP < end) bad |= table_columns<N>(g, i, c + k * STEP, r, had, has, fresh[i], old[k]);
+      }
       continue;
     }
-    const int64_t t = (u - tables) * kThreads + threadIdx.x;
+    const int64_t t = (int64_t)(u - tables) * kThreads + threadIdx.x;
     if (t >= g.num_tokens) continue;
     int32_t pos = 0;
     int64_t slot = -1;
@@ -206,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
       const int r = row[lo];
       if (r >= 0) {
         pos = ctx[lo] + (int32_t)(t - cu[lo]);
-        const int had = (int)zl::blocks_of(ctx[lo], g.bs), c = pos / g.bs;
+        const int had = zl::blocks_of32(ctx[lo], g.bs), c = pos / g.bs;
         const int64_t k = (int64_t)fresh[lo] + c - had;
         const int32_t id = c < had ? g.seq_blocks[(int64_t)r * g.max_blocks + c] : k < g.num_new ? g.new_blocks[k] : -1;
         if (id >= 0 && id < g.num_blocks) slot = (int64_t)id * g.bs + pos % g.bs;
@@ -235,8 +250,8 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
                      "step_tables: bad sizes n=%d rows=%d new=%lld T=%lld max_blocks=%d bs=%d blocks=%lld", num_seqs,
                      num_rows, (long long)num_new, (long long)num_tokens, max_blocks_per_seq, block_size,
                      (long long)num_blocks);
-  if (num_tokens > INT32_MAX || num_blocks > INT32_MAX)
-    return set_error(ZL_ERR_INVALID_ARG, "step_tables: more than 2^31-1 token rows or blocks");
+  if (num_tokens > INT32_MAX || num_blocks > INT32_MAX || max_blocks_per_seq > 1 << 30)
+    return set_error(ZL_ERR_INVALID_ARG, "step_tables: more than 2^31-1 token rows or blocks, or 2^30 blocks to a row");
   if (num_seqs > kMaxSeqs || (rows && num_rows > kMaxRows))
     return set_error(ZL_ERR_UNSUPPORTED, "step_tables: at most %d requests (have %d) and %d table rows (have %d)",
                      kMaxSeqs, num_seqs, kMaxRows, num_rows);
@@ -257,7 +272,7 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   if (smem > 32 * 1024)  // with the static part it may pass 48 KB
     ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   int64_t blocks = (int64_t)num_seqs * ((max_blocks_per_seq + kStretch - 1) / kStretch) + (num_tokens + kThreads - 1) / kThreads;
-  const int64_t most = 4 * ctx->num_sms;
+  const int64_t most = 2 * ctx->num_sms;
   blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
   kernel<<<(unsigned)blocks, kThreads, smem, S(stream)>>>(g);
   ZL_LAUNCH_CHECK(ctx);

@@ -15,6 +15,8 @@ namespace zl {
 
 // Blocks that `tokens` cached tokens take.
 ZL_HD int64_t blocks_of(int64_t tokens, int bs) { return tokens <= 0 ? 0 : (tokens + bs - 1) / bs; }
+// The same for a length in [0, 2^31 - 1]: a division in 32 bits.
+ZL_HD int32_t blocks_of32(uint32_t tokens, int bs) { return (int32_t)((tokens + (uint32_t)bs - 1) / (uint32_t)bs); }
 
 // Row (of head_dim elements) of token `t` of block `id` and kv head `kvh` in a
 // pool [num_blocks][hkv][bs][d]; -1 when the id is outside the pool.
@@ -36,9 +38,9 @@ ZL_HD StepRequest step_request(int64_t context, int64_t query, int bs, int64_t m
   r.tokens = query > 0 ? (int32_t)query : 0;
   r.had = r.need = 0;
   if (r.ok) {
-    const int64_t had = blocks_of(context, bs), has = blocks_of(context + query, bs);
-    r.had = (int32_t)had;
-    r.need = (int32_t)(has - had);
+    const int32_t has = blocks_of32((uint32_t)(context + query), bs);
+    r.had = blocks_of32((uint32_t)context, bs);
+    r.need = has - r.had;
     r.ok = has <= max_blocks;
   }
   return r;
