@@ -155,9 +155,9 @@ def test_python_checks_refuse_other_devices(attn):
     with pytest.raises(zb.InvalidArgument, match="device"):
         attn.qk_norm_rope(f, f, f, i, torch.zeros(4, dtype=torch.float64), f)
     with pytest.raises(zb.InvalidArgument, match="cuda:0"):
-        attn.block_bounds(pool, i2, i, pool[:, :, :2])
+        attn.block_bounds(pool, i2, i, pool[:, :, :2].contiguous())
     with pytest.raises(zb.InvalidArgument, match="cuda:0"):
-        attn.block_scores(f, pool, i2, i, f, 16)
+        attn.block_scores(f, pool[:, :, :2].contiguous(), i2, i, f, 16)
     with pytest.raises(zb.InvalidArgument, match="cuda:0"):
         attn.select_blocks(f, i, i2[None], 16)
     with pytest.raises(zb.InvalidArgument, match="cuda:0"):

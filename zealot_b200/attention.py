@@ -21,13 +21,15 @@ class CudaAttention:
         self.ctx = ctx
         self.lib = ctx.lib
 
-    def _check(self, dtype, *tensors) -> None:
-        """Each tensor is a contiguous one of `dtype` on the context's device."""
+    def _check(self, *tensors) -> None:
+        """(tensor or None, dtype, elements) each: contiguous, on the context's device. These checks are
+        most of a small call's host time, so they are one pass with nothing built until one fails."""
         device = self.ctx.device
-        for t in tensors:
-            if t.dtype != dtype or t.get_device() != device or not t.is_contiguous():
-                raise InvalidArgument(f"need a contiguous {dtype} tensor on cuda:{device}, got {t.dtype} on "
-                                      f"{t.device}, strides {tuple(t.stride())}")
+        for t, dtype, n in tensors:
+            if t is not None and (t.dtype is not dtype or t.numel() != n or t.get_device() != device
+                                  or not t.is_contiguous()):
+                raise InvalidArgument(f"need a contiguous {dtype} tensor of {n} elements on cuda:{device}, got "
+                                      f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}")
 
     # ----------------------------------------------------------- step tables
     def step_tables(self, seq_blocks, rows, context_lens, query_lens, new_blocks, block_tables, cu_seqlens,
@@ -39,21 +41,16 @@ class CudaAttention:
         Writes block_tables [n][max_blocks], cu_seqlens [n+1], seq_lens [n], last_rows [n], and for each
         token row positions [T] and slot_mapping [T] (int64; all others int32)."""
         import torch
-        n, T = query_lens.numel(), slot_mapping.numel()
-        self._check(torch.int32, seq_blocks, context_lens, query_lens, new_blocks, block_tables, cu_seqlens,
-                    seq_lens, positions, last_rows)
-        self._check(torch.int64, slot_mapping)
+        i32, n, T, num_new = torch.int32, query_lens.numel(), slot_mapping.numel(), new_blocks.numel()
         _need(seq_blocks.dim() == 2, "seq_blocks is [num_rows][max_blocks]")
         num_rows, max_blocks = seq_blocks.shape
-        if rows is not None:
-            self._check(torch.int32, rows)
-            _need(rows.numel() == n, "one table row per request")
-        _need(context_lens.numel() == n and seq_lens.numel() == n and last_rows.numel() == n
-              and cu_seqlens.numel() == n + 1 and block_tables.numel() == n * max_blocks
-              and positions.numel() == T, "step_tables shapes")
+        self._check((seq_blocks, i32, num_rows * max_blocks), (rows, i32, n), (context_lens, i32, n),
+                    (query_lens, i32, n), (new_blocks, i32, num_new), (block_tables, i32, n * max_blocks),
+                    (cu_seqlens, i32, n + 1), (seq_lens, i32, n), (positions, i32, T),
+                    (slot_mapping, torch.int64, T), (last_rows, i32, n))
         check(self.lib.zl_step_tables(
             self.ctx.handle, seq_blocks.data_ptr(), num_rows, ptr(rows), context_lens.data_ptr(),
-            query_lens.data_ptr(), new_blocks.data_ptr(), new_blocks.numel(), block_tables.data_ptr(),
+            query_lens.data_ptr(), new_blocks.data_ptr(), num_new, block_tables.data_ptr(),
             cu_seqlens.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(),
             last_rows.data_ptr(), n, T, max_blocks, block_size, num_blocks, self.ctx.stream(stream)))
 
@@ -62,42 +59,38 @@ class CudaAttention:
                      k_weight=None, eps: float = 1e-6, interleaved: bool = False, k_pool=None, v_pool=None,
                      slot_mapping=None, stream=None) -> None:
         """RMS norm of each head of q [T][H][d] and k [T][Hkv][d] (a weight [d] or None), rotation of the
-        first 2 * inv_freq.numel() elements of each head by positions[t] * inv_freq (float64), and the
-        stores: q_out, k_out, v_out packed, and the pools [num_blocks][Hkv][bs][d] at slot_mapping.
-        q, k and v may be views of one projection's rows (any stride from token to token)."""
+        first 2 * inv_freq.numel() elements of each head by positions[t] * inv_freq (float64; None: no
+        rotation), and the stores: q_out, k_out, v_out packed, and the pools [num_blocks][Hkv][bs][d] at
+        slot_mapping. q, k and v may be views of one projection's rows (any stride from token to token)."""
         import torch
-        T, Hkv, d = k.shape
-        device, dtype = self.ctx.device, q.dtype
-        _need(q.dim() == 3 and q.shape[0] == T and q.shape[2] == d and v.shape == k.shape, "q/k/v shapes")
-        H = q.shape[1]
-        for t, heads in ((q, H), (k, Hkv), (v, Hkv)):
-            _need(t.dtype == dtype and t.get_device() == device, "q, k and v: one dtype, on the context's device")
-            _need(t.stride(2) == 1 and (t.stride(1) == d or heads == 1), "the heads of a token are packed")
-        for t, heads in ((q_out, H), (k_out, Hkv), (v_out, Hkv)):
-            if t is not None:
-                self._check(dtype, t)
-                _need(t.shape == (T, heads, d), "output shape")
-        for w in (q_weight, k_weight):
-            if w is not None:
-                self._check(dtype, w)
-                _need(w.numel() == d, "a norm weight has head_dim elements")
-        rot = 0
+        dtype, device = q.dtype, self.ctx.device
+        T, H, d = q.shape
+        Hkv = k.shape[1]
+        strides = []
+        for t, n in ((q, H), (k, Hkv), (v, Hkv)):
+            if t.dtype is not dtype or t.get_device() != device or t.shape != (T, n, d):
+                raise InvalidArgument("q [T][H][d], k and v [T][Hkv][d]: one dtype, on the context's device")
+            token, head, element = t.stride()
+            if (element != 1 and d != 1) or (head != d and n != 1):
+                raise InvalidArgument("the heads of a token are packed")
+            strides.append(token)
+        rot = bs = num_blocks = 0
         if inv_freq is not None:
-            self._check(torch.float64, inv_freq)
-            self._check(torch.int32, positions)
-            _need(positions.numel() == T, "one position per token")
+            _need(positions is not None, "inv_freq needs positions")
             rot = 2 * inv_freq.numel()
-        bs = num_blocks = 0
+        pool = 0
         if k_pool is not None or v_pool is not None:
             _need(k_pool is not None and v_pool is not None and slot_mapping is not None,
                   "both pools and a slot_mapping, or none")
-            self._check(dtype, k_pool, v_pool)
-            self._check(torch.int64, slot_mapping)
-            _need(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.shape[1] == Hkv
-                  and k_pool.shape[3] == d and slot_mapping.numel() == T, "pools [num_blocks][Hkv][bs][d], slots [T]")
-            num_blocks, bs = k_pool.shape[0], k_pool.shape[2]
+            num_blocks, pool_heads, bs, pool_d = k_pool.shape
+            _need(pool_heads == Hkv and pool_d == d, "pools are [num_blocks][Hkv][bs][d]")
+            pool = num_blocks * Hkv * bs * d
+        nk = T * Hkv * d
+        self._check((q_out, dtype, T * H * d), (k_out, dtype, nk), (v_out, dtype, nk), (q_weight, dtype, d),
+                    (k_weight, dtype, d), (positions, torch.int32, T), (inv_freq, torch.float64, rot // 2),
+                    (k_pool, dtype, pool), (v_pool, dtype, pool), (slot_mapping, torch.int64, T))
         check(self.lib.zl_qk_norm_rope(
-            self.ctx.handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
+            self.ctx.handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides,
             ptr(q_weight), ptr(k_weight), eps, ptr(positions), ptr(inv_freq), rot, int(interleaved), ptr(q_out),
             ptr(k_out), ptr(v_out), ptr(k_pool), ptr(v_pool), ptr(slot_mapping), bs, num_blocks, T, H, Hkv, d,
             dtype_code(dtype), self.ctx.stream(stream)))
@@ -167,77 +160,69 @@ class CudaAttention:
                                          ptr(out), dtype_code(out.dtype), self.ctx.stream(stream)))
 
     # ------------------------------------------- decode over selected blocks
-    def _paged(self, block_tables, seq_lens):
-        """(B, max_blocks) of a table [B][max_blocks] and its lengths [B], both int32."""
-        import torch
-        self._check(torch.int32, block_tables, seq_lens)
-        _need(block_tables.dim() == 2 and seq_lens.numel() == block_tables.shape[0],
-              "block_tables [B][max_blocks], seq_lens [B]")
-        return block_tables.shape
-
     def block_bounds(self, k_pool, block_tables, seq_lens, bounds, tok_begin=None, stream=None) -> None:
         """Elementwise minimum and maximum of the keys of each block that holds a token in
         [tok_begin[b], seq_lens[b]): k_pool [num_blocks][Hkv][bs][d] -> bounds [num_blocks][Hkv][2][d]."""
         import torch
-        B, max_blocks = self._paged(block_tables, seq_lens)
-        self._check(k_pool.dtype, k_pool, bounds)
-        if tok_begin is not None:
-            self._check(torch.int32, tok_begin)
-            _need(tok_begin.numel() == B, "one tok_begin per sequence")
-        _need(k_pool.dim() == 4, "k_pool is [num_blocks][Hkv][bs][d]")
+        _need(k_pool.dim() == 4 and block_tables.dim() == 2, "k_pool [num_blocks][Hkv][bs][d], block_tables [B][max]")
         num_blocks, Hkv, bs, d = k_pool.shape
-        _need(bounds.shape == (num_blocks, Hkv, 2, d), "bounds is [num_blocks][Hkv][2][d]")
+        B, max_blocks = block_tables.shape
+        i32, dtype, row = torch.int32, k_pool.dtype, num_blocks * Hkv * d
+        self._check((k_pool, dtype, row * bs), (bounds, dtype, row * 2), (block_tables, i32, B * max_blocks),
+                    (seq_lens, i32, B), (tok_begin, i32, B))
         check(self.lib.zl_block_bounds(
             self.ctx.handle, k_pool.data_ptr(), block_tables.data_ptr(), ptr(tok_begin), seq_lens.data_ptr(),
-            bounds.data_ptr(), B, Hkv, d, bs, max_blocks, num_blocks, dtype_code(k_pool.dtype),
-            self.ctx.stream(stream)))
+            bounds.data_ptr(), B, Hkv, d, bs, max_blocks, num_blocks, dtype_code(dtype), self.ctx.stream(stream)))
 
     def block_scores(self, q, bounds, block_tables, seq_lens, scores, block_size: int, scale: float = 0.0,
                      gqa_map: int = GQA_GROUPED, stream=None) -> None:
         """Upper bound of every block's attention scores for q [B][H][d] (the largest over a kv head's
         query heads): scores [B][Hkv][max_blocks] float32, -inf where a sequence has no block."""
         import torch
-        B, max_blocks = self._paged(block_tables, seq_lens)
-        self._check(q.dtype, q, bounds)
-        self._check(torch.float32, scores)
-        _need(q.dim() == 3 and q.shape[0] == B and bounds.dim() == 4, "q [B][H][d], bounds [num_blocks][Hkv][2][d]")
+        _need(q.dim() == 3 and bounds.dim() == 4 and block_tables.dim() == 2,
+              "q [B][H][d], bounds [num_blocks][Hkv][2][d], block_tables [B][max]")
         num_blocks, Hkv, two, d = bounds.shape
-        _need(two == 2 and q.shape[2] == d and scores.shape == (B, Hkv, max_blocks), "block_scores shapes")
+        B, max_blocks = block_tables.shape
+        H, i32, dtype = q.shape[1], torch.int32, q.dtype
+        _need(two == 2, "bounds is [num_blocks][Hkv][2][d]")
+        self._check((q, dtype, B * H * d), (bounds, dtype, num_blocks * Hkv * 2 * d),
+                    (block_tables, i32, B * max_blocks), (seq_lens, i32, B), (scores, torch.float32, B * Hkv * max_blocks))
         check(self.lib.zl_block_scores(
             self.ctx.handle, q.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
-            scores.data_ptr(), B, q.shape[1], Hkv, d, block_size, max_blocks, num_blocks, scale, gqa_map,
-            dtype_code(q.dtype), self.ctx.stream(stream)))
+            scores.data_ptr(), B, H, Hkv, d, block_size, max_blocks, num_blocks, scale, gqa_map,
+            dtype_code(dtype), self.ctx.stream(stream)))
 
     def select_blocks(self, scores, seq_lens, selected, block_size: int, num_first: int = 1, num_last: int = 1,
                       stream=None) -> None:
         """Of each sequence's blocks the first num_first, the last num_last and the best others by
         scores [B][Hkv][max_blocks]: selected [B][Hkv][max_selected] int32, ascending, -1 after the last."""
         import torch
-        self._check(torch.float32, scores)
-        self._check(torch.int32, seq_lens, selected)
-        _need(scores.dim() == 3 and selected.dim() == 3 and selected.shape[:2] == scores.shape[:2]
-              and seq_lens.numel() == scores.shape[0], "select_blocks shapes")
+        _need(scores.dim() == 3 and selected.dim() == 3, "scores [B][Hkv][max_blocks], selected [B][Hkv][max_selected]")
         B, Hkv, max_blocks = scores.shape
+        top = selected.shape[2]
+        self._check((scores, torch.float32, B * Hkv * max_blocks), (seq_lens, torch.int32, B),
+                    (selected, torch.int32, B * Hkv * top))
         check(self.lib.zl_select_blocks(
             self.ctx.handle, scores.data_ptr(), seq_lens.data_ptr(), selected.data_ptr(), B, Hkv, block_size,
-            max_blocks, selected.shape[2], num_first, num_last, self.ctx.stream(stream)))
+            max_blocks, top, num_first, num_last, self.ctx.stream(stream)))
 
     def paged_forward_selected(self, q, k_pool, v_pool, block_tables, seq_lens, selected, o, scale: float = 0.0,
                                gqa_map: int = GQA_GROUPED, stream=None) -> None:
         """paged_forward over the blocks that selected [B][Hkv][max_selected] lists (indices into a
         sequence's table row; a negative one ends the list): q/o [B][H][d]."""
         import torch
-        B, max_blocks = self._paged(block_tables, seq_lens)
-        self._check(q.dtype, q, k_pool, v_pool, o)
-        self._check(torch.int32, selected)
-        _need(k_pool.dim() == 4 and k_pool.shape == v_pool.shape, "pools are [num_blocks][Hkv][bs][d]")
+        _need(q.dim() == 3 and k_pool.dim() == 4 and block_tables.dim() == 2 and selected.dim() == 3,
+              "q [B][H][d], pools [num_blocks][Hkv][bs][d], block_tables [B][max], selected [B][Hkv][max_selected]")
         num_blocks, Hkv, bs, d = k_pool.shape
-        _need(q.dim() == 3 and q.shape[0] == B and q.shape[2] == d and o.shape == q.shape, "q/o shape")
-        _need(selected.dim() == 3 and selected.shape[:2] == (B, Hkv), "selected is [B][Hkv][max_selected]")
+        B, max_blocks = block_tables.shape
+        H, top, i32, dtype = q.shape[1], selected.shape[2], torch.int32, q.dtype
+        pool = num_blocks * Hkv * bs * d
+        self._check((q, dtype, B * H * d), (o, dtype, B * H * d), (k_pool, dtype, pool), (v_pool, dtype, pool),
+                    (block_tables, i32, B * max_blocks), (seq_lens, i32, B), (selected, i32, B * Hkv * top))
         check(self.lib.zl_paged_decode_selected(
             self.ctx.handle, q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
-            seq_lens.data_ptr(), selected.data_ptr(), o.data_ptr(), B, q.shape[1], Hkv, d, bs, max_blocks,
-            num_blocks, selected.shape[2], scale, gqa_map, dtype_code(q.dtype), self.ctx.stream(stream)))
+            seq_lens.data_ptr(), selected.data_ptr(), o.data_ptr(), B, H, Hkv, d, bs, max_blocks, num_blocks, top,
+            scale, gqa_map, dtype_code(dtype), self.ctx.stream(stream)))
 
     # ---------------------------------------------------------------- prefill
     def forward_gpu(self, q, k, v, cu_seqlens, o, num_heads: int, num_kv_heads: int,

@@ -18,9 +18,9 @@ BF16 = 1
 
 def dtype_code(t) -> int:
     import torch
-    if t == torch.float32:
+    if t is torch.float32:
         return F32
-    if t == torch.bfloat16:
+    if t is torch.bfloat16:
         return BF16
     raise TypeError(f"unsupported dtype {t}: the kernels take float32 or bfloat16")
 
@@ -55,7 +55,8 @@ def device_view(address: int, shape, dtype):
 
 def current_stream(device: int) -> int:
     import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: a Stream object for every call would cost more than the call
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 class GpuContext:
