@@ -59,7 +59,12 @@ def freqs(rot, base=10000.0):
     (33, 28, 4, 128, 64, True, True, 131072), (9, 8, 1, 256, 256, False, True, 4096), (9, 8, 1, 256, 256, True, True, 70000),
     (13, 6, 2, 80, 80, False, True, 4096), (13, 6, 2, 80, 40, True, False, 4096), (11, 3, 1, 72, 16, False, True, 100),
     (7, 3, 3, 33, 10, False, True, 100), (7, 3, 3, 33, 32, True, True, 100), (3, 2, 1, 1, 0, False, True, 10),
-    (300, 40, 8, 128, 128, False, True, 2**31 - 1), (1000, 5, 1, 64, 0, False, True, 10), (2, 1, 1, 120, 8, False, True, 50)])
+    (300, 40, 8, 128, 128, False, True, 2**31 - 1), (1000, 5, 1, 64, 0, False, True, 10), (2, 1, 1, 120, 8, False, True, 50),
+    # enough tokens for several to a CTA: rows that fill their lanes and rows that do not, heads that share the groups
+    # evenly and heads that do not, a last CTA with fewer tokens
+    (2503, 8, 1, 96, 96, False, True, 4096), (1777, 12, 4, 64, 64, False, True, 9999), (1301, 3, 1, 256, 256, True, True, 500),
+    (3001, 8, 2, 80, 40, True, True, 4096), (2049, 28, 4, 128, 64, False, False, 70000), (1999, 40, 8, 72, 24, False, True, 100),
+    (1500, 1, 1, 8, 8, False, True, 100), (4001, 16, 16, 48, 0, False, True, 10), (1400, 70, 2, 128, 128, False, True, 1000)])
 def test_norm_rotate_and_cache(ctx, T, H, Hkv, d, rot, inter, norm, far, bf16):
     import torch
     import zealot_b200 as zb

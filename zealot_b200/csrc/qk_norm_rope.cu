@@ -354,7 +354,12 @@ __global__ void __launch_bounds__(256, kResident<T>) rope_tokens_kernel(RopeArgs
     zl::ptx::copies_wait<kAhead - 1>();
     const T* slot = reinterpret_cast<const T*>(dyn + (s % kAhead * 2 * 256 + threadIdx.x) * RUN);
     r.use = r.use && h < heads;
-    finish_row(g, ln, r, c, load_run(slot, Run<E>{}), load_run(slot + 256 * E, Run<E>{}), cs + c * half, cache[c]);
+    Run<E> a{}, b{};  // zeros in the lanes behind the row's end: they take part in its sum
+    if (r.use) {
+      a = load_run(slot, a);
+      b = load_run(slot + 256 * E, b);
+    }
+    finish_row(g, ln, r, c, a, b, cs + c * half, cache[c]);
     if (h < heads && (c += slices) >= tokens) {
       c = slice;
       h += hpb;
