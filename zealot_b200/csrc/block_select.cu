@@ -783,7 +783,7 @@ zl_status zl_block_scores(zl_ctx* ctx, const void* q, const void* bounds, const 
   const cudaStream_t st = S(stream);
   const int64_t rows = (int64_t)num_seqs * num_kv_heads;
   const int p16 = scores_parts(rows, (max_blocks_per_seq + 15) / 16, kScoreWarps, kScoreCtas * ctx->num_sms),
-            p4 = scores_parts(rows, (max_blocks_per_seq + 3) / 4, 8, 8 * ctx->num_sms);
+            p4 = scores_parts(rows, (max_blocks_per_seq + 3) / 4, 8, 4 * ctx->num_sms);
   const bool vec = head_dim * dtype_size(dtype) % 16 == 0 && head_dim <= 256 && aligned16(q) && aligned16(bounds) &&
                    rows * p4 <= INT32_MAX && rows * p16 <= INT32_MAX &&
                    (double)num_blocks * num_kv_heads <= INT32_MAX;

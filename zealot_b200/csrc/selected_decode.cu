@@ -122,46 +122,69 @@ __device__ __forceinline__ int resolve(const SelArgs& g, const Job& w, int e, in
 }
 
 // Joins the warps' (m, l, o) and then the cluster's, and writes the heads' outputs.
-// o: [kWarps][HEADS][DT] unnormalised, in units of 2^m; rows of DT elements, d used.
+// o: [kWarps][HEADS][DT] unnormalised, in units of 2^m; rows of DT elements, d used. A
+// part that saw nothing has l = 0 and is left out, its m being -inf.
 template <typename T, int HEADS, int DT>
 __device__ __forceinline__ void finish(const SelArgs& g, const Job& w, int cluster, int rank, float* o,
                                        float (*m)[HEADS], float (*l)[HEADS]) {
   __shared__ float mc[HEADS], lc[HEADS];
+  __shared__ float factor[kWarps][HEADS];
+  const int tid = threadIdx.x;
   __syncthreads();
-  if (threadIdx.x < HEADS) {
-    const int h = threadIdx.x;
+  if (tid < HEADS) {
     float M = -INFINITY, L = 0.f;
-    for (int i = 0; i < kWarps; i++) M = fmaxf(M, m[i][h]);
-    for (int i = 0; i < kWarps; i++)
-      if (m[i][h] != -INFINITY || l[i][h] != 0.f) L += l[i][h] * exp2f(m[i][h] - M);
-    mc[h] = M;
-    lc[h] = L;
+    for (int i = 0; i < kWarps; i++) M = fmaxf(M, m[i][tid]);
+    for (int i = 0; i < kWarps; i++) {
+      const float f = l[i][tid] != 0.f ? exp2f(m[i][tid] - M) : 0.f;
+      factor[i][tid] = f;
+      L = fmaf(l[i][tid], f, L);
+    }
+    mc[tid] = M;
+    lc[tid] = L;
   }
-  for (int i = threadIdx.x; i < HEADS * DT; i += kThreads) {
+  __syncthreads();
+  for (int i = tid; i < w.heads * DT; i += kThreads) {
     const int h = i / DT;
-    float M = -INFINITY, acc = 0.f;
-    for (int k = 0; k < kWarps; k++) M = fmaxf(M, m[k][h]);
-    for (int k = 0; k < kWarps; k++)
-      if (l[k][h] != 0.f) acc += o[k * HEADS * DT + i] * exp2f(m[k][h] - M);
+    float acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWarps; k++) {
+      const float f = factor[k][h];
+      if (f != 0.f) acc = fmaf(o[k * HEADS * DT + i], f, acc);
+    }
     o[i] = acc;
   }
-  T* out = (T*)g.out;
   cg::cluster_group cl = cg::this_cluster();
   if (cluster > 1) cl.sync();
   else __syncthreads();
-  for (int i = rank * kThreads + threadIdx.x; i < w.heads * DT; i += cluster * kThreads) {
+  T* out = (T*)g.out;
+  for (int i = rank * kThreads + tid; i < w.heads * DT; i += cluster * kThreads) {
     const int h = i / DT, e = i - h * DT;
     if (e >= g.d) continue;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int r = 0; r < cluster; r++) M = fmaxf(M, *cl.map_shared_rank(&mc[h], r));
-    for (int r = 0; r < cluster; r++) {
-      const float lr = *cl.map_shared_rank(&lc[h], r);
-      if (lr == 0.f) continue;  // nothing seen there
-      const float a = exp2f(*cl.map_shared_rank(&mc[h], r) - M);
-      L += lr * a;
-      acc += *cl.map_shared_rank(o + i, r) * a;
+    float y = o[i], L = lc[h];
+    if (cluster > 1) {
+      // all remote loads at once: one trip over the cluster's network for most threads
+      float mr[kMaxCluster], lr[kMaxCluster], yr[kMaxCluster], M = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; r++) {
+        mr[r] = -INFINITY;
+        lr[r] = yr[r] = 0.f;
+        if (r < cluster) {
+          mr[r] = *cl.map_shared_rank(&mc[h], r);
+          lr[r] = *cl.map_shared_rank(&lc[h], r);
+          yr[r] = *cl.map_shared_rank(o + i, r);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; r++) M = fmaxf(M, mr[r]);
+      y = L = 0.f;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; r++) {
+        const float f = lr[r] != 0.f ? exp2f(mr[r] - M) : 0.f;
+        L = fmaf(lr[r], f, L);
+        if (f != 0.f) y = fmaf(yr[r], f, y);
+      }
     }
-    const float y = L != 0.f ? acc / L : 0.f;
+    y = L != 0.f ? y / L : 0.f;
     T* at = out + ((int64_t)w.b * g.H + w.head(g, h)) * g.d + e;
     if constexpr (sizeof(T) == 2) *at = __float2bfloat16_rn(y);
     else *at = y;
@@ -524,24 +547,32 @@ zl_status launch_decode_selected_fast(zl_ctx* ctx, const void* q, const void* k_
     return ZL_ERR_UNSUPPORTED;
   const int group = H / Hkv;
   // query heads that share a read of the keys and values
-  const int most = dtype == ZL_BF16 ? 8 : d <= 128 ? 4 : 2;
+  const int most = dtype == ZL_BF16 || d <= 128 ? 8 : 4;
   const int subs = (group + most - 1) / most, per_sub = (group + subs - 1) / subs;
   SelArgs g{q, k_pool, v_pool, block_tables, seq_lens, selected, out, H, Hkv, d, bs, max_blocks, max_selected,
             num_blocks, scale * 1.4426950408889634f, map == ZL_GQA_MODULO, group, subs, per_sub, ctx->d_status};
   const int64_t jobs = (int64_t)B * Hkv * subs;
-  // CTAs per list: as many as one wave of the GPU has room for (two to an SM), while each
-  // warp has a tile of its own
-  const int64_t tokens = (int64_t)max_selected * bs;
+  // CTAs per list: as many as one wave of the GPU has room for, while each warp has a tile or
+  // two of its own
+  const int64_t tokens = (int64_t)max_selected * bs, room = (d <= 128 ? 2 : 1) * (int64_t)ctx->num_sms;
   int cluster = 1;
-  while (cluster < kMaxCluster && jobs * cluster <= ctx->num_sms && tokens >= cluster * 128) cluster *= 2;
+  while (cluster < kMaxCluster && 2 * jobs * cluster <= room && tokens >= cluster * 128) cluster *= 2;
   if (jobs * cluster > INT32_MAX) return ZL_ERR_UNSUPPORTED;
   if (dtype == ZL_BF16)
     return d <= 64    ? launch(ctx, selected_mma_kernel<64, 4>, ring_bytes(128, 16, 4), g, jobs, cluster, st)
            : d <= 128 ? launch(ctx, selected_mma_kernel<128, 3>, ring_bytes(256, 16, 3), g, jobs, cluster, st)
                       : launch(ctx, selected_mma_kernel<256, 3>, ring_bytes(512, 16, 3), g, jobs, cluster, st);
-  return d <= 64    ? launch(ctx, selected_f32_kernel<2, 4, 4>, ring_bytes(256, 8, 4), g, jobs, cluster, st)
-         : d <= 128 ? launch(ctx, selected_f32_kernel<4, 4, 3>, ring_bytes(512, 8, 3), g, jobs, cluster, st)
-                    : launch(ctx, selected_f32_kernel<8, 2, 3>, ring_bytes(1024, 8, 3), g, jobs, cluster, st);
+  // NV, heads at a time, ring slots
+  if (d <= 64)
+    return per_sub <= 2   ? launch(ctx, selected_f32_kernel<2, 2, 4>, ring_bytes(256, 8, 4), g, jobs, cluster, st)
+           : per_sub <= 4 ? launch(ctx, selected_f32_kernel<2, 4, 4>, ring_bytes(256, 8, 4), g, jobs, cluster, st)
+                          : launch(ctx, selected_f32_kernel<2, 8, 4>, ring_bytes(256, 8, 4), g, jobs, cluster, st);
+  if (d <= 128)
+    return per_sub <= 2   ? launch(ctx, selected_f32_kernel<4, 2, 3>, ring_bytes(512, 8, 3), g, jobs, cluster, st)
+           : per_sub <= 4 ? launch(ctx, selected_f32_kernel<4, 4, 3>, ring_bytes(512, 8, 3), g, jobs, cluster, st)
+                          : launch(ctx, selected_f32_kernel<4, 8, 3>, ring_bytes(512, 8, 3), g, jobs, cluster, st);
+  return per_sub <= 2 ? launch(ctx, selected_f32_kernel<8, 2, 3>, ring_bytes(1024, 8, 3), g, jobs, cluster, st)
+                      : launch(ctx, selected_f32_kernel<8, 4, 3>, ring_bytes(1024, 8, 3), g, jobs, cluster, st);
 }
 
 }  // namespace zl

@@ -127,11 +127,11 @@ __device__ __forceinline__ bool table_columns(const StepArgs& g, int i, int c, i
   return bad;
 }
 
-// A CTA takes units: N columns per thread and step of a table row's stretch of kStretch
-// columns, then stretches of kThreads token rows.
-constexpr int kStretch = 8192;
+// A CTA takes units: kThreads / lanes stretches of table rows at a time, `lanes` threads (a
+// power of two) to a stretch of lanes * N * kDepth columns, then stretches of kThreads token rows.
+constexpr int kDepth = 4;
 template <int N>
-__global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
+__global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g, int log_lanes) {
   extern __shared__ int32_t sh[];
   const int n = g.num_seqs;
   int32_t* cu = sh;                                             // [n + 1] first token row
@@ -181,30 +181,30 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g) {
       g.last_rows[i] = max(min(cu[i + 1], cap) - 1, 0);
     }
   }
-  const int stretches = (g.max_blocks + kStretch - 1) / kStretch;
-  // fewer than 2^32: at most 2^13 requests of 2^18 stretches (a table row of fewer than 2^30 columns),
-  // and fewer than 2^24 stretches of tokens
-  const uint32_t tables = (uint32_t)n * stretches, units = tables + (uint32_t)((g.num_tokens + kThreads - 1) / kThreads);
+  const int lanes = 1 << log_lanes, width = lanes * N * kDepth, stretches = (g.max_blocks + width - 1) / width, at_once = kThreads >> log_lanes;
+  // fewer than 2^32: at most 2^13 requests of 2^17 stretches (a table row of at most 2^30 columns, and all
+  // threads to a stretch of such), and fewer than 2^23 stretches of tokens
+  const uint32_t pieces = (uint32_t)n * stretches, tables = (pieces + at_once - 1) / at_once;
+  const uint32_t units = tables + (uint32_t)((g.num_tokens + kThreads - 1) / kThreads);
   for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
     if (u < tables) {
-      const int i = (int)(u / stretches), c0 = (int)(u - (uint32_t)i * stretches) * kStretch;
+      const uint32_t piece = u * at_once + (threadIdx.x >> log_lanes);
+      if (piece >= pieces) continue;
+      const int i = (int)(piece / stretches), c0 = (int)(piece - (uint32_t)i * stretches) * width;
       const int r = row[i];
       int had = 0, has = 0;
       if (r >= 0) {
         had = zl::blocks_of32(ctx[i], g.bs);
         has = zl::blocks_of32(ctx[i] + cu[i + 1] - cu[i], g.bs);
       }
-      constexpr int STEP = kThreads * N, DEPTH = 4;
-      const int end = min(c0 + kStretch, g.max_blocks);
-      for (int c = c0 + threadIdx.x * N; c < end; c += STEP * DEPTH) {
-        Ids<N> old[DEPTH];  // all loads before the first store
+      const int c = c0 + (threadIdx.x & (lanes - 1)) * N, step = lanes * N;
+      Ids<N> old[kDepth];  // all loads before the first store
 #pragma unroll
-        for (int k = 0; k < DEPTH; k++)
-          if (c + k * STEP < min(had, end)) old[k] = load_ids<N>(g.seq_blocks + (int64_t)r * g.max_blocks + c + k * STEP);
+      for (int k = 0; k < kDepth; k++)
+        if (c + k * step < min(had, g.max_blocks)) old[k] = load_ids<N>(g.seq_blocks + (int64_t)r * g.max_blocks + c + k * step);
 #pragma unroll
-        for (int k = 0; k < DEPTH; k++)
-          if (c + k * STEP < end) bad |= table_columns<N>(g, i, c + k * STEP, r, had, has, fresh[i], old[k]);
-      }
+      for (int k = 0; k < kDepth; k++)
+        if (c + k * step < g.max_blocks) bad |= table_columns<N>(g, i, c + k * step, r, had, has, fresh[i], old[k]);
       continue;
     }
     const int64_t t = (int64_t)(u - tables) * kThreads + threadIdx.x;
@@ -271,10 +271,20 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   const auto kernel = vec ? step_tables_kernel<4> : step_tables_kernel<1>;
   if (smem > 32 * 1024)  // with the static part it may pass 48 KB
     ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  int64_t blocks = (int64_t)num_seqs * ((max_blocks_per_seq + kStretch - 1) / kStretch) + (num_tokens + kThreads - 1) / kThreads;
+  // Threads to a table row: one step of each while all rows then fit the GPU at once (the
+  // shortest way for a small step), kDepth steps otherwise.
+  const int wide = vec ? 4 : 1;
   const int64_t most = 2 * ctx->num_sms;
+  int log_lanes = 3;
+  while (1 << log_lanes < kThreads && (int64_t)wide << log_lanes < max_blocks_per_seq) log_lanes++;
+  while (log_lanes > 3 && ((int64_t)num_seqs << log_lanes) > most * kThreads &&
+         ((int64_t)wide * kDepth << (log_lanes - 1)) >= max_blocks_per_seq)
+    log_lanes--;
+  const int64_t width = (int64_t)wide * kDepth << log_lanes, lanes = 1 << log_lanes;
+  const int64_t pieces = num_seqs * ((max_blocks_per_seq + width - 1) / width);
+  int64_t blocks = (pieces * lanes + kThreads - 1) / kThreads + (num_tokens + kThreads - 1) / kThreads;
   blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
-  kernel<<<(unsigned)blocks, kThreads, smem, S(stream)>>>(g);
+  kernel<<<(unsigned)blocks, kThreads, smem, S(stream)>>>(g, log_lanes);
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }
