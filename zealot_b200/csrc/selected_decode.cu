@@ -558,21 +558,34 @@ zl_status launch_decode_selected_fast(zl_ctx* ctx, const void* q, const void* k_
   int cluster = 1;
   while (cluster < kMaxCluster && 2 * jobs * cluster <= room && tokens >= cluster * 128) cluster *= 2;
   if (jobs * cluster > INT32_MAX) return ZL_ERR_UNSUPPORTED;
-  if (dtype == ZL_BF16)
-    return d <= 64    ? launch(ctx, selected_mma_kernel<64, 4>, ring_bytes(128, 16, 4), g, jobs, cluster, st)
-           : d <= 128 ? launch(ctx, selected_mma_kernel<128, 3>, ring_bytes(256, 16, 3), g, jobs, cluster, st)
-                      : launch(ctx, selected_mma_kernel<256, 3>, ring_bytes(512, 16, 3), g, jobs, cluster, st);
-  // NV, heads at a time, ring slots
+  // Heads of 65 to 128 elements: two CTAs of three ring slots or three of two to an SM, the
+  // same bytes on their way but other rounds. A round that fills the SMs costs its bytes, the
+  // last one at least a CTA's own latency, which is that of 1.25 CTAs to an SM (measured with
+  // 1 MB lists: 2 x 148 CTAs 48 us, 148 or fewer 30 us). At 384 lists the two give 86 and 76 us,
+  // at 512 89 and 98 us.
+  auto rounds = [&](int64_t ctas) {
+    const int64_t rest = jobs * cluster % ctas, least = ctx->num_sms * 5 / 4;
+    return jobs * cluster - rest + (rest == 0 ? 0 : rest > least ? rest : least);
+  };
+  const bool three = rounds(3 * ctx->num_sms) < rounds(2 * ctx->num_sms);
+  auto run = [&](void (*kernel)(SelArgs, int), size_t smem) { return launch(ctx, kernel, smem, g, jobs, cluster, st); };
+  if (dtype == ZL_BF16) {
+    if (d <= 64) return run(selected_mma_kernel<64, 4>, ring_bytes(128, 16, 4));
+    if (d <= 128)
+      return three ? run(selected_mma_kernel<128, 2>, ring_bytes(256, 16, 2))
+                   : run(selected_mma_kernel<128, 3>, ring_bytes(256, 16, 3));
+    return run(selected_mma_kernel<256, 3>, ring_bytes(512, 16, 3));
+  }
+  // elements / 32, heads at a time, ring slots
   if (d <= 64)
-    return per_sub <= 2   ? launch(ctx, selected_f32_kernel<2, 2, 4>, ring_bytes(256, 8, 4), g, jobs, cluster, st)
-           : per_sub <= 4 ? launch(ctx, selected_f32_kernel<2, 4, 4>, ring_bytes(256, 8, 4), g, jobs, cluster, st)
-                          : launch(ctx, selected_f32_kernel<2, 8, 4>, ring_bytes(256, 8, 4), g, jobs, cluster, st);
-  if (d <= 128)
-    return per_sub <= 2   ? launch(ctx, selected_f32_kernel<4, 2, 3>, ring_bytes(512, 8, 3), g, jobs, cluster, st)
-           : per_sub <= 4 ? launch(ctx, selected_f32_kernel<4, 4, 3>, ring_bytes(512, 8, 3), g, jobs, cluster, st)
-                          : launch(ctx, selected_f32_kernel<4, 8, 3>, ring_bytes(512, 8, 3), g, jobs, cluster, st);
-  return per_sub <= 2 ? launch(ctx, selected_f32_kernel<8, 2, 3>, ring_bytes(1024, 8, 3), g, jobs, cluster, st)
-                      : launch(ctx, selected_f32_kernel<8, 4, 3>, ring_bytes(1024, 8, 3), g, jobs, cluster, st);
+    return per_sub <= 2   ? run(selected_f32_kernel<2, 2, 4>, ring_bytes(256, 8, 4))
+           : per_sub <= 4 ? run(selected_f32_kernel<2, 4, 4>, ring_bytes(256, 8, 4))
+                          : run(selected_f32_kernel<2, 8, 4>, ring_bytes(256, 8, 4));
+  if (d <= 128 && per_sub <= 4)
+    return three ? run(per_sub <= 2 ? selected_f32_kernel<4, 2, 2> : selected_f32_kernel<4, 4, 2>, ring_bytes(512, 8, 2))
+                 : run(per_sub <= 2 ? selected_f32_kernel<4, 2, 3> : selected_f32_kernel<4, 4, 3>, ring_bytes(512, 8, 3));
+  if (d <= 128) return run(selected_f32_kernel<4, 8, 3>, ring_bytes(512, 8, 3));  // its registers allow two to an SM
+  return run(per_sub <= 2 ? selected_f32_kernel<8, 2, 3> : selected_f32_kernel<8, 4, 3>, ring_bytes(1024, 8, 3));
 }
 
 }  // namespace zl
