@@ -492,8 +492,7 @@ __device__ __forceinline__ uint32_t limit_by_counts(const uint32_t (&key)[R], in
 }
 
 // The same for many keys: three digits of 11, 11 and 10 bits, a histogram in shared
-// memory for each over the keys that share the digits before it. A warp whose keys all
-// fall into one bin adds them with one atomic.
+// memory for each over the keys that share the digits before it.
 template <int THREADS, int R>
 __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], int m) {
   constexpr int BINS = 2048, PER = BINS / THREADS, W = THREADS / 32;
@@ -513,14 +512,7 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
     for (int i = 0; i < R; i++) {
       const bool in = key[i] != 0 && (key[i] & mask) == limit;
       const int bin = key[i] >> shift & ((1 << width) - 1);
-      const unsigned who = __ballot_sync(0xffffffffu, in);
-      if (!who) continue;
-      const int one = __shfl_sync(0xffffffffu, bin, __ffs(who) - 1);
-      if (__all_sync(0xffffffffu, !in || bin == one)) {
-        if (lane == 0) atomicAdd(&hist[one], __popc(who));
-      } else if (in) {
-        atomicAdd(&hist[bin], 1);
-      }
+      if (in) atomicAdd(&hist[bin], 1);
     }
     __syncthreads();
     // sums from the top bin down: this thread has bins [top - PER + 1, top]
@@ -832,8 +824,9 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
   const unsigned n = (unsigned)rows;
   const cudaStream_t st = S(stream);
   if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4, false><<<n, 128, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 2048) select_reg_kernel<256, 8, true><<<n, 256, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 8192) select_reg_kernel<512, 16, true><<<n, 512, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 2048) select_reg_kernel<512, 4, true><<<n, 512, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 8192) select_reg_kernel<1024, 8, true><<<n, 1024, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 16384) select_reg_kernel<1024, 16, true><<<n, 1024, 0, st>>>(g);
   else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24, true><<<n, 1024, 0, st>>>(g);
   else select_kernel<<<n, kSelThreads, 0, st>>>(g);
   ZL_LAUNCH_CHECK(ctx);
