@@ -129,55 +129,62 @@ __device__ __forceinline__ void merge(uint4& lo, uint4& hi, const uint4& a, cons
   hi.w = word_max<T>(hi.w, b.w);
 }
 
-// Rows of 16-byte chunks, up to 32 CH of them: one warp per block and kv head, LPR
-// lanes to a row (a power of two), CH chunks to a lane, 32 / LPR rows at a time and
-// eight such loads in flight. The lanes of all sequences' heads run through the
-// blocks together: head h of block j is unit j * Hkv + h, so a step that touches one
-// block per sequence keeps the warps of one CTA busy.
+// Rows of 16-byte chunks, up to 32 CH of them: one warp per block and kv head, LPR lanes
+// to a row (a power of two), CH chunks to a lane, ROWS = 32 / LPR * DEPTH rows at a time,
+// all of whose loads are in flight at once. A warp keeps to one head; the warps of the
+// heads of one block, whose keys lie side by side, are neighbours.
 template <typename T, int LPR, int CH>
 __global__ void __launch_bounds__(256, 4)
 bounds_vec_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __restrict__ tok_begin,
                   T* __restrict__ bounds) {
-  constexpr int RPL = 32 / LPR, DEPTH = CH == 1 ? 8 : 4, VEC = 16 / sizeof(T);
+  constexpr int RPL = 32 / LPR, DEPTH = CH == 1 ? 8 : 4, ROWS = RPL * DEPTH, VEC = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, sub = lane / LPR, ch = lane % LPR;
-  const int chunks = g.d / VEC;
+  const int chunks = g.d / VEC, warps = gridDim.x * 8, step = warps / g.Hkv;  // blocks at a time
+  const int gw = blockIdx.x * 8 + (threadIdx.x >> 5), j0 = gw / g.Hkv, h = gw - j0 * g.Hkv;
+  if (j0 >= step) return;
+  const bool mine[2] = {ch < chunks, ch + LPR < chunks};
+  const int64_t block = (int64_t)g.Hkv * g.bs * chunks, head = (int64_t)h * g.bs * chunks;  // in 16-byte chunks
+  const uint4* pool = reinterpret_cast<const uint4*>(k_pool) + head + ch;
+  uint4* out0 = reinterpret_cast<uint4*>(bounds) + (int64_t)h * 2 * chunks + ch;
   for (int b = blockIdx.y; b < g.B; b += gridDim.y) {
-    const int64_t len = seq_len(g, b), n = zl::blocks_of(len, g.bs);
-    const int64_t first = tok_begin ? max(tok_begin[b], 0) / g.bs : 0;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    int64_t u = first * g.Hkv + blockIdx.x * 8 + (threadIdx.x >> 5);
-    int64_t id = u < n * g.Hkv ? block_id(g, b, u / g.Hkv) : -1, next;
-    for (; u < n * g.Hkv; u += step, id = next) {
-      const int64_t j = u / g.Hkv;
-      const int h = (int)(u - j * g.Hkv);
-      next = u + step < n * g.Hkv ? block_id(g, b, (u + step) / g.Hkv) : -1;
+    const int64_t len = seq_len(g, b);
+    const int n = (int)zl::blocks_of(len, g.bs);
+    const int64_t first = (tok_begin ? max(tok_begin[b], 0) / g.bs : 0) + (int64_t)j0;
+    if (first >= n) continue;
+    int j = (int)first;
+    int64_t id = block_id(g, b, j), next;
+    for (; j < n; j += step, id = next) {
+      next = j + step < n ? block_id(g, b, j + step) : -1;
       if (id < 0) continue;
-      const uint4* rows = reinterpret_cast<const uint4*>(k_pool) + zl::pool_row(id, g.num_blocks, g.Hkv, h, g.bs, 0) * chunks;
-      const int toks = (int)min((int64_t)g.bs, len - j * g.bs);
-      uint4* out = reinterpret_cast<uint4*>(bounds) + (id * g.Hkv + h) * 2 * chunks;
+      const uint4* rows = pool + id * block;
+      const int toks = (int)min((int64_t)g.bs, len - (int64_t)j * g.bs);
       uint4 lo[CH], hi[CH];
-      // every lane starts from a row of its own, or from the last where the block has fewer
-#pragma unroll
-      for (int c = 0; c < CH; c++) {
-        const int x = ch + c * LPR;
-        lo[c] = make_uint4(0, 0, 0, 0);
-        if (x < chunks) lo[c] = __ldg(rows + (int64_t)min(sub, toks - 1) * chunks + x);
-        hi[c] = lo[c];
-      }
-      for (int t = RPL; t < toks; t += RPL * DEPTH) {
+      for (int t = 0; t < toks; t += ROWS) {
         uint4 v[DEPTH][CH];
+        if (t + ROWS <= toks) {
+          const uint4* p = rows + (int64_t)(t + sub) * chunks;
 #pragma unroll
-        for (int k = 0; k < DEPTH; k++)
+          for (int k = 0; k < DEPTH; k++, p += RPL * chunks)
 #pragma unroll
-          for (int c = 0; c < CH; c++) {
-            const int r = min(t + k * RPL + sub, toks - 1), x = ch + c * LPR;  // a row twice changes nothing
-            v[k][c] = x < chunks ? __ldg(rows + (int64_t)r * chunks + x) : make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < CH; c++) v[k][c] = mine[c] ? __ldg(p + c * LPR) : make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int k = 0; k < DEPTH; k++) {
+            const int r = min(t + k * RPL + sub, toks - 1);  // a row twice changes nothing
+#pragma unroll
+            for (int c = 0; c < CH; c++)
+              v[k][c] = mine[c] ? __ldg(rows + (int64_t)r * chunks + c * LPR) : make_uint4(0, 0, 0, 0);
           }
+        }
 #pragma unroll
-        for (int k = 0; k < DEPTH; k++)
+        for (int c = 0; c < CH; c++) {
+          if (t == 0) lo[c] = hi[c] = v[0][c];
+          else merge<T>(lo[c], hi[c], v[0][c], v[0][c]);
 #pragma unroll
-          for (int c = 0; c < CH; c++) merge<T>(lo[c], hi[c], v[k][c], v[k][c]);
+          for (int k = 1; k < DEPTH; k++) merge<T>(lo[c], hi[c], v[k][c], v[k][c]);
+        }
       }
+      uint4* out = out0 + id * g.Hkv * 2 * chunks;
 #pragma unroll
       for (int c = 0; c < CH; c++) {
 #pragma unroll
@@ -193,10 +200,9 @@ bounds_vec_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __re
           z.w = __shfl_xor_sync(0xffffffffu, hi[c].w, o);
           merge<T>(lo[c], hi[c], a, z);
         }
-        const int x = ch + c * LPR;
-        if (x < chunks && sub == 0) {
-          out[x] = lo[c];
-          out[chunks + x] = hi[c];
+        if (mine[c] && sub == 0) {
+          out[c * LPR] = lo[c];
+          out[chunks + c * LPR] = hi[c];
         }
       }
     }
@@ -383,9 +389,17 @@ __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts,
       sides[1][k][e] = max_nan(f, 0.f);
     }
     __syncthreads();
-    for (int tile = part * 8 + (threadIdx.x >> 5); tile < tiles; tile += parts * 8) {
-      const int j = tile * 4 + tg;
-      const int64_t id = j < nb ? block_id(g, b, j) : -1;
+    const int32_t* table = g.tables + (int64_t)b * g.max_blocks;
+    const T* mine = bounds + (int64_t)h * 2 * g.d + li * VEC;
+    const int64_t block = (int64_t)g.Hkv * 2 * g.d;
+    int j = (part * 8 + (threadIdx.x >> 5)) * 4 + tg;
+    int32_t id = j < nb ? table[j] : -1, next;
+    for (int tile = part * 8 + (threadIdx.x >> 5); tile < tiles; tile += parts * 8, j += parts * 32, id = next) {
+      next = j + parts * 32 < nb ? table[j + parts * 32] : -1;
+      if (id >= g.num_blocks) {
+        atomicOr(g.status, ZL_DEV_OOB);
+        id = -1;
+      }
       uint4 v[2][NV];
 #pragma unroll
       for (int z = 0; z < 2; z++)
@@ -393,7 +407,7 @@ __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts,
         for (int k = 0; k < NV; k++) {
           v[z][k] = make_uint4(0, 0, 0, 0);
           if (id >= 0 && (k * 8 + li) * VEC < g.d)
-            v[z][k] = __ldg(reinterpret_cast<const uint4*>(bounds + ((id * g.Hkv + h) * 2 + z) * g.d + (k * 8 + li) * VEC));
+            v[z][k] = __ldg(reinterpret_cast<const uint4*>(mine + id * block + z * g.d + k * 8 * VEC));
         }
       float best = -INFINITY;
       for (int i = 0; i < heads; i++) {
@@ -549,7 +563,7 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
 // Tables of up to THREADS R blocks: each thread keeps R keys, key i of thread t being
 // block i * THREADS + t.
 template <int THREADS, int R, bool DIGITS>
-__global__ void __launch_bounds__(THREADS) select_reg_kernel(SelectArgs g) {
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 4 : 1) select_reg_kernel(SelectArgs g) {
   constexpr int W = THREADS / 32;
   __shared__ uint32_t before[R * W];
   __shared__ int total_above;
@@ -681,18 +695,17 @@ dim3 grid_of(int64_t units, int64_t blocks) {
   return dim3((unsigned)(x < 1 ? 1 : x > 4096 ? 4096 : x), (unsigned)y);
 }
 
-constexpr int kBoundsWaves = 32;
+constexpr int kBoundsWaves = 16;
 template <typename T>
 void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* tok_begin, void* bounds, int num_sms,
                        cudaStream_t st) {
   const int chunks = g.d * (int)sizeof(T) / 16;
-  // Every block of long prompts, or the few that a step's tokens touched: with
-  // tok_begin the grid is one that an idle GPU starts at once, and its CTAs go on
-  // from block to block where there are more.
+  // CTAs for each sequence: with tok_begin, which is a step's few tokens or a chunk of a
+  // prompt, some 4 to an SM in all; for whole prompts of any lengths some kBoundsWaves.
   int64_t x = ((int64_t)g.max_blocks * g.Hkv + 7) / 8;
-  const int64_t few = ((tok_begin ? 4 : kBoundsWaves) * (int64_t)num_sms + g.B - 1) / g.B;
-  if (x > few) x = few;
-  if (x > INT32_MAX) x = INT32_MAX;
+  const int64_t few = ((tok_begin ? 4 : kBoundsWaves) * (int64_t)num_sms + g.B - 1) / g.B, least = (g.Hkv + 7) / 8;
+  x = x > few ? few : x;
+  x = x < least ? least : x;
   const dim3 grid((unsigned)x, (unsigned)(g.B < 65535 ? g.B : 65535));
   const T* k = (const T*)k_pool;
   T* o = (T*)bounds;
@@ -823,8 +836,10 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
                      num_first, num_last, ctx->d_status};
   const unsigned n = (unsigned)rows;
   const cudaStream_t st = S(stream);
+  const bool many = rows > 2 * ctx->num_sms;  // more rows than CTAs of 1024 threads at once
   if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4, false><<<n, 128, 0, st>>>(g);
   else if (max_blocks_per_seq <= 2048) select_reg_kernel<512, 4, true><<<n, 512, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 8192 && many) select_reg_kernel<512, 16, true><<<n, 512, 0, st>>>(g);
   else if (max_blocks_per_seq <= 8192) select_reg_kernel<1024, 8, true><<<n, 1024, 0, st>>>(g);
   else if (max_blocks_per_seq <= 16384) select_reg_kernel<1024, 16, true><<<n, 1024, 0, st>>>(g);
   else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24, true><<<n, 1024, 0, st>>>(g);
