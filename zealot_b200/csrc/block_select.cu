@@ -252,7 +252,7 @@ scores_elem_kernel(PagedArgs g, const T* __restrict__ q, const T* __restrict__ b
 // Each warp keeps a ring of ST tiles (16 blocks' bounds) in shared memory, filled by
 // asynchronous copies, and the block ids of one tile more. Chunk ch of row r lies at
 // ch ^ swz(r), so that the two rows that a quarter warp reads do not meet in a bank.
-constexpr int kScoreWarps = 4, kScoreCtas = 3;
+constexpr int kScoreWarps = 1, kScoreCtas = 12;
 template <int DT, int ST>
 __global__ void __launch_bounds__(kScoreWarps * 32)
 scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
