@@ -123,6 +123,23 @@ def test_selected_odd_lists(ctx, d, bs, bf16):
 
 
 @pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("d,B", [(64, 40), (128, 3)])
+def test_selected_long_lists(ctx, d, B, bf16):
+    """Lists of more blocks than a CTA resolves at a time (512), ending in its first part, in its second
+    and not at all; many lists (one CTA each) and few (eight CTAs each)."""
+    rng = np.random.default_rng(B)
+    top = 700 if B > 8 else 4800
+    lens = [top + 60] * B
+    q, kp, vp, table, lens = decode_case(rng, B, lens, 8, 4, d, 1, B * (top + 60))
+    sel = lists(rng, lens, 4, 1, top)
+    sel[0, :, 511] = -1
+    sel[1, :, 512] = -1
+    sel[1, 0, 600] = -2
+    sel[2, 1, 600] = -1
+    check(ctx, q, kp, vp, table, lens, sel, bf16)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
 def test_selected_bad_ids(ctx, bf16):
     rng = np.random.default_rng(9)
     q, kp, vp, table, lens = decode_case(rng, 3, [200, 200, 200], 8, 2, 128, 16, 60)

@@ -1,0 +1,73 @@
+"""Decoder steps whose batch StepTables built on the device against the same steps laid out on
+the host by StepBatch.build: equal bytes in logits and pools, over a prompt step and decode steps
+in which requests come and go."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def test_decoder_steps_from_device_tables(ctx):
+    import torch
+    import zealot_b200 as zb
+    from zealot_b200.decoder import Decoder, DecoderConfig, StepBatch, StepTables, random_weights
+    cfg = DecoderConfig(num_layers=2, hidden=512, num_heads=4, num_kv_heads=2, head_dim=128, intermediate=1024, vocab=1000)
+    dec = Decoder(ctx, cfg, random_weights(cfg, 3))
+    rng = np.random.default_rng(1)
+    nb, bs, mb = 64, 16, 6
+    bm = zb.BlockManager(nb, bs)
+    steps = StepTables(ctx, num_rows=5, max_blocks_per_seq=mb, max_seqs=5, max_tokens=200, block_size=bs, num_blocks=nb)
+    pools, pools_host = dec.new_pools(nb, bs), dec.new_pools(nb, bs)
+    seqs = {}  # row -> (length, block ids)
+
+    def step(new, old):
+        """new: {row: prompt length}, old: rows that decode one token."""
+        rows = [*new, *old]
+        context = [0] * len(new) + [seqs[r][0] for r in old]
+        query = [*new.values()] + [1] * len(old)
+        for r in new:
+            seqs[r] = (0, [])
+        ids = []
+        for r, c, q in zip(rows, context, query):
+            ids += [bm.allocate().block_id for _ in range(steps.blocks_needed(c, q))]
+            seqs[r] = (c + q, seqs[r][1] + ids[len(ids) - steps.blocks_needed(c, q):])
+        toks = [rng.integers(0, cfg.vocab, q) for q in query]
+        table = np.full((len(old), mb), -1, np.int32)
+        for i, r in enumerate(old):
+            table[i, :len(seqs[r][1])] = seqs[r][1]
+        host = StepBatch.build(toks[:len(new)], [int(t[0]) for t in toks[len(new):]], table, [seqs[r][0] for r in old],
+                               [seqs[r][1] for r in new], bs)
+        dev = steps.build(torch.from_numpy(np.concatenate(toks)).cuda(), rows, context, query, ids, len(new))
+        a = dec.step(dev, *pools, bs)
+        b = dec.step(host, *pools_host, bs)
+        ctx.check_status()
+        assert torch.equal(a, b)
+        for x, y in zip([*pools[0], *pools[1]], [*pools_host[0], *pools_host[1]]):
+            assert torch.equal(x, y)
+
+    step({3: 40, 0: 1, 2: 17}, [])
+    for _ in range(10):
+        step({}, [0, 3, 2])
+    step({4: 33, 1: 16}, [2, 0])        # row 3 waits, two prompts arrive
+    del seqs[0]                         # a finished sequence's row is taken over
+    step({0: 20}, [3, 1, 4, 2])
+    for _ in range(8):
+        step({}, [0, 1, 2, 3, 4])
+
+
+def test_step_tables_build_refusals(ctx):
+    import torch
+    import zealot_b200 as zb
+    from zealot_b200.decoder import StepTables
+    steps = StepTables(ctx, 4, 4, 2, 10, 16, 32)
+    toks = lambda n: torch.zeros(n, dtype=torch.int64, device="cuda")
+    with pytest.raises(zb.InvalidArgument):
+        steps.build(toks(3), [0], [1], [3], [0], 1)          # a prompt chunk that does not start at 0
+    with pytest.raises(zb.InvalidArgument):
+        steps.build(toks(2), [0], [1], [2], [], 0)           # a decode row of two tokens
+    with pytest.raises(zb.InvalidArgument):
+        steps.build(toks(1), [0], [0], [3], [0], 1)          # tokens missing
+    with pytest.raises(zb.InvalidArgument):
+        steps.build(toks(3), [0, 1, 2], [1, 1, 1], [1, 1, 1], [], 0)  # three requests
+    with pytest.raises(zb.InvalidArgument):
+        steps.build(toks(11), [0], [0], [11], [0], 1)        # eleven tokens

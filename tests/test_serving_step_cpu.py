@@ -21,7 +21,7 @@ def _refused(lib, name, base, code, text, **change):
     assert text in lib.zl_last_error().decode(), lib.zl_last_error()
 
 
-TABLES = dict(ctx=None, seq_blocks=P, num_rows=4, rows=P, context_lens=P, query_lens=P, new_blocks=P, num_new=1,
+TABLES = dict(ctx=None, seq_blocks=8 * P, num_rows=4, rows=P, context_lens=P, query_lens=P, new_blocks=P, num_new=1,
               block_tables=P, cu_seqlens=P, seq_lens=P, positions=P, slot_mapping=P, last_rows=P, num_seqs=2,
               num_tokens=3, max_blocks=8, block_size=16, num_blocks=64, stream=None)
 
@@ -31,7 +31,9 @@ TABLES = dict(ctx=None, seq_blocks=P, num_rows=4, rows=P, context_lens=P, query_
     (INVALID, "bad sizes", dict(num_seqs=-1)), (INVALID, "bad sizes", dict(num_rows=-1)),
     (INVALID, "bad sizes", dict(num_new=-1)), (INVALID, "bad sizes", dict(num_tokens=-1)),
     (INVALID, "bad sizes", dict(max_blocks=-1)), (INVALID, "bad sizes", dict(block_size=0)),
-    (INVALID, "bad sizes", dict(num_blocks=-1)), (INVALID, "2^31-1", dict(num_tokens=2**31)),
+    (INVALID, "bad sizes", dict(num_blocks=-1)), (INVALID, "2^31-1", dict(num_tokens=2**31)), (INVALID, "2^31-1", dict(num_tokens=2**31 - 1)),
+    (INVALID, "2^31-1", dict(max_blocks=2**30 + 1)), (INVALID, "overlaps", dict(seq_blocks=P)),
+    (INVALID, "overlaps", dict(seq_blocks=P + 2 * 8 * 4 - 4)), (INVALID, "overlaps", dict(seq_blocks=P - 4 * 8 * 4 + 4)),
     (INVALID, "2^31-1", dict(num_blocks=2**31)),
     (UNSUPPORTED, "at most", dict(num_seqs=8193, num_rows=9000)), (UNSUPPORTED, "at most", dict(num_rows=2**18 + 1)),
     (INVALID, "without `rows`", dict(rows=None, num_rows=1)),
@@ -79,6 +81,7 @@ SCORES = dict(ctx=None, q=P, bounds=P, tables=P, seq_lens=P, scores=P, B=2, H=8,
 @pytest.mark.parametrize("text,change", [
     ("null context", {}), ("dtype", dict(dtype=2)), ("head shape", dict(Hkv=0)), ("head shape", dict(d=0)),
     ("bad sizes", dict(B=-1)), ("bad sizes", dict(bs=0)), ("bad sizes", dict(max_blocks=-1)),
+    ("bad sizes", dict(max_blocks=2**30 + 1)),
     ("bad sizes", dict(num_blocks=-1)), ("null pointer", dict(tables=None)), ("null pointer", dict(seq_lens=None)),
     ("null pointer", dict(bounds=None))])
 def test_block_bounds_and_scores_refusals(lib, name, base, text, change):
@@ -99,6 +102,7 @@ SELECT = dict(ctx=None, scores=P, seq_lens=P, selected=P, B=2, Hkv=2, bs=16, max
 @pytest.mark.parametrize("text,change", [
     ("null context", {}), ("bad sizes", dict(B=-1)), ("bad sizes", dict(Hkv=0)), ("bad sizes", dict(bs=0)),
     ("bad sizes", dict(max_blocks=-1)), ("bad sizes", dict(max_selected=-1)), ("first", dict(num_first=-1)),
+    ("bad sizes", dict(max_blocks=2**30 + 1)), ("bad sizes", dict(max_selected=2**30 + 1)),
     ("first", dict(num_last=-1)), ("first", dict(num_first=3, num_last=2)), ("too large", dict(B=2**30, Hkv=2)),
     ("null pointer", dict(scores=None)), ("null pointer", dict(seq_lens=None)), ("null pointer", dict(selected=None))])
 def test_select_blocks_refusals(lib, text, change):
@@ -114,6 +118,7 @@ SELECTED = dict(ctx=None, q=P, k_pool=P, v_pool=P, tables=P, seq_lens=P, selecte
     (INVALID, "head shape", dict(d=0)), (UNSUPPORTED, "head_dim", dict(d=512)), (INVALID, "bad sizes", dict(B=-1)),
     (INVALID, "bad sizes", dict(bs=0)), (INVALID, "bad sizes", dict(max_blocks=-1)),
     (INVALID, "bad sizes", dict(num_blocks=-1)), (INVALID, "bad sizes", dict(max_selected=-1)),
+    (INVALID, "bad sizes", dict(max_selected=2**30 + 1)),
     (INVALID, "too large", dict(B=2**28, H=8)),
     *[(INVALID, "null pointer", {k: None}) for k in ("q", "k_pool", "v_pool", "tables", "seq_lens", "selected", "out")]])
 def test_paged_decode_selected_refusals(lib, code, text, change):

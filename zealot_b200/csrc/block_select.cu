@@ -683,7 +683,7 @@ zl_status check_paged(const char* who, int B, int H, int Hkv, int d, int bs, int
   if (!dtype_ok(dtype)) return set_error(ZL_ERR_INVALID_ARG, "%s: bad dtype %d", who, (int)dtype);
   if (H <= 0 || Hkv <= 0 || d <= 0 || H % Hkv)
     return set_error(ZL_ERR_INVALID_ARG, "%s: bad head shape H=%d Hkv=%d d=%d", who, H, Hkv, d);
-  if (B < 0 || bs <= 0 || max_blocks < 0 || num_blocks < 0)
+  if (B < 0 || bs <= 0 || max_blocks < 0 || max_blocks > 1 << 30 || num_blocks < 0)
     return set_error(ZL_ERR_INVALID_ARG, "%s: bad sizes B=%d bs=%d max_blocks=%d blocks=%lld", who, B, bs, max_blocks,
                      (long long)num_blocks);
   return ZL_OK;
@@ -819,7 +819,8 @@ zl_status zl_block_scores(zl_ctx* ctx, const void* q, const void* bounds, const 
 zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_lens, int32_t* selected, int num_seqs,
                            int num_kv_heads, int block_size, int max_blocks_per_seq, int max_selected, int num_first,
                            int num_last, zl_stream stream) {
-  if (num_seqs < 0 || num_kv_heads <= 0 || block_size <= 0 || max_blocks_per_seq < 0 || max_selected < 0)
+  if (num_seqs < 0 || num_kv_heads <= 0 || block_size <= 0 || max_blocks_per_seq < 0 ||
+      max_blocks_per_seq > 1 << 30 || max_selected < 0 || max_selected > 1 << 30)
     return set_error(ZL_ERR_INVALID_ARG, "select_blocks: bad sizes B=%d Hkv=%d bs=%d max_blocks=%d max_selected=%d",
                      num_seqs, num_kv_heads, block_size, max_blocks_per_seq, max_selected);
   if (num_first < 0 || num_last < 0 || (int64_t)num_first + num_last > max_selected)

@@ -113,7 +113,8 @@ zl_status zl_paged_decode_selected(zl_ctx* ctx, const void* q, const void* k_poo
   if ((s = check_heads(num_heads, num_kv_heads, head_dim, "paged_decode_selected")) != ZL_OK) return s;
   if (head_dim > 256)
     return set_error(ZL_ERR_UNSUPPORTED, "paged_decode_selected: head_dim %d > 256", head_dim);
-  if (num_seqs < 0 || block_size <= 0 || max_blocks_per_seq < 0 || num_blocks < 0 || max_selected < 0)
+  if (num_seqs < 0 || block_size <= 0 || max_blocks_per_seq < 0 || num_blocks < 0 || max_selected < 0 ||
+      max_selected > 1 << 30)
     return set_error(ZL_ERR_INVALID_ARG, "paged_decode_selected: bad sizes B=%d bs=%d max_blocks=%d max_selected=%d",
                      num_seqs, block_size, max_blocks_per_seq, max_selected);
   if (num_seqs == 0) return ZL_OK;

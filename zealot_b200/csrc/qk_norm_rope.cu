@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(256, kResident<T>) rope_tokens_kernel(RopeArgs
       a = load_run(slot, a);
       b = load_run(slot + 256 * E, b);
     }
-    finish_row(g, ln, r, c, a, b, cs + c * half, cache[c]);
+    finish_row(g, ln, r, c, a, b, cs + c * half, r.use ? cache[c] : -1);
     if (h < heads && (c += slices) >= tokens) {
       c = slice;
       h += hpb;
@@ -382,7 +382,7 @@ zl_status launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
     rope_token_kernel<T, LG, E><<<dim3((unsigned)g.tokens, blocks < 65535 ? blocks : 65535), 256, 0, st>>>(g);
     return ZL_OK;
   }
-  const int hpb = (heads + blocks - 1) / blocks, slices = NG / hpb;
+  const int hpb = (heads + blocks - 1) / blocks, slices = NG / hpb < per ? NG / hpb : (int)per;
   const size_t smem = (size_t)kAhead * 256 * 2 * E * sizeof(T) + per * (g.rot / 2) * sizeof(float2);
   const auto kernel = rope_tokens_kernel<T, LG, E>;
   ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));

@@ -250,8 +250,9 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
                      "step_tables: bad sizes n=%d rows=%d new=%lld T=%lld max_blocks=%d bs=%d blocks=%lld", num_seqs,
                      num_rows, (long long)num_new, (long long)num_tokens, max_blocks_per_seq, block_size,
                      (long long)num_blocks);
-  if (num_tokens > INT32_MAX || num_blocks > INT32_MAX || max_blocks_per_seq > 1 << 30)
-    return set_error(ZL_ERR_INVALID_ARG, "step_tables: more than 2^31-1 token rows or blocks, or 2^30 blocks to a row");
+  // (2^31 - 1 token rows is what a saturated sum reads as)
+  if (num_tokens >= INT32_MAX || num_blocks > INT32_MAX || max_blocks_per_seq > 1 << 30)
+    return set_error(ZL_ERR_INVALID_ARG, "step_tables: 2^31-1 token rows, more blocks, or more than 2^30 to a row");
   if (num_seqs > kMaxSeqs || (rows && num_rows > kMaxRows))
     return set_error(ZL_ERR_UNSUPPORTED, "step_tables: at most %d requests (have %d) and %d table rows (have %d)",
                      kMaxSeqs, num_seqs, kMaxRows, num_rows);
@@ -261,6 +262,10 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
       (num_seqs && max_blocks_per_seq && (!block_tables || (num_rows && !seq_blocks))) || (num_new && !new_blocks) ||
       (num_tokens && (!positions || !slot_mapping)))
     return set_error(ZL_ERR_INVALID_ARG, "step_tables: null pointer");
+  const size_t row_bytes = (size_t)max_blocks_per_seq * 4;
+  const auto lo = reinterpret_cast<uintptr_t>(seq_blocks), to = reinterpret_cast<uintptr_t>(block_tables);
+  if (row_bytes && num_seqs && num_rows && lo < to + num_seqs * row_bytes && to < lo + num_rows * row_bytes)
+    return set_error(ZL_ERR_INVALID_ARG, "step_tables: block_tables overlaps seq_blocks");
   DeviceScope dev(ctx);
   if (dev.status != ZL_OK) return dev.status;
   StepArgs g{seq_blocks, rows, context_lens, query_lens, new_blocks, block_tables, cu_seqlens, seq_lens, positions,

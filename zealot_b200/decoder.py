@@ -7,9 +7,10 @@
 `reshape_and_cache`, varlen causal prefill and paged decode for every layer,
 then the final RMSNorm and lm_head on the requested rows.
 
-`StepBatch.build` lays out one step the way the engine schedules it
+`StepBatch.build` lays out one step on the host the way the engine schedules it
 (src/scheduler.rs:88-113): prefill chunks first, packed back to back, then one
-row per decode sequence.
+row per decode sequence. `StepTables` keeps the sequences' block tables on the
+device and builds the same from the requests' lengths there.
 """
 from __future__ import annotations
 
@@ -142,6 +143,59 @@ class StepBatch:
             ptr(self.tokens), ptr(self.slot_mapping), ptr(self.cu_prefill), self.num_prefill,
             self.max_prefill_len, self.prefill_tokens, ptr(self.block_tables), ptr(self.seq_lens),
             self.num_decode, self.max_blocks_per_seq, ptr(self.last_rows), self.num_last)
+
+
+class StepTables:
+    """Block tables of up to num_rows sequences, kept on the device, and the metadata of one step
+    at a time built from them there (zl_step_tables). A step uploads three numbers a request and
+    the ids of the blocks that it opens, in place of the whole tables and a slot for every token."""
+
+    def __init__(self, ctx: GpuContext, num_rows: int, max_blocks_per_seq: int, max_seqs: int,
+                 max_tokens: int, block_size: int, num_blocks: int):
+        import torch
+        from .attention import CudaAttention
+        self.ctx, self.attn = ctx, CudaAttention(ctx)
+        self.block_size, self.num_blocks, self.max_blocks = block_size, num_blocks, max_blocks_per_seq
+
+        def new(*shape, dtype=torch.int32):
+            return torch.full(shape, -1, dtype=dtype, device=f"cuda:{ctx.device}")
+
+        self.seq_blocks = new(num_rows, max_blocks_per_seq)
+        self.block_tables = new(max_seqs, max_blocks_per_seq)
+        self.cu_seqlens, self.seq_lens, self.last_rows = new(max_seqs + 1), new(max_seqs), new(max_seqs)
+        self.positions, self.slot_mapping = new(max_tokens), new(max_tokens, dtype=torch.int64)
+
+    def blocks_needed(self, context_len: int, query_len: int) -> int:
+        """New blocks that a request opens, to be taken from the BlockManager."""
+        bs = self.block_size
+        return -(-(context_len + query_len) // bs) - -(-context_len // bs)
+
+    def build(self, tokens, rows, context_lens, query_lens, new_blocks, num_prefill: int, stream=None) -> StepBatch:
+        """The step of requests that add query_lens[i] tokens to the context_lens[i] cached ones of
+        table row rows[i]: first num_prefill prompt chunks, each a whole prompt (context 0), then one
+        token for each of the others. tokens: int64 device ids of all rows, in that order; new_blocks:
+        the ids that the requests open, in request order (blocks_needed of each). The batch holds views
+        of this object's buffers: the next build on it overwrites them."""
+        import torch
+        n, P = len(query_lens), int(sum(query_lens[:num_prefill]))
+        T = P + n - num_prefill
+        if len(rows) != n or len(context_lens) != n or any(c != 0 for c in context_lens[:num_prefill]):
+            raise InvalidArgument("a row and lengths for each request, prompt chunks from position 0")
+        if any(q != 1 for q in query_lens[num_prefill:]) or tokens.numel() != T:
+            raise InvalidArgument("one token for each decode row, and all tokens")
+        if n > self.seq_lens.numel() or T > self.positions.numel():
+            raise InvalidArgument(f"{n} requests of {T} tokens: more than this object was made for")
+        up = torch.tensor([*rows, *context_lens, *query_lens, *new_blocks], dtype=torch.int32).to(self.seq_blocks.device)
+        self.attn.step_tables(self.seq_blocks, up[:n], up[n:2 * n], up[2 * n:3 * n], up[3 * n:], self.block_tables[:n],
+                              self.cu_seqlens[:n + 1], self.seq_lens[:n], self.positions[:T], self.slot_mapping[:T],
+                              self.last_rows[:n], self.block_size, self.num_blocks, stream=stream)
+        if stream is not None:  # `up` stays until that stream has read it
+            up.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
+        return StepBatch(
+            tokens=tokens, slot_mapping=self.slot_mapping[:T], cu_prefill=self.cu_seqlens[:num_prefill + 1],
+            num_prefill=num_prefill, max_prefill_len=int(max(query_lens[:num_prefill], default=0)), prefill_tokens=P,
+            block_tables=self.block_tables[num_prefill:n], seq_lens=self.seq_lens[num_prefill:n],
+            num_decode=n - num_prefill, max_blocks_per_seq=self.max_blocks, last_rows=self.last_rows[:n])
 
 
 class Decoder:
