@@ -473,54 +473,23 @@ __device__ __forceinline__ bool select_ends(const SelectArgs& g, int64_t row, in
   return m == 0;
 }
 
-// The threshold among keys in registers, by counting: two bits a pass, the counts for
-// the three larger values of the next digit being summed over a warp as 10-bit fields of
-// one word (R <= 31). No atomics; for few keys a thread.
-template <int THREADS, int R>
-__device__ __forceinline__ uint32_t limit_by_counts(const uint32_t (&key)[R], int m) {
-  constexpr int W = THREADS / 32;
-  __shared__ __align__(16) int4 part[2][W];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t limit = 0;
-  for (int bit = 30, p = 0; bit >= 0; bit -= 2, p ^= 1) {
-    const uint32_t c1 = limit | 1u << bit, c2 = limit | 2u << bit, c3 = limit | 3u << bit;
-    uint32_t c = 0;
-#pragma unroll
-    for (int i = 0; i < R; i++) c += (key[i] >= c1) + ((key[i] >= c2) << 10) + ((key[i] >= c3) << 20);
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) part[p][warp] = make_int4(c & 1023, c >> 10 & 1023, c >> 20, 0);
-    __syncthreads();
-    int s1 = 0, s2 = 0, s3 = 0;
-#pragma unroll
-    for (int w = 0; w < W; w++) {
-      const int4 x = part[p][w];
-      s1 += x.x;
-      s2 += x.y;
-      s3 += x.z;
-    }
-    if (s3 >= m) limit = c3;
-    else if (s2 >= m) limit = c2;
-    else if (s1 >= m) limit = c1;
-  }
-  return limit;
-}
-
-// The same for many keys: three digits of 11, 11 and 10 bits, a histogram in shared
-// memory for each over the keys that share the digits before it.
-template <int THREADS, int R>
+// The threshold among keys in registers, BITS bits at a time (the last digit has what is
+// left): a histogram in shared memory for each digit over the keys that share the digits
+// before it.
+template <int THREADS, int R, int BITS>
 __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], int m) {
-  constexpr int BINS = 2048, PER = BINS / THREADS, W = THREADS / 32;
-  static_assert(PER * THREADS == BINS, "");
+  constexpr int BINS = 1 << BITS, PER = BINS > THREADS ? BINS / THREADS : 1, W = THREADS / 32;
   __shared__ int hist[BINS];
   __shared__ int sums[W];
   __shared__ int found[2];  // the digit, and how many keys of its bin are still to be chosen
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t limit = 0, mask = 0;
 #pragma unroll
-  for (int pass = 0; pass < 3; pass++) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
+  for (int left = 32; left > 0; left -= BITS) {
+    const int width = left < BITS ? left : BITS, shift = left - width;
 #pragma unroll
-    for (int k = 0; k < PER; k++) hist[k * THREADS + tid] = 0;
+    for (int k = 0; k < PER; k++)
+      if (k * THREADS + tid < BINS) hist[k * THREADS + tid] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < R; i++) {
@@ -529,11 +498,11 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
       if (in) atomicAdd(&hist[bin], 1);
     }
     __syncthreads();
-    // sums from the top bin down: this thread has bins [top - PER + 1, top]
+    // sums from the top bin down: this thread has bins [top - PER + 1, top], or none
     const int top = BINS - 1 - tid * PER;
     int own = 0;
 #pragma unroll
-    for (int k = 0; k < PER; k++) own += hist[top - k];
+    for (int k = 0; k < PER; k++) own += top >= 0 ? hist[top - k] : 0;
     int incl = own;
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, incl, o);
@@ -545,7 +514,7 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
     int above = incl - own + __reduce_add_sync(0xffffffffu, lane < warp ? s : 0);
 #pragma unroll
     for (int k = 0; k < PER; k++) {  // one bin holds the m-th key from the top
-      const int c = hist[top - k];
+      const int c = top >= 0 ? hist[top - k] : 0;
       if (above < m && m <= above + c) {
         found[0] = top - k;
         found[1] = m - above;
@@ -562,7 +531,7 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
 
 // Tables of up to THREADS R blocks: each thread keeps R keys, key i of thread t being
 // block i * THREADS + t.
-template <int THREADS, int R, bool DIGITS>
+template <int THREADS, int R, int BITS>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 4 : 1) select_reg_kernel(SelectArgs g) {
   constexpr int W = THREADS / 32;
   __shared__ uint32_t before[R * W];
@@ -584,9 +553,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 4 : 1) select_reg_ke
     const int j = i * THREADS + tid;
     key[i] = j >= lo && j < hi ? zl::score_key(key[i]) : 0;  // 0 is no score's key (-inf has 0x007fffff)
   }
-  uint32_t limit;
-  if constexpr (DIGITS) limit = limit_by_digits<THREADS, R>(key, m);
-  else limit = limit_by_counts<THREADS, R>(key, m);
+  const uint32_t limit = limit_by_digits<THREADS, R, BITS>(key, m);
   // counts of each warp's keys above (low half) and at the limit (high half), by index order
 #pragma unroll
   for (int i = 0; i < R; i++) {
@@ -838,12 +805,13 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
   const unsigned n = (unsigned)rows;
   const cudaStream_t st = S(stream);
   const bool many = rows > 2 * ctx->num_sms;  // more rows than CTAs of 1024 threads at once
-  if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4, false><<<n, 128, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 2048) select_reg_kernel<512, 4, true><<<n, 512, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 8192 && many) select_reg_kernel<512, 16, true><<<n, 512, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 8192) select_reg_kernel<1024, 8, true><<<n, 1024, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 16384) select_reg_kernel<1024, 16, true><<<n, 1024, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24, true><<<n, 1024, 0, st>>>(g);
+  if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4, 8><<<n, 128, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 1024) select_reg_kernel<256, 4, 8><<<n, 256, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 2048) select_reg_kernel<512, 4, 8><<<n, 512, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 8192 && many) select_reg_kernel<512, 16, 11><<<n, 512, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 8192) select_reg_kernel<1024, 8, 11><<<n, 1024, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 16384) select_reg_kernel<1024, 16, 11><<<n, 1024, 0, st>>>(g);
+  else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24, 11><<<n, 1024, 0, st>>>(g);
   else select_kernel<<<n, kSelThreads, 0, st>>>(g);
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
