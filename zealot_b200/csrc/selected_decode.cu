@@ -402,19 +402,17 @@ __global__ void __launch_bounds__(kThreads) selected_f32_kernel(SelArgs g, int c
     const int h = i / DT, e = i - h * DT;
     q_sh[i] = h < w.heads && e < g.d ? ((const float*)g.q)[((int64_t)w.b * g.H + w.head(g, h)) * g.d + e] * g.scale2 : 0.f;
   }
-  float4 o[HEADS][NV];
+  namespace px = zl::ptx;
+  uint64_t o[HEADS][NV][2];  // packed pairs: half the instructions of single ones
   float m[HEADS], l[HEADS];
 #pragma unroll
   for (int h = 0; h < HEADS; h++) {
     m[h] = -INFINITY;
     l[h] = 0.f;
 #pragma unroll
-    for (int v = 0; v < NV; v++) o[h][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int v = 0; v < NV; v++) o[h][v][0] = o[h][v][1] = 0;
   }
-  auto row4 = [](uint32_t a) {
-    const uint4 x = zl::ptx::lds16(a);
-    return make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
-  };
+  const uint32_t qs = px::smem_u32(q_sh) + li * 16;
   for (int e = w.e0; e < w.e1; e += kEntries) {
     if (e > w.e0) __syncthreads();
     const int toks = resolve(g, w, e, min(kEntries, w.e1 - e), entries, &list_end) * g.bs;
@@ -434,45 +432,47 @@ __global__ void __launch_bounds__(kThreads) selected_f32_kernel(SelArgs g, int c
         __syncwarp();
         // this lane's elements of rows tg and 4 + tg
         const uint32_t ks = mine + slot * 2 * TILE + tg * ROW + li * 16, vs = ks + TILE;
-        float s[HEADS][2];
+        uint64_t s2[HEADS][2];
 #pragma unroll
-        for (int h = 0; h < HEADS; h++) s[h][0] = s[h][1] = 0.f;
+        for (int h = 0; h < HEADS; h++) s2[h][0] = s2[h][1] = 0;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-          const float4 k0 = row4(ks + v * 128), k1 = row4(ks + 4 * ROW + v * 128);
+          const ulonglong2 k0 = px::lds_f2x2(ks + v * 128), k1 = px::lds_f2x2(ks + 4 * ROW + v * 128);
 #pragma unroll
           for (int h = 0; h < HEADS; h++) {
-            const float4 x = *reinterpret_cast<const float4*>(&q_sh[h * DT + v * 32 + li * 4]);
-            s[h][0] = fmaf(x.x, k0.x, fmaf(x.y, k0.y, fmaf(x.z, k0.z, fmaf(x.w, k0.w, s[h][0]))));
-            s[h][1] = fmaf(x.x, k1.x, fmaf(x.y, k1.y, fmaf(x.z, k1.z, fmaf(x.w, k1.w, s[h][1]))));
+            const ulonglong2 x = px::lds_f2x2(qs + (h * DT + v * 32) * 4);
+            s2[h][0] = px::f2_fma(x.x, k0.x, px::f2_fma(x.y, k0.y, s2[h][0]));
+            s2[h][1] = px::f2_fma(x.x, k1.x, px::f2_fma(x.y, k1.y, s2[h][1]));
           }
         }
-        float a[HEADS];
+        uint64_t a[HEADS], p[HEADS][2];
 #pragma unroll
         for (int h = 0; h < HEADS; h++) {
+          float s[2];
 #pragma unroll
           for (int u = 0; u < 2; u++) {
-            s[h][u] += __shfl_xor_sync(0xffffffffu, s[h][u], 1);
-            s[h][u] += __shfl_xor_sync(0xffffffffu, s[h][u], 2);
-            s[h][u] += __shfl_xor_sync(0xffffffffu, s[h][u], 4);
-            if (!(seen[slot] >> (4 * u + tg) & 1)) s[h][u] = -INFINITY;
+            const float2 both = px::f2_unpack(s2[h][u]);
+            s[u] = both.x + both.y;
+            s[u] += __shfl_xor_sync(0xffffffffu, s[u], 1);
+            s[u] += __shfl_xor_sync(0xffffffffu, s[u], 2);
+            s[u] += __shfl_xor_sync(0xffffffffu, s[u], 4);
+            if (!(seen[slot] >> (4 * u + tg) & 1)) s[u] = -INFINITY;
           }
-          const float to = fmaxf(m[h], fmaxf(s[h][0], s[h][1])), base = to == -INFINITY ? 0.f : to;
-          a[h] = m[h] == -INFINITY ? 0.f : exp2f(m[h] - base);
-          s[h][0] = exp2f(s[h][0] - base);
-          s[h][1] = exp2f(s[h][1] - base);
+          const float to = fmaxf(m[h], fmaxf(s[0], s[1])), base = to == -INFINITY ? 0.f : to;
+          const float f = m[h] == -INFINITY ? 0.f : px::ex2(m[h] - base), p0 = px::ex2(s[0] - base), p1 = px::ex2(s[1] - base);
           m[h] = to;
-          l[h] = fmaf(l[h], a[h], s[h][0] + s[h][1]);
+          l[h] = fmaf(l[h], f, p0 + p1);
+          a[h] = px::f2_pack(f, f);
+          p[h][0] = px::f2_pack(p0, p0);
+          p[h][1] = px::f2_pack(p1, p1);
         }
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-          const float4 v0 = row4(vs + v * 128), v1 = row4(vs + 4 * ROW + v * 128);
+          const ulonglong2 v0 = px::lds_f2x2(vs + v * 128), v1 = px::lds_f2x2(vs + 4 * ROW + v * 128);
 #pragma unroll
           for (int h = 0; h < HEADS; h++) {
-            o[h][v].x = fmaf(o[h][v].x, a[h], fmaf(s[h][0], v0.x, s[h][1] * v1.x));
-            o[h][v].y = fmaf(o[h][v].y, a[h], fmaf(s[h][0], v0.y, s[h][1] * v1.y));
-            o[h][v].z = fmaf(o[h][v].z, a[h], fmaf(s[h][0], v0.z, s[h][1] * v1.z));
-            o[h][v].w = fmaf(o[h][v].w, a[h], fmaf(s[h][0], v0.w, s[h][1] * v1.w));
+            o[h][v][0] = px::f2_fma(o[h][v][0], a[h], px::f2_fma(p[h][0], v0.x, px::f2_mul(p[h][1], v1.x)));
+            o[h][v][1] = px::f2_fma(o[h][v][1], a[h], px::f2_fma(p[h][0], v0.y, px::f2_mul(p[h][1], v1.y)));
           }
         }
         __syncwarp();  // the next fetch takes this slot
@@ -497,7 +497,8 @@ __global__ void __launch_bounds__(kThreads) selected_f32_kernel(SelArgs g, int c
     }
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      float x[4] = {o[h][v].x * a, o[h][v].y * a, o[h][v].z * a, o[h][v].w * a};
+      const float2 lo = px::f2_unpack(o[h][v][0]), hi = px::f2_unpack(o[h][v][1]);
+      float x[4] = {lo.x * a, lo.y * a, hi.x * a, hi.y * a};
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         x[i] += __shfl_xor_sync(0xffffffffu, x[i], 8);
