@@ -7,6 +7,7 @@ reference Rust interfaces it stands in for:
   GpuContext        src/gpu_context.rs:16-52
   CudaAttention     src/attention/cuda.rs:20-210 (paged_forward, forward_gpu)
                     + reshape_and_cache (src/kv_cache.rs:212-357)
+                    + step_tables, qk_norm_rope and decode over selected blocks
   BlockManager      src/block_manager.rs:41-165
   KVCache           src/kv_cache.rs:51-357
   CudaModelRunner   src/cuda_runner.rs / the ModelRunner trait (src/engine.rs:15-37)

@@ -1,7 +1,11 @@
 """CudaAttention: the attention operators of the hot path.
 
 Mirrors src/attention/cuda.rs:20-210 of the reference (paged_forward,
-forward_gpu) plus the KV scatter that replaced KVCache::store_kv's copies.
+forward_gpu) plus the KV scatter that replaced KVCache::store_kv's copies, and,
+without a counterpart there, a step's metadata from lengths (step_tables), the
+norm and rotation of queries and keys with the cache write (qk_norm_rope) and
+decode over selected blocks (block_bounds, block_scores, select_blocks,
+paged_forward_selected).
 Arguments keep the reference's names and meaning; tensors are torch device
 tensors, checked here and handed to the C ABI by address.
 """

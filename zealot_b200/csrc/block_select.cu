@@ -132,7 +132,10 @@ __device__ __forceinline__ void merge(uint4& lo, uint4& hi, const uint4& a, cons
 // Rows of 16-byte chunks, up to 32 CH of them: one warp per block and kv head, LPR lanes
 // to a row (a power of two), CH chunks to a lane, ROWS = 32 / LPR * DEPTH rows at a time,
 // all of whose loads are in flight at once. A warp keeps to one head; the warps of the
-// heads of one block, whose keys lie side by side, are neighbours.
+// heads of one block, whose keys lie side by side, are neighbours. HBM-bound: 16 prompts of
+// 256 to 8,192 tokens, 8 heads of 128 bf16, 27.9 us for 156 MB (5.6 TB/s); 64 of 2,048 to 4,096
+// 72 us (6.2 TB/s). The work per block had to shrink for that: with a division and a search for
+// each block 34 us, and 37 with copies ahead through shared memory on top.
 template <typename T, int LPR, int CH>
 __global__ void __launch_bounds__(256, 4)
 bounds_vec_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __restrict__ tok_begin,
@@ -252,6 +255,10 @@ scores_elem_kernel(PagedArgs g, const T* __restrict__ q, const T* __restrict__ b
 // Each warp keeps a ring of ST tiles (16 blocks' bounds) in shared memory, filled by
 // asynchronous copies, and the block ids of one tile more. Chunk ch of row r lies at
 // ch ^ swz(r), so that the two rows that a quarter warp reads do not meet in a bank.
+// HBM-bound: 8 sequences of 131,072 tokens, 64 query and 8 key heads, 44.2 us for 271 MB (6.1
+// TB/s). Loads straight into registers took 74 us, the ring 60, 32-bit row numbers and whole
+// rounds of CTAs 45. CTAs of one warp start and end on their own: 64 sequences of 2,048 to 4,096
+// tokens 11.6 us against 13.4 with four warps to a CTA.
 constexpr int kScoreWarps = 1, kScoreCtas = 12;
 template <int DT, int ST>
 __global__ void __launch_bounds__(kScoreWarps * 32)
@@ -364,7 +371,9 @@ scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
 
 // fp32 (and bf16 with more than 8 query heads to a kv head): eight lanes share a
 // block's rows, a warp scores four blocks at a time on the CUDA cores; q's two sides
-// are in shared memory, 8 heads at a time.
+// are in shared memory, 8 heads at a time. 8 sequences of 65,536 to 131,072 tokens, 32
+// fp32 query heads: 91 us for 402 MB (4.4 TB/s), bound by the latency of each tile's
+// loads and products; three CTAs of more registers to an SM took 115.
 template <typename T, int NV>
 __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts, const T* __restrict__ q,
                                                          const T* __restrict__ bounds, float scale,
@@ -436,13 +445,16 @@ __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts,
 
 // ---------------------------------------------------------------- selection
 
-// The `top` blocks of one (sequence, kv head), ascending: the first `nf`, the
-// last `nl` and the best of those between, equal scores by the lower index.
-// With m = top - (nf + nl) still to choose from the middle, the threshold is
-// the largest key that at least m middle keys reach; it is found from the top bit
-// down by counting, which needs no atomics and costs the same for every
-// distribution of the scores. A key's place in the output is the number of keys
-// above the threshold before it and of equal ones, of which the first few count.
+// The `top` blocks of one (sequence, kv head), ascending: the first `first`, the
+// last `last` and the best of those between, equal scores by the lower index.
+// With m = top - (first + last) still to choose from the middle, the threshold is
+// the largest key that at least m middle keys reach. A key's place in the output is
+// the number of keys above the threshold before it and of equal ones, of which the
+// first few count: no key's place depends on the order of the threads.
+//
+// Reads 4 bytes a block, so bound by its own steps: some 100 instructions a key and
+// warp, and the barriers between digits. 256 of up to 8,192 blocks in 512 rows 18-19
+// us (72 % of issue slots used), in 8 rows 7 us; 32 of some 100 in 32 rows 3.6 us.
 struct SelectArgs {
   const float* scores;
   const int32_t* seq_lens;
@@ -804,7 +816,11 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
                      num_first, num_last, ctx->d_status};
   const unsigned n = (unsigned)rows;
   const cudaStream_t st = S(stream);
-  const bool many = rows > 2 * ctx->num_sms;  // more rows than CTAs of 1024 threads at once
+  // Threads by the table's width, a few keys to each: with 256 threads and 32 keys instead of
+  // 1,024 and 8, 8 rows of 8,192 blocks take 15.4 us, not 7.0. Digits of 8 bits need 256 bins to
+  // clear and sum, of 11 bits one pass less: 1,600 rows of 650 blocks 10.4 and 21 us, 512 rows of
+  // 8,192 20.4 and 19.1. More rows than CTAs of 1,024 threads at once take half the threads (18.1).
+  const bool many = rows > 2 * ctx->num_sms;
   if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4, 8><<<n, 128, 0, st>>>(g);
   else if (max_blocks_per_seq <= 1024) select_reg_kernel<256, 4, 8><<<n, 256, 0, st>>>(g);
   else if (max_blocks_per_seq <= 2048) select_reg_kernel<512, 4, 8><<<n, 512, 0, st>>>(g);

@@ -14,6 +14,13 @@
 // the table entries and of the token rows. No CTA reads what another writes:
 // entries below `had` are only read, entries from `had` on are taken from the
 // list of new ids.
+//
+// Measured on one B200 (GPU time, replayed back to back): 64 decode rows with
+// tables of 257 blocks 3.7 us, bound by latency (two dependent reads, the sums,
+// one more read). 1,024 requests with tables of 8,192 blocks and 65,536 token
+// rows 17.6 us: 49.7 MB, 2.8 TB/s, of which some 6 us are every CTA's own sums.
+// On the way there: 4-byte entries 88 us, 16-byte ones 25, 32-bit divisions
+// 20, all of a stretch's loads before its first store and CTAs of 512 threads 17.
 #include "zl_internal.h"
 #include "zl_pages.h"
 
@@ -277,7 +284,8 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   if (smem > 32 * 1024)  // with the static part it may pass 48 KB
     ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   // Threads to a table row: one step of each while all rows then fit the GPU at once (the
-  // shortest way for a small step), kDepth steps otherwise.
+  // shortest way for a small step: 64 rows of 257 blocks 3.7 us, 4.0 with kDepth steps of a
+  // quarter of the threads), kDepth steps otherwise (1,024 rows of 8,192: 17.6 us, 20 with one).
   const int wide = vec ? 4 : 1;
   const int64_t most = 2 * ctx->num_sms;
   int log_lanes = 3;
