@@ -1,0 +1,70 @@
+"""The native call path of the serving-step operators (zealot_b200/calls.c) without a GPU: its tensor
+checks, and that every call passes its arguments to the C function in that function's order."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from test_serving_step_cpu import BOUNDS, ROPE, SCORES, SELECT, SELECTED, TABLES
+
+CALLS = {"step_tables": TABLES, "qk_norm_rope": ROPE, "block_bounds": BOUNDS, "block_scores": SCORES,
+         "select_blocks": SELECT, "paged_decode_selected": SELECTED}
+
+
+def test_addresses():
+    import torch
+    from zealot_b200 import calls
+    f, i = torch.zeros((3, 4)), torch.zeros(5, dtype=torch.int32)
+    got = calls.addresses(-1, f, torch.float32, 12, None, torch.float32, 7, i, torch.int32, 5)  # -1: the CPU
+    assert got == (f.data_ptr(), 0, i.data_ptr())
+    assert calls.addresses(-1) == ()
+    for bad in ((f, torch.float64, 12), (f, torch.float32, 11), (f.T, torch.float32, 12), (f[:, ::2], torch.float32, 6)):
+        assert calls.addresses(-1, i, torch.int32, 5, *bad) == 1
+    assert calls.addresses(0, f, torch.float32, 12) == 0  # another device
+    assert calls.addresses(-1, torch.zeros(0), torch.float32, 0) == (0,)
+    with pytest.raises(TypeError):
+        calls.addresses(-1, f, torch.float32)
+    with pytest.raises(TypeError):
+        calls.addresses()
+    with pytest.raises(AttributeError):
+        calls.addresses(-1, "no tensor", torch.float32, 1)
+    with pytest.raises(TypeError):
+        calls.addresses(-1, f, torch.float32, "12")
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_calls_pass_what_ctypes_passes(name):
+    """Each argument changed in turn to one that the C function refuses in words: the same status and words."""
+    from zealot_b200 import _capi, calls
+    lib = _capi.load()
+    base, typed, native = CALLS[name], getattr(lib, "zl_" + name), getattr(calls, name)
+    pointers = {k for k, t in zip(base, _capi.SIGNATURES["zl_" + name][1]) if t is ctypes.c_void_p}
+    for key in [None, *base]:
+        for value in ([None] if key in pointers else [-1, 0, 7, 300, 2**30 + 1] if key else [0]):
+            args = dict(base) if key is None else dict(base, **{key: value})
+            args = [float(v) if k in ("eps", "scale") else v for k, v in args.items()]
+            want = typed(*args), lib.zl_last_error()
+            assert (native(*args), lib.zl_last_error()) == want, (key, value)
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_calls_refuse_what_does_not_fit(name):
+    from zealot_b200 import calls
+    args = list(CALLS[name].values())
+    with pytest.raises(TypeError):
+        getattr(calls, name)(*args[:-1])
+    with pytest.raises(TypeError):
+        getattr(calls, name)(*args, 0)
+    key = "num_seqs" if "num_seqs" in CALLS[name] else "B" if "B" in CALLS[name] else "H"
+    for bad, error in (("x", TypeError), (2**31, OverflowError), (2**70, OverflowError), (np.zeros(2), TypeError)):
+        with pytest.raises(error):
+            getattr(calls, name)(*dict(CALLS[name], **{key: bad}).values())
+
+
+def test_c_floats_arrive():
+    """The two float arguments, in calls that end before a device is needed."""
+    from zealot_b200 import calls
+    with pytest.raises(TypeError):
+        calls.block_scores(*dict(SCORES, scale="x").values())
+    with pytest.raises(TypeError):
+        calls.qk_norm_rope(*dict(ROPE, eps=None).values())

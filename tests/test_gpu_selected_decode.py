@@ -231,3 +231,19 @@ def test_selected_is_paged_decode_when_all_blocks_are_listed(ctx):
     attn.paged_forward_selected(*args, empty, b)
     assert torch.all(b == 0)
     ctx.check_status()
+
+
+def test_closed_context_is_refused(ctx):
+    import torch
+    import zealot_b200 as zb
+    other = zb.GpuContext(0)
+    attn = zb.CudaAttention(other)
+    scores = torch.zeros((1, 1, 4), device="cuda")
+    lens = torch.zeros(1, dtype=torch.int32, device="cuda")
+    selected = torch.full((1, 1, 2), 5, dtype=torch.int32, device="cuda")
+    attn.select_blocks(scores, lens, selected, 16)
+    other.check_status()
+    assert selected.tolist() == [[[-1, -1]]]
+    other.close()
+    with pytest.raises(zb.InvalidArgument, match="null context"):
+        attn.select_blocks(scores, lens, selected, 16)

@@ -138,7 +138,7 @@ class _Context:
     """Stands in for a GpuContext: the Python checks come before any call on it."""
     device = 0
     lib = None
-    handle = None
+    address = 0
 
 
 @pytest.fixture()

@@ -11,6 +11,7 @@ tensors, checked here and handed to the C ABI by address.
 """
 from __future__ import annotations
 
+from . import calls  # native, built by build.py beside the library
 from .context import GpuContext, GQA_GROUPED, dtype_code, ptr
 from .errors import check, InvalidArgument
 
@@ -25,15 +26,16 @@ class CudaAttention:
         self.ctx = ctx
         self.lib = ctx.lib
 
-    def _check(self, *tensors) -> None:
-        """(tensor or None, dtype, elements) each: contiguous, on the context's device. These checks are
-        most of a small call's host time, so they are one pass with nothing built until one fails."""
-        device = self.ctx.device
-        for t, dtype, n in tensors:
-            if t is not None and (t.dtype is not dtype or t.numel() != n or t.get_device() != device
-                                  or not t.is_contiguous()):
-                raise InvalidArgument(f"need a contiguous {dtype} tensor of {n} elements on cuda:{device}, got "
-                                      f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}")
+    def _addresses(self, *triples):
+        """(tensor or None, dtype, elements), flat: the addresses of tensors that are contiguous, of that
+        dtype and size and on the context's device. Small calls are bound by such checks, so one native
+        pass does them (calls.c)."""
+        got = calls.addresses(self.ctx.device, *triples)
+        if type(got) is not tuple:
+            t, dtype, n = triples[3 * got:3 * got + 3]
+            raise InvalidArgument(f"need a contiguous {dtype} tensor of {n} elements on cuda:{self.ctx.device}, got "
+                                  f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}")
+        return got
 
     # ----------------------------------------------------------- step tables
     def step_tables(self, seq_blocks, rows, context_lens, query_lens, new_blocks, block_tables, cu_seqlens,
@@ -45,18 +47,15 @@ class CudaAttention:
         Writes block_tables [n][max_blocks], cu_seqlens [n+1], seq_lens [n], last_rows [n], and for each
         token row positions [T] and slot_mapping [T] (int64; all others int32)."""
         import torch
-        i32, n, T, num_new = torch.int32, query_lens.numel(), slot_mapping.numel(), new_blocks.numel()
+        i32, n, T, new = torch.int32, query_lens.numel(), slot_mapping.numel(), new_blocks.numel()
         _need(seq_blocks.dim() == 2, "seq_blocks is [num_rows][max_blocks]")
-        num_rows, max_blocks = seq_blocks.shape
-        self._check((seq_blocks, i32, num_rows * max_blocks), (rows, i32, n), (context_lens, i32, n),
-                    (query_lens, i32, n), (new_blocks, i32, num_new), (block_tables, i32, n * max_blocks),
-                    (cu_seqlens, i32, n + 1), (seq_lens, i32, n), (positions, i32, T),
-                    (slot_mapping, torch.int64, T), (last_rows, i32, n))
-        check(self.lib.zl_step_tables(
-            self.ctx.handle, seq_blocks.data_ptr(), num_rows, ptr(rows), context_lens.data_ptr(),
-            query_lens.data_ptr(), new_blocks.data_ptr(), num_new, block_tables.data_ptr(),
-            cu_seqlens.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(),
-            last_rows.data_ptr(), n, T, max_blocks, block_size, num_blocks, self.ctx.stream(stream)))
+        num_rows, width = seq_blocks.shape
+        old, row, c, q, fresh, tables, cu, lens, pos, slots, last = self._addresses(
+            seq_blocks, i32, num_rows * width, rows, i32, n, context_lens, i32, n, query_lens, i32, n, new_blocks, i32, new,
+            block_tables, i32, n * width, cu_seqlens, i32, n + 1, seq_lens, i32, n, positions, i32, T,
+            slot_mapping, torch.int64, T, last_rows, i32, n)
+        check(calls.step_tables(self.ctx.address, old, num_rows, row, c, q, fresh, new, tables, cu, lens, pos,
+                                slots, last, n, T, width, block_size, num_blocks, self.ctx.stream(stream)))
 
     # ------------------------------------- query / key norm, rotation, scatter
     def qk_norm_rope(self, q, k, v, positions, inv_freq, q_out=None, k_out=None, v_out=None, q_weight=None,
@@ -78,11 +77,10 @@ class CudaAttention:
             if (element != 1 and d != 1) or (head != d and n != 1):
                 raise InvalidArgument("the heads of a token are packed")
             strides.append(token)
-        rot = bs = num_blocks = 0
+        rot = bs = num_blocks = pool = 0
         if inv_freq is not None:
             _need(positions is not None, "inv_freq needs positions")
             rot = 2 * inv_freq.numel()
-        pool = 0
         if k_pool is not None or v_pool is not None:
             _need(k_pool is not None and v_pool is not None and slot_mapping is not None,
                   "both pools and a slot_mapping, or none")
@@ -90,14 +88,13 @@ class CudaAttention:
             _need(pool_heads == Hkv and pool_d == d, "pools are [num_blocks][Hkv][bs][d]")
             pool = num_blocks * Hkv * bs * d
         nk = T * Hkv * d
-        self._check((q_out, dtype, T * H * d), (k_out, dtype, nk), (v_out, dtype, nk), (q_weight, dtype, d),
-                    (k_weight, dtype, d), (positions, torch.int32, T), (inv_freq, torch.float64, rot // 2),
-                    (k_pool, dtype, pool), (v_pool, dtype, pool), (slot_mapping, torch.int64, T))
-        check(self.lib.zl_qk_norm_rope(
-            self.ctx.handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides,
-            ptr(q_weight), ptr(k_weight), eps, ptr(positions), ptr(inv_freq), rot, int(interleaved), ptr(q_out),
-            ptr(k_out), ptr(v_out), ptr(k_pool), ptr(v_pool), ptr(slot_mapping), bs, num_blocks, T, H, Hkv, d,
-            dtype_code(dtype), self.ctx.stream(stream)))
+        qo, ko, vo, qw, kw, pos, freq, kp, vp, slots = self._addresses(
+            q_out, dtype, T * H * d, k_out, dtype, nk, v_out, dtype, nk, q_weight, dtype, d, k_weight, dtype, d,
+            positions, torch.int32, T, inv_freq, torch.float64, rot // 2, k_pool, dtype, pool, v_pool, dtype, pool,
+            slot_mapping, torch.int64, T)
+        check(calls.qk_norm_rope(self.ctx.address, q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, qw, kw,
+                                 eps, pos, freq, rot, int(interleaved), qo, ko, vo, kp, vp, slots, bs, num_blocks, T,
+                                 H, Hkv, d, dtype_code(dtype), self.ctx.stream(stream)))
 
     # ------------------------------------------------------------ KV scatter
     def reshape_and_cache(self, k, v, k_pool, v_pool, slot_mapping, num_kv_heads: int,
@@ -170,13 +167,12 @@ class CudaAttention:
         import torch
         _need(k_pool.dim() == 4 and block_tables.dim() == 2, "k_pool [num_blocks][Hkv][bs][d], block_tables [B][max]")
         num_blocks, Hkv, bs, d = k_pool.shape
-        B, max_blocks = block_tables.shape
+        B, width = block_tables.shape
         i32, dtype, row = torch.int32, k_pool.dtype, num_blocks * Hkv * d
-        self._check((k_pool, dtype, row * bs), (bounds, dtype, row * 2), (block_tables, i32, B * max_blocks),
-                    (seq_lens, i32, B), (tok_begin, i32, B))
-        check(self.lib.zl_block_bounds(
-            self.ctx.handle, k_pool.data_ptr(), block_tables.data_ptr(), ptr(tok_begin), seq_lens.data_ptr(),
-            bounds.data_ptr(), B, Hkv, d, bs, max_blocks, num_blocks, dtype_code(dtype), self.ctx.stream(stream)))
+        k, table, begin, lens, out = self._addresses(
+            k_pool, dtype, row * bs, block_tables, i32, B * width, tok_begin, i32, B, seq_lens, i32, B, bounds, dtype, row * 2)
+        check(calls.block_bounds(self.ctx.address, k, table, begin, lens, out, B, Hkv, d, bs, width, num_blocks,
+                                 dtype_code(dtype), self.ctx.stream(stream)))
 
     def block_scores(self, q, bounds, block_tables, seq_lens, scores, block_size: int, scale: float = 0.0,
                      gqa_map: int = GQA_GROUPED, stream=None) -> None:
@@ -186,15 +182,14 @@ class CudaAttention:
         _need(q.dim() == 3 and bounds.dim() == 4 and block_tables.dim() == 2,
               "q [B][H][d], bounds [num_blocks][Hkv][2][d], block_tables [B][max]")
         num_blocks, Hkv, two, d = bounds.shape
-        B, max_blocks = block_tables.shape
+        B, width = block_tables.shape
         H, i32, dtype = q.shape[1], torch.int32, q.dtype
         _need(two == 2, "bounds is [num_blocks][Hkv][2][d]")
-        self._check((q, dtype, B * H * d), (bounds, dtype, num_blocks * Hkv * 2 * d),
-                    (block_tables, i32, B * max_blocks), (seq_lens, i32, B), (scores, torch.float32, B * Hkv * max_blocks))
-        check(self.lib.zl_block_scores(
-            self.ctx.handle, q.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
-            scores.data_ptr(), B, H, Hkv, d, block_size, max_blocks, num_blocks, scale, gqa_map,
-            dtype_code(dtype), self.ctx.stream(stream)))
+        x, ends, table, lens, out = self._addresses(
+            q, dtype, B * H * d, bounds, dtype, num_blocks * Hkv * 2 * d, block_tables, i32, B * width, seq_lens, i32, B,
+            scores, torch.float32, B * Hkv * width)
+        check(calls.block_scores(self.ctx.address, x, ends, table, lens, out, B, H, Hkv, d, block_size, width,
+                                 num_blocks, scale, gqa_map, dtype_code(dtype), self.ctx.stream(stream)))
 
     def select_blocks(self, scores, seq_lens, selected, block_size: int, num_first: int = 1, num_last: int = 1,
                       stream=None) -> None:
@@ -202,13 +197,12 @@ class CudaAttention:
         scores [B][Hkv][max_blocks]: selected [B][Hkv][max_selected] int32, ascending, -1 after the last."""
         import torch
         _need(scores.dim() == 3 and selected.dim() == 3, "scores [B][Hkv][max_blocks], selected [B][Hkv][max_selected]")
-        B, Hkv, max_blocks = scores.shape
+        B, Hkv, width = scores.shape
         top = selected.shape[2]
-        self._check((scores, torch.float32, B * Hkv * max_blocks), (seq_lens, torch.int32, B),
-                    (selected, torch.int32, B * Hkv * top))
-        check(self.lib.zl_select_blocks(
-            self.ctx.handle, scores.data_ptr(), seq_lens.data_ptr(), selected.data_ptr(), B, Hkv, block_size,
-            max_blocks, top, num_first, num_last, self.ctx.stream(stream)))
+        sc, lens, out = self._addresses(scores, torch.float32, B * Hkv * width, seq_lens, torch.int32, B,
+                                        selected, torch.int32, B * Hkv * top)
+        check(calls.select_blocks(self.ctx.address, sc, lens, out, B, Hkv, block_size, width, top, num_first,
+                                  num_last, self.ctx.stream(stream)))
 
     def paged_forward_selected(self, q, k_pool, v_pool, block_tables, seq_lens, selected, o, scale: float = 0.0,
                                gqa_map: int = GQA_GROUPED, stream=None) -> None:
@@ -218,15 +212,15 @@ class CudaAttention:
         _need(q.dim() == 3 and k_pool.dim() == 4 and block_tables.dim() == 2 and selected.dim() == 3,
               "q [B][H][d], pools [num_blocks][Hkv][bs][d], block_tables [B][max], selected [B][Hkv][max_selected]")
         num_blocks, Hkv, bs, d = k_pool.shape
-        B, max_blocks = block_tables.shape
+        B, width = block_tables.shape
         H, top, i32, dtype = q.shape[1], selected.shape[2], torch.int32, q.dtype
         pool = num_blocks * Hkv * bs * d
-        self._check((q, dtype, B * H * d), (o, dtype, B * H * d), (k_pool, dtype, pool), (v_pool, dtype, pool),
-                    (block_tables, i32, B * max_blocks), (seq_lens, i32, B), (selected, i32, B * Hkv * top))
-        check(self.lib.zl_paged_decode_selected(
-            self.ctx.handle, q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
-            seq_lens.data_ptr(), selected.data_ptr(), o.data_ptr(), B, H, Hkv, d, bs, max_blocks, num_blocks, top,
-            scale, gqa_map, dtype_code(dtype), self.ctx.stream(stream)))
+        x, k, v, table, lens, picked, out = self._addresses(
+            q, dtype, B * H * d, k_pool, dtype, pool, v_pool, dtype, pool, block_tables, i32, B * width, seq_lens, i32, B,
+            selected, i32, B * Hkv * top, o, dtype, B * H * d)
+        check(calls.paged_decode_selected(self.ctx.address, x, k, v, table, lens, picked, out, B, H, Hkv, d, bs,
+                                          width, num_blocks, top, scale, gqa_map, dtype_code(dtype),
+                                          self.ctx.stream(stream)))
 
     # ---------------------------------------------------------------- prefill
     def forward_gpu(self, q, k, v, cu_seqlens, o, num_heads: int, num_kv_heads: int,

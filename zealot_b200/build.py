@@ -10,7 +10,8 @@ Every .cu / .cc file under zealot_b200/csrc is compiled with
 -gencode arch=compute_100a,code=sm_100a and linked into
 zealot_b200/libzealot_attn.so (static CUDA runtime, no libcuda link: the
 driver entry points are resolved at run time, so the library also loads on a
-machine without a GPU driver).
+machine without a GPU driver). zealot_b200/calls.c, the Python call path of the
+small operators, becomes zealot_b200/calls.so beside it.
 """
 from __future__ import annotations
 
@@ -19,11 +20,13 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libzealot_attn.so")
+CALLS = os.path.join(HERE, "calls.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -72,7 +75,20 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _build_calls(force)
     return LIB
+
+
+def _build_calls(force: bool) -> None:
+    src = os.path.join(HERE, "calls.c")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "zealot_attn.h")))
+    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest:
+        return
+    cmd = ["gcc", "-O2", "-Wall", "-shared", "-fPIC", f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", src,
+           "-o", CALLS, f"-L{HERE}", "-l:libzealot_attn.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"gcc failed for {src}:\n{r.stdout}\n{r.stderr}")
 
 
 if __name__ == "__main__":

@@ -69,6 +69,7 @@ class GpuContext:
         h = ctypes.c_void_p()
         check(self.lib.zl_ctx_create(ctypes.byref(cfg), ctypes.byref(h)))
         self.handle = h
+        self.address = h.value  # the same for the native calls; 0 once closed
 
     def stream(self, stream=None) -> int:
         if stream is None:
@@ -93,6 +94,7 @@ class GpuContext:
         if getattr(self, "handle", None):
             self.lib.zl_ctx_destroy(self.handle)
             self.handle = None
+            self.address = 0
 
     def __del__(self):
         try:
