@@ -73,6 +73,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 bounds_elem_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __restrict__ tok_begin,
                    T* __restrict__ bounds) {
+  zl::ptx::griddep_enter();
   const int lane = threadIdx.x & 31;
   for (int64_t u = blockIdx.y; u < (int64_t)g.B * g.Hkv; u += gridDim.y) {
     const int b = (int)(u / g.Hkv), h = (int)(u - (int64_t)b * g.Hkv);
@@ -140,6 +141,7 @@ template <typename T, int LPR, int CH>
 __global__ void __launch_bounds__(256, 4)
 bounds_vec_kernel(PagedArgs g, const T* __restrict__ k_pool, const int32_t* __restrict__ tok_begin,
                   T* __restrict__ bounds) {
+  zl::ptx::griddep_enter();
   constexpr int RPL = 32 / LPR, DEPTH = CH == 1 ? 8 : 4, ROWS = RPL * DEPTH, VEC = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, sub = lane / LPR, ch = lane % LPR;
   const int chunks = g.d / VEC, warps = gridDim.x * 8, step = warps / g.Hkv;  // blocks at a time
@@ -219,6 +221,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 scores_elem_kernel(PagedArgs g, const T* __restrict__ q, const T* __restrict__ bounds, float scale,
                    float* __restrict__ scores) {
+  zl::ptx::griddep_enter();
   const int lane = threadIdx.x & 31;
   const int group = g.H / g.Hkv;
   for (int64_t u = blockIdx.y; u < (int64_t)g.B * g.Hkv; u += gridDim.y) {
@@ -264,6 +267,7 @@ template <int DT, int ST>
 __global__ void __launch_bounds__(kScoreWarps * 32)
 scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
                   const __nv_bfloat16* __restrict__ bounds, float scale, float* __restrict__ scores) {
+  zl::ptx::griddep_enter();
   constexpr int KC = DT / 32, ROW = DT * 4;  // a row: lo and hi side by side, DT elements each
   constexpr int CPR = DT / 4;                // its 16-byte chunks
   extern __shared__ __align__(128) uint8_t ring[];
@@ -378,6 +382,7 @@ template <typename T, int NV>
 __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts, const T* __restrict__ q,
                                                          const T* __restrict__ bounds, float scale,
                                                          float* __restrict__ scores) {
+  zl::ptx::griddep_enter();
   constexpr int VEC = 16 / sizeof(T), DT = NV * 8 * VEC;
   __shared__ __align__(16) float sides[2][8][DT];
   const int lane = threadIdx.x & 31, tg = lane >> 3, li = lane & 7;
@@ -545,6 +550,7 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
 // block i * THREADS + t.
 template <int THREADS, int R, int BITS>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 4 : 1) select_reg_kernel(SelectArgs g) {
+  zl::ptx::griddep_enter();
   constexpr int W = THREADS / 32;
   __shared__ uint32_t before[R * W];
   __shared__ int total_above;
@@ -619,6 +625,7 @@ __device__ __forceinline__ int block_count(int c, int* red) {  // sum over the C
 }
 
 __global__ void __launch_bounds__(kSelThreads) select_kernel(SelectArgs g) {
+  zl::ptx::griddep_enter();
   __shared__ int red[kSelThreads / 32];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -688,10 +695,10 @@ void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* to
   const dim3 grid((unsigned)x, (unsigned)(g.B < 65535 ? g.B : 65535));
   const T* k = (const T*)k_pool;
   T* o = (T*)bounds;
-  if (chunks <= 8) bounds_vec_kernel<T, 8, 1><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
-  else if (chunks <= 16) bounds_vec_kernel<T, 16, 1><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
-  else if (chunks <= 32) bounds_vec_kernel<T, 32, 1><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
-  else bounds_vec_kernel<T, 32, 2><<<grid, 256, 0, st>>>(g, k, tok_begin, o);
+  if (chunks <= 8) zl::launch_ahead(bounds_vec_kernel<T, 8, 1>, grid, 256, 0, st, g, k, tok_begin, o);
+  else if (chunks <= 16) zl::launch_ahead(bounds_vec_kernel<T, 16, 1>, grid, 256, 0, st, g, k, tok_begin, o);
+  else if (chunks <= 32) zl::launch_ahead(bounds_vec_kernel<T, 32, 1>, grid, 256, 0, st, g, k, tok_begin, o);
+  else zl::launch_ahead(bounds_vec_kernel<T, 32, 2>, grid, 256, 0, st, g, k, tok_begin, o);
 }
 
 // CTAs for each of `rows` rows of `tiles` tiles, `warps` tiles at a time: not more than
@@ -709,7 +716,7 @@ zl_status launch_scores_mma(const PagedArgs& g, int parts, unsigned grid, const 
   using namespace zl;
   constexpr int smem = kScoreWarps * ST * 16 * DT * 4;
   ZL_CUDA_TRY(cudaFuncSetAttribute(scores_mma_kernel<DT, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  scores_mma_kernel<DT, ST><<<grid, kScoreWarps * 32, smem, st>>>(g, parts, q, bounds, scale, scores);
+  zl::launch_ahead(scores_mma_kernel<DT, ST>, grid, kScoreWarps * 32, smem, st, g, parts, q, bounds, scale, scores);
   return ZL_OK;
 }
 
@@ -740,9 +747,9 @@ zl_status zl_block_bounds(zl_ctx* ctx, const void* k_pool, const int32_t* block_
   } else {
     const dim3 grid = grid_of((int64_t)num_seqs * num_kv_heads, max_blocks_per_seq);
     if (dtype == ZL_F32)
-      bounds_elem_kernel<float><<<grid, 256, 0, st>>>(g, (const float*)k_pool, tok_begin, (float*)bounds);
+      zl::launch_ahead(bounds_elem_kernel<float>, grid, 256, 0, st, g, (const float*)k_pool, tok_begin, (float*)bounds);
     else
-      bounds_elem_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(g, (const __nv_bfloat16*)k_pool, tok_begin,
+      zl::launch_ahead(bounds_elem_kernel<__nv_bfloat16>, grid, 256, 0, st, g, (const __nv_bfloat16*)k_pool, tok_begin,
                                                               (__nv_bfloat16*)bounds);
   }
   ZL_LAUNCH_CHECK(ctx);
@@ -780,16 +787,16 @@ zl_status zl_block_scores(zl_ctx* ctx, const void* q, const void* bounds, const 
                           : launch_scores_mma<256, 2>(g, p16, n16, qb, bb, sc, scores, st);
     if (s != ZL_OK) return s;
   } else if (vec && dtype == ZL_BF16) {
-    if (head_dim <= 128) scores_vec_kernel<__nv_bfloat16, 2><<<n4, 256, 0, st>>>(g, p4, qb, bb, sc, scores);
-    else scores_vec_kernel<__nv_bfloat16, 4><<<n4, 256, 0, st>>>(g, p4, qb, bb, sc, scores);
+    if (head_dim <= 128) zl::launch_ahead(scores_vec_kernel<__nv_bfloat16, 2>, n4, 256, 0, st, g, p4, qb, bb, sc, scores);
+    else zl::launch_ahead(scores_vec_kernel<__nv_bfloat16, 4>, n4, 256, 0, st, g, p4, qb, bb, sc, scores);
   } else if (vec) {
-    if (head_dim <= 64) scores_vec_kernel<float, 2><<<n4, 256, 0, st>>>(g, p4, qf, bf, sc, scores);
-    else if (head_dim <= 128) scores_vec_kernel<float, 4><<<n4, 256, 0, st>>>(g, p4, qf, bf, sc, scores);
-    else scores_vec_kernel<float, 8><<<n4, 256, 0, st>>>(g, p4, qf, bf, sc, scores);
+    if (head_dim <= 64) zl::launch_ahead(scores_vec_kernel<float, 2>, n4, 256, 0, st, g, p4, qf, bf, sc, scores);
+    else if (head_dim <= 128) zl::launch_ahead(scores_vec_kernel<float, 4>, n4, 256, 0, st, g, p4, qf, bf, sc, scores);
+    else zl::launch_ahead(scores_vec_kernel<float, 8>, n4, 256, 0, st, g, p4, qf, bf, sc, scores);
   } else {
     const dim3 grid = grid_of(rows, max_blocks_per_seq);
-    if (dtype == ZL_F32) scores_elem_kernel<float><<<grid, 256, 0, st>>>(g, qf, bf, sc, scores);
-    else scores_elem_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(g, qb, bb, sc, scores);
+    if (dtype == ZL_F32) zl::launch_ahead(scores_elem_kernel<float>, grid, 256, 0, st, g, qf, bf, sc, scores);
+    else zl::launch_ahead(scores_elem_kernel<__nv_bfloat16>, grid, 256, 0, st, g, qb, bb, sc, scores);
   }
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
@@ -821,14 +828,14 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
   // clear and sum, of 11 bits one pass less: 1,600 rows of 650 blocks 10.4 and 21 us, 512 rows of
   // 8,192 20.4 and 19.1. More rows than CTAs of 1,024 threads at once take half the threads (18.1).
   const bool many = rows > 2 * ctx->num_sms;
-  if (max_blocks_per_seq <= 512) select_reg_kernel<128, 4, 8><<<n, 128, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 1024) select_reg_kernel<256, 4, 8><<<n, 256, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 2048) select_reg_kernel<512, 4, 8><<<n, 512, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 8192 && many) select_reg_kernel<512, 16, 11><<<n, 512, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 8192) select_reg_kernel<1024, 8, 11><<<n, 1024, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 16384) select_reg_kernel<1024, 16, 11><<<n, 1024, 0, st>>>(g);
-  else if (max_blocks_per_seq <= 24576) select_reg_kernel<1024, 24, 11><<<n, 1024, 0, st>>>(g);
-  else select_kernel<<<n, kSelThreads, 0, st>>>(g);
+  if (max_blocks_per_seq <= 512) zl::launch_ahead(select_reg_kernel<128, 4, 8>, n, 128, 0, st, g);
+  else if (max_blocks_per_seq <= 1024) zl::launch_ahead(select_reg_kernel<256, 4, 8>, n, 256, 0, st, g);
+  else if (max_blocks_per_seq <= 2048) zl::launch_ahead(select_reg_kernel<512, 4, 8>, n, 512, 0, st, g);
+  else if (max_blocks_per_seq <= 8192 && many) zl::launch_ahead(select_reg_kernel<512, 16, 11>, n, 512, 0, st, g);
+  else if (max_blocks_per_seq <= 8192) zl::launch_ahead(select_reg_kernel<1024, 8, 11>, n, 1024, 0, st, g);
+  else if (max_blocks_per_seq <= 16384) zl::launch_ahead(select_reg_kernel<1024, 16, 11>, n, 1024, 0, st, g);
+  else if (max_blocks_per_seq <= 24576) zl::launch_ahead(select_reg_kernel<1024, 24, 11>, n, 1024, 0, st, g);
+  else zl::launch_ahead(select_kernel, n, kSelThreads, 0, st, g);
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }

@@ -75,6 +75,7 @@ __device__ __forceinline__ int64_t cache_row(const RopeArgs& g, int64_t t, int h
 // the warp's shared memory so that a pair's elements meet.
 template <typename T>
 __global__ void __launch_bounds__(256) rope_elem_kernel(RopeArgs g) {
+  zl::ptx::griddep_enter();
   __shared__ float rows[8][kMaxDim];
   const int lane = threadIdx.x & 31;
   float* x = rows[threadIdx.x >> 5];
@@ -289,6 +290,7 @@ __device__ __forceinline__ void token_tables(const RopeArgs& g, int64_t t0, int 
 // Few tokens: one to a CTA, and its heads over gridDim.y of them.
 template <typename T, int LG, int E>
 __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
+  zl::ptx::griddep_enter();
   __shared__ __align__(16) float2 cs[kMaxDim / 2];
   __shared__ int64_t cache[1];
   const Lane<LG, E> ln(g);
@@ -324,6 +326,7 @@ constexpr int kTokens = 16, kAhead = 4, kFew = 2;
 template <typename T> constexpr int kResident = sizeof(T) == 2 ? 3 : 4;
 template <typename T, int LG, int E>
 __global__ void __launch_bounds__(256, kResident<T>) rope_tokens_kernel(RopeArgs g, int per, int hpb, int slices) {
+  zl::ptx::griddep_enter();
   constexpr int RUN = E * sizeof(T);
   extern __shared__ __align__(16) uint8_t dyn[];  // [kAhead][2][256] runs, then the angles
   __shared__ int64_t cache[kTokens];
@@ -389,14 +392,14 @@ zl_status launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
   const int64_t room = kResident<T> * (int64_t)num_sms, rounds = (g.tokens + room * kTokens - 1) / (room * kTokens);
   const int64_t per = (g.tokens + room * rounds - 1) / (room * rounds);
   if (per < kFew) {  // one token to a CTA: 1,024 tokens 13.2 us this way, 10.9 two to a CTA; 64 tokens 3.1
-    rope_token_kernel<T, LG, E><<<dim3((unsigned)g.tokens, blocks < 65535 ? blocks : 65535), 256, 0, st>>>(g);
+    launch_ahead(rope_token_kernel<T, LG, E>, dim3((unsigned)g.tokens, blocks < 65535 ? blocks : 65535), 256, 0, st, g);
     return ZL_OK;
   }
   const int hpb = (heads + blocks - 1) / blocks, slices = NG / hpb < per ? NG / hpb : (int)per;
   const size_t smem = (size_t)kAhead * 256 * 2 * E * sizeof(T) + per * (g.rot / 2) * sizeof(float2);
   const auto kernel = rope_tokens_kernel<T, LG, E>;
   ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<(unsigned)((g.tokens + per - 1) / per), 256, smem, st>>>(g, (int)per, hpb, slices);
+  launch_ahead(kernel, (unsigned)((g.tokens + per - 1) / per), 256, smem, st, g, (int)per, hpb, slices);
   return ZL_OK;
 }
 
@@ -464,8 +467,8 @@ extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, 
     const int64_t units = num_tokens * (num_heads + 2 * (int64_t)num_kv_heads);
     int64_t blocks = (units + 7) / 8;
     if (blocks > (int64_t)ctx->num_sms * 32) blocks = (int64_t)ctx->num_sms * 32;
-    if (dtype == ZL_F32) rope_elem_kernel<float><<<(unsigned)blocks, 256, 0, st>>>(g);
-    else rope_elem_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, st>>>(g);
+    if (dtype == ZL_F32) launch_ahead(rope_elem_kernel<float>, (unsigned)blocks, 256, 0, st, g);
+    else launch_ahead(rope_elem_kernel<__nv_bfloat16>, (unsigned)blocks, 256, 0, st, g);
   }
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;

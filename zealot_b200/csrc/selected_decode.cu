@@ -242,6 +242,7 @@ constexpr size_t ring_bytes(int rowb, int tok, int st) { return (size_t)kWarps *
 // and 2, and neither has a bank conflict.
 template <int DT, int ST>
 __global__ void __launch_bounds__(kThreads) selected_mma_kernel(SelArgs g, int cluster) {
+  zl::ptx::griddep_enter();
   constexpr int KC = DT / 32, VH = DT / 64, ROW = DT * 2;
   constexpr uint32_t TILE = 16 * ROW;
   extern __shared__ __align__(128) uint8_t ring[];
@@ -393,6 +394,7 @@ __global__ void __launch_bounds__(kThreads) selected_mma_kernel(SelArgs g, int c
 // fp32, head_dim up to 32 NV, a multiple of 4; HEADS query heads at a time.
 template <int NV, int HEADS, int ST>
 __global__ void __launch_bounds__(kThreads) selected_f32_kernel(SelArgs g, int cluster) {
+  zl::ptx::griddep_enter();
   constexpr int DT = NV * 32, ROW = DT * 4;
   constexpr uint32_t TILE = 8 * ROW;
   extern __shared__ __align__(128) uint8_t ring[];
@@ -527,12 +529,14 @@ zl_status launch(zl_ctx* ctx, void (*kernel)(SelArgs, int), size_t smem, const S
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch_ahead
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   ZL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, g, cluster));
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;

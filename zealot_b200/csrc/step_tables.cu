@@ -23,6 +23,7 @@
 // 20, all of a stretch's loads before its first store and CTAs of 512 threads 17.
 #include "zl_internal.h"
 #include "zl_pages.h"
+#include "zl_ptx.cuh"
 
 namespace {
 
@@ -139,6 +140,7 @@ __device__ __forceinline__ bool table_columns(const StepArgs& g, int i, int c, i
 constexpr int kDepth = 4;
 template <int N>
 __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g, int log_lanes) {
+  zl::ptx::griddep_enter();
   extern __shared__ int32_t sh[];
   const int n = g.num_seqs;
   int32_t* cu = sh;                                             // [n + 1] first token row
@@ -297,7 +299,7 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   const int64_t pieces = num_seqs * ((max_blocks_per_seq + width - 1) / width);
   int64_t blocks = (pieces * lanes + kThreads - 1) / kThreads + (num_tokens + kThreads - 1) / kThreads;
   blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
-  kernel<<<(unsigned)blocks, kThreads, smem, S(stream)>>>(g, log_lanes);
+  launch_ahead(kernel, (unsigned)blocks, kThreads, smem, S(stream), g, log_lanes);
   ZL_LAUNCH_CHECK(ctx);
   return ZL_OK;
 }

@@ -103,6 +103,24 @@ inline cudaStream_t S(zl_stream s) { return reinterpret_cast<cudaStream_t>(s); }
   } while (0)
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Launches `kernel` so that its CTAs may take their places while the kernel ahead of it on the
+// stream drains; every such kernel waits for that one (griddep_wait) before it reads or writes
+// anything. Errors are left for ZL_LAUNCH_CHECK.
+template <typename... P, typename... A>
+inline void launch_ahead(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 inline size_t dtype_size(zl_dtype t) { return t == ZL_F32 ? 4 : 2; }
 inline bool dtype_ok(zl_dtype t) { return t == ZL_F32 || t == ZL_BF16; }
 

@@ -103,6 +103,14 @@ __device__ __forceinline__ void griddep_launch_dependents() {
 // their writes are visible; returns at once otherwise.
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// The first thing in a kernel that was launched ahead (launch_ahead): waits for the grids before,
+// then lets the next one take its place. In this order, so that a grid that starts ahead of this
+// one's end still starts after the end of the one before.
+__device__ __forceinline__ void griddep_enter() {
+  griddep_wait();
+  griddep_launch_dependents();
+}
+
 // ------------------------------------------- cp.async and 16-byte shared loads
 // 16 bytes to shared memory in the background; zeros, and nothing read, where !use.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool use) {
