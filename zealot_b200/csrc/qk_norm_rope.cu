@@ -15,9 +15,9 @@
 // the product in fp32 would be off by 0.06 radians.
 //
 // Measured on one B200 (GPU time, replayed back to back), 32 query and 8 key
-// heads of 128, bf16: 64 tokens into the cache 3.1 us, bound by latency; 53,067
-// tokens into the cache and packed rows 253-257 us, 1.52 GB at 5.9-6.0 TB/s
-// (92 % of the copy rate), bound by HBM with the SMs' issue slots half used.
+// heads of 128, bf16: 64 tokens into the cache 2.9 us, bound by latency; 53,067
+// tokens into the cache and packed rows 251 us, 1.52 GB at 6.07 TB/s (93 % of
+// the copy rate), bound by HBM.
 #include "zl_internal.h"
 #include "zl_pages.h"
 #include "zl_ptx.cuh"
@@ -127,66 +127,60 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(RopeArgs g) {
   }
 }
 
-// E elements: 16 bytes, or 8 for four of bf16.
+// E elements as packed fp32 pairs (one instruction for two): 16 bytes of a row, or 8 for four
+// of bf16.
+namespace px = zl::ptx;
 template <int E>
 struct Run {
-  float x[E];
+  uint64_t p[E / 2];
 };
+__device__ __forceinline__ uint64_t pair_of(uint32_t w) {  // two bf16
+  return px::f2_pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 __device__ __forceinline__ Run<4> load_run(const float* p, Run<4>) {
-  const float4 v = *reinterpret_cast<const float4*>(p);
-  return {{v.x, v.y, v.z, v.w}};
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+  return {{v.x, v.y}};
 }
 __device__ __forceinline__ Run<4> load_run(const __nv_bfloat16* p, Run<4>) {
   const uint2 v = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
-  return {{a.x, a.y, b.x, b.y}};
+  return {{pair_of(v.x), pair_of(v.y)}};
 }
 __device__ __forceinline__ Run<8> load_run(const __nv_bfloat16* p, Run<8>) {
   const uint4 v = *reinterpret_cast<const uint4*>(p);
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-  Run<8> r;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const float2 f = __bfloat1622float2(h[i]);
-    r.x[2 * i] = f.x;
-    r.x[2 * i + 1] = f.y;
-  }
-  return r;
+  return {{pair_of(v.x), pair_of(v.y), pair_of(v.z), pair_of(v.w)}};
+}
+__device__ __forceinline__ uint32_t bf16_pair(uint64_t p) {
+  const float2 f = px::f2_unpack(p);
+  return px::pack_bf16x2(f.x, f.y);
 }
 __device__ __forceinline__ void store_run(float* p, const Run<4>& q) {
-  *reinterpret_cast<float4*>(p) = make_float4(q.x[0], q.x[1], q.x[2], q.x[3]);
+  *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(q.p[0], q.p[1]);
 }
 __device__ __forceinline__ void store_run(__nv_bfloat16* p, const Run<4>& q) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(zl::ptx::pack_bf16x2(q.x[0], q.x[1]), zl::ptx::pack_bf16x2(q.x[2], q.x[3]));
+  *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pair(q.p[0]), bf16_pair(q.p[1]));
 }
 __device__ __forceinline__ void store_run(__nv_bfloat16* p, const Run<8>& q) {
-  *reinterpret_cast<uint4*>(p) =
-      make_uint4(zl::ptx::pack_bf16x2(q.x[0], q.x[1]), zl::ptx::pack_bf16x2(q.x[2], q.x[3]),
-                 zl::ptx::pack_bf16x2(q.x[4], q.x[5]), zl::ptx::pack_bf16x2(q.x[6], q.x[7]));
+  *reinterpret_cast<uint4*>(p) = make_uint4(bf16_pair(q.p[0]), bf16_pair(q.p[1]), bf16_pair(q.p[2]), bf16_pair(q.p[3]));
 }
 
-// Rotates a lane's two runs by the angles of its E pairs. Two pairs' angles are 16 bytes, and
-// those of neighbouring lanes lie side by side: `lanes` such pieces, then the next two pairs'.
+// Rotates a lane's two runs by the angles of its E pairs: 16 bytes (c0, c1, s0, s1) for two of
+// them, `lanes` such pieces of neighbouring lanes side by side, then the next two pairs'.
 template <int E>
-__device__ __forceinline__ void rotate(Run<E>& a, Run<E>& b, const float4* cs, int lanes, bool interleaved) {
+__device__ __forceinline__ void rotate(Run<E>& a, Run<E>& b, const ulonglong2* cs, int lanes, bool interleaved) {
+  constexpr uint64_t kSigns = 0x8000000080000000ull;
 #pragma unroll
-  for (int x = 0; x < E; x += 2) {
-    const float4 t = cs[x / 2 * lanes];
-    if (interleaved) {  // 2 x, 2 x + 1 and 2 x + 2, 2 x + 3 of the 2 E elements in a row
-      Run<E>& q = x < E / 2 ? a : b;
-      const int i = 2 * (x % (E / 2));
-      const float y0 = q.x[i], z0 = q.x[i + 1], y1 = q.x[i + 2], z1 = q.x[i + 3];
-      q.x[i] = y0 * t.x - z0 * t.y;
-      q.x[i + 1] = z0 * t.x + y0 * t.y;
-      q.x[i + 2] = y1 * t.z - z1 * t.w;
-      q.x[i + 3] = z1 * t.z + y1 * t.w;
+  for (int x = 0; x < E / 2; x++) {
+    const ulonglong2 t = cs[x * lanes];
+    if (interleaved) {  // the two pairs are two whole p's of the 2 E elements in a row
+      uint64_t(&q)[E / 2] = x < E / 4 ? a.p : b.p;
+      const int i = 2 * (x % (E / 4));
+      const float2 c = px::f2_unpack(t.x), s = px::f2_unpack(t.y), u = px::f2_unpack(q[i]), v = px::f2_unpack(q[i + 1]);
+      q[i] = px::f2_pack(u.x * c.x - u.y * s.x, u.y * c.x + u.x * s.x);
+      q[i + 1] = px::f2_pack(v.x * c.y - v.y * s.y, v.y * c.y + v.x * s.y);
     } else {
-      const float y0 = a.x[x], z0 = b.x[x], y1 = a.x[x + 1], z1 = b.x[x + 1];
-      a.x[x] = y0 * t.x - z0 * t.y;
-      b.x[x] = z0 * t.x + y0 * t.y;
-      a.x[x + 1] = y1 * t.z - z1 * t.w;
-      b.x[x + 1] = z1 * t.z + y1 * t.w;
+      const uint64_t y = a.p[x], z = b.p[x];
+      a.p[x] = px::f2_fma(z, t.y ^ kSigns, px::f2_mul(y, t.x));
+      b.p[x] = px::f2_fma(y, t.y, px::f2_mul(z, t.x));
     }
   }
 }
@@ -202,15 +196,15 @@ template <typename T>
 struct HeadRows {
   const T* src;  // the head's row of the CTA's first token
   T *out, *pool;
-  const T* w;
   int64_t stride, out_stride;
-  bool use, turn;
+  bool use, turn, norm, isk;
   __device__ __forceinline__ HeadRows(const RopeArgs& g, int h, int64_t t0, bool mine, bool turned) {
-    const bool isq = h < g.H, isk = !isq && h < g.H + g.Hkv;
+    const bool isq = h < g.H;
+    isk = !isq && h < g.H + g.Hkv;
     const int hh = isq ? h : isk ? h - g.H : h - g.H - g.Hkv;
     out = (T*)(isq ? g.q_out : isk ? g.k_out : g.v_out);
     pool = (T*)(isq ? nullptr : isk ? g.k_pool : g.v_pool);
-    w = (const T*)(isq ? g.q_weight : isk ? g.k_weight : nullptr);
+    norm = isq ? g.q_weight != nullptr : isk && g.k_weight;
     use = mine && h < g.H + 2 * g.Hkv && (out || pool);
     turn = turned && (isq || isk);
     stride = isq ? g.q_stride : isk ? g.k_stride : g.v_stride;
@@ -226,8 +220,8 @@ template <int LG, int E>
 struct Lane {  // a lane's place in its row
   int u, e0, e1;
   bool mine, turned;
-  __device__ __forceinline__ explicit Lane(const RopeArgs& g) {
-    u = threadIdx.x % LG;
+  __device__ __forceinline__ explicit Lane(const RopeArgs& g, int lane = threadIdx.x % LG) {
+    u = lane;
     mine = u * 2 * E < g.d;
     turned = u * 2 * E < g.rot;
     const bool halves = turned && !g.interleaved;
@@ -236,36 +230,75 @@ struct Lane {  // a lane's place in its row
   }
 };
 
-// Norms and rotates one row and stores it: token c of the CTA, whose angles are cs and
-// whose pool rows start at element `at` (-1: none).
+// What a CTA's rows share: the weights of q and k in fp32, each lane's in the order of its two
+// runs, 16 bytes of neighbouring lanes side by side; its tokens' angles in rotate()'s order; and,
+// in elements, the pool rows of its tokens' kv head 0 (-1: none).
+template <int LG, int E>
+struct Shared {
+  float4 weights[2][E / 2][LG];
+  ulonglong2* cs;
+  int64_t* cache;
+};
 template <typename T, int LG, int E>
-__device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>& ln, const HeadRows<T>& r, int c,
-                                           Run<E> a, Run<E> b, const float2* cs, int64_t at) {
-  float ss = 0.f, s2 = 0.f;
-#pragma unroll
-  for (int x = 0; x < E; x++) {
-    ss = fmaf(a.x[x], a.x[x], ss);
-    s2 = fmaf(b.x[x], b.x[x], s2);
+__device__ __forceinline__ void fill_shared(const RopeArgs& g, int64_t t0, int tokens, Shared<LG, E>& sh) {
+  const int half = g.rot / 2;
+  float* cs = reinterpret_cast<float*>(sh.cs);
+  for (int i = threadIdx.x; i < tokens * half; i += 256) {
+    const int t = i / half, p = i - t * half, u = p / E, x = p % E;  // pair x of lane u
+    const float2 y = turn(g.positions[t0 + t], g.inv_freq[p]);
+    float* to = cs + 2 * t * half + (x / 2 * (half / E) + u) * 4 + x % 2;
+    to[0] = y.x;
+    to[2] = y.y;
   }
-  ss += s2;
+  for (int i = threadIdx.x; i < 2 * (E / 2) * LG; i += 256) {
+    const int which = i / (E / 2 * LG), j = i / LG % (E / 2);
+    const T* w = (const T*)(which ? g.k_weight : g.q_weight);
+    const Lane<LG, E> ln(g, i % LG);
+    if (w && ln.mine) {
+      w += (j < E / 4 ? ln.e0 : ln.e1 - E) + 4 * j;
+      sh.weights[which][j][ln.u] = make_float4(to_f(w[0]), to_f(w[1]), to_f(w[2]), to_f(w[3]));
+    }
+  }
+  if (threadIdx.x < tokens) {
+    const int64_t row = cache_row(g, t0 + threadIdx.x, 0);
+    sh.cache[threadIdx.x] = row < 0 ? -1 : row * g.d;
+  }
+}
+
+// Norms and rotates one row and stores it to `out` (unless r.out is null) and to the pool row at
+// element `at` (unless -1); cs: its token's angles.
+template <typename T, int LG, int E>
+__device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>& ln, const HeadRows<T>& r, Run<E> a,
+                                           Run<E> b, const Shared<LG, E>& sh, const ulonglong2* cs, T* out, int64_t at) {
+  uint64_t sa = 0, sb = 0;
+#pragma unroll
+  for (int x = 0; x < E / 2; x++) {
+    sa = px::f2_fma(a.p[x], a.p[x], sa);
+    sb = px::f2_fma(b.p[x], b.p[x], sb);
+  }
+  const float2 both = px::f2_unpack(px::f2_add(sa, sb));
+  float ss = both.x + both.y;
 #pragma unroll
   for (int o = LG / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (!r.use) return;
-  if (r.w) {
-    const Run<E> wa = load_run(r.w + ln.e0, Run<E>{}), wb = load_run(r.w + ln.e1, Run<E>{});
+  if (r.norm) {
     const float y = ss * g.inv_d + g.eps, q = rsqrtf(y);
     const float inv = q * fmaf(-0.5f * y * q, q, 1.5f);  // a Newton step: right to fp32's last place or so
+    const uint64_t inv2 = px::f2_pack(inv, inv);
+    const ulonglong2* w = reinterpret_cast<const ulonglong2*>(&sh.weights[r.isk][0][ln.u]);
 #pragma unroll
-    for (int x = 0; x < E; x++) {
-      a.x[x] = a.x[x] * inv * wa.x[x];
-      b.x[x] = b.x[x] * inv * wb.x[x];
+    for (int j = 0; j < E / 4; j++) {
+      const ulonglong2 wa = w[j * LG], wb = w[(E / 4 + j) * LG];
+      a.p[2 * j] = px::f2_mul(px::f2_mul(a.p[2 * j], inv2), wa.x);
+      a.p[2 * j + 1] = px::f2_mul(px::f2_mul(a.p[2 * j + 1], inv2), wa.y);
+      b.p[2 * j] = px::f2_mul(px::f2_mul(b.p[2 * j], inv2), wb.x);
+      b.p[2 * j + 1] = px::f2_mul(px::f2_mul(b.p[2 * j + 1], inv2), wb.y);
     }
   }
-  if (r.turn) rotate(a, b, reinterpret_cast<const float4*>(cs) + ln.u, g.rot / (2 * E), g.interleaved);
+  if (r.turn) rotate(a, b, cs + ln.u, g.rot / (2 * E), g.interleaved);
   if (r.out) {
-    T* to = r.out + c * r.out_stride;
-    store_run(to + ln.e0, a);
-    store_run(to + ln.e1, b);
+    store_run(out + ln.e0, a);
+    store_run(out + ln.e1, b);
   }
   if (r.pool && at >= 0) {
     store_run(r.pool + at + ln.e0, a);
@@ -273,25 +306,12 @@ __device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>&
   }
 }
 
-// The CTA's angles, in rotate()'s order, and, in elements, the pool rows of its tokens' kv head 0.
-template <int E>
-__device__ __forceinline__ void token_tables(const RopeArgs& g, int64_t t0, int tokens, float2* cs, int64_t* cache) {
-  const int half = g.rot / 2;
-  for (int i = threadIdx.x; i < tokens * half; i += 256) {
-    const int t = i / half, p = i - t * half, u = p / E, x = p % E;  // pair x of lane u
-    cs[t * half + (x / 2 * (half / E) + u) * 2 + x % 2] = turn(g.positions[t0 + t], g.inv_freq[p]);
-  }
-  if (threadIdx.x < tokens) {
-    const int64_t row = cache_row(g, t0 + threadIdx.x, 0);
-    cache[threadIdx.x] = row < 0 ? -1 : row * g.d;
-  }
-}
-
 // Few tokens: one to a CTA, and its heads over gridDim.y of them.
 template <typename T, int LG, int E>
 __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
   zl::ptx::griddep_enter();
-  __shared__ __align__(16) float2 cs[kMaxDim / 2];
+  __shared__ Shared<LG, E> sh;
+  __shared__ ulonglong2 cs[kMaxDim / 4];
   __shared__ int64_t cache[1];
   const Lane<LG, E> ln(g);
   const int64_t t0 = blockIdx.x;
@@ -305,11 +325,16 @@ __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
       b = load_run(r.src + ln.e1, b);
     }
     if (!tables) {  // while the row is on its way
-      token_tables<E>(g, t0, 1, cs, cache);
+      if (threadIdx.x == 0) {
+        sh.cs = cs;
+        sh.cache = cache;
+      }
+      __syncthreads();
+      fill_shared<T, LG, E>(g, t0, 1, sh);
       __syncthreads();
       tables = true;
     }
-    finish_row(g, ln, r, 0, a, b, cs, cache[0]);
+    finish_row(g, ln, r, a, b, sh, cs, r.out, cache[0]);
   }
 }
 
@@ -317,68 +342,77 @@ __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
 // kAhead - 1 steps from now into its own slots of shared memory, in the background: bytes on
 // their way without registers, and without a barrier, since each thread waits for its own.
 // 53,067 tokens as above: loads into registers 649 us (462 with two tokens at a time: too few
-// bytes on their way), these copies in runs of 8 bytes 268-284, of 16 bytes 273, and with the
-// angles in an order without bank conflicts 254-260.
+// bytes on their way), these copies in runs of 8 bytes 268-284, of 16 bytes 273, with the
+// angles in an order without bank conflicts 254-260, on packed pairs 251. Run for a second the
+// board's power limit holds it at 270-274.
 // The groups are shared out as `hpb` heads by `slices` parts of the tokens.
 constexpr int kTokens = 16, kAhead = 4, kFew = 2;
-// CTAs to an SM, by registers (80 or 64 a thread): bf16 254 us with 3 and 260 with 4, fp32 (20,000
-// tokens of the same heads) 193 and 190.
-template <typename T> constexpr int kResident = sizeof(T) == 2 ? 3 : 4;
+constexpr int kResident = 4;  // CTAs to an SM: 64 registers a thread; with 3 of 80, 252 us and, at 4,096 tokens, 25.6, not 24.1
 template <typename T, int LG, int E>
-__global__ void __launch_bounds__(256, kResident<T>) rope_tokens_kernel(RopeArgs g, int per, int hpb, int slices) {
+__global__ void __launch_bounds__(256, kResident) rope_tokens_kernel(RopeArgs g, int per, int hpb, int slices) {
   zl::ptx::griddep_enter();
-  constexpr int RUN = E * sizeof(T);
+  constexpr int RUN = E * sizeof(T), SLOT = 256 * 2 * RUN;
   extern __shared__ __align__(16) uint8_t dyn[];  // [kAhead][2][256] runs, then the angles
+  __shared__ Shared<LG, E> sh;
   __shared__ int64_t cache[kTokens];
-  float2* cs = reinterpret_cast<float2*>(dyn + kAhead * 256 * 2 * RUN);
+  ulonglong2* cs = reinterpret_cast<ulonglong2*>(dyn + kAhead * SLOT);
+  if (threadIdx.x == 0) {
+    sh.cs = cs;
+    sh.cache = cache;
+  }
   const Lane<LG, E> ln(g);
   const int64_t t0 = (int64_t)blockIdx.x * per;
-  const int tokens = (int)min((int64_t)per, g.tokens - t0), half = g.rot / 2, group = threadIdx.x / LG;
+  const int tokens = (int)min((int64_t)per, g.tokens - t0), group = threadIdx.x / LG;
   const int slice = group / hpb, heads = slice < slices ? g.H + 2 * g.Hkv : 0;  // a group that is left over: none
-  const uint32_t slots = zl::ptx::smem_u32(dyn) + threadIdx.x * RUN;
+  const uint32_t mine = zl::ptx::smem_u32(dyn) + threadIdx.x * RUN;
   int h2 = group - slice * hpb, c2 = slice;  // head and token of the next copy
   if (c2 >= tokens) h2 = heads;
   HeadRows<T> ahead(g, h2, t0, ln.mine, ln.turned), r = ahead;
   int h = h2, c = c2;
-  auto fetch = [&](int slot) {
+  const T* src = ahead.src + c2 * ahead.stride;
+  T* out = r.out + c * r.out_stride;
+  uint32_t to = mine, from = threadIdx.x * RUN;  // slots of the next copy and of the next step
+  auto fetch = [&]() {
     if (h2 < heads) {
       if (ahead.use) {
-        const uint32_t to = slots + slot * 256 * 2 * RUN;
-        const T* src = ahead.src + c2 * ahead.stride;
         zl::ptx::copy_async<RUN>(to, src + ln.e0);
         zl::ptx::copy_async<RUN>(to + 256 * RUN, src + ln.e1);
       }
+      src += slices * ahead.stride;
       if ((c2 += slices) >= tokens) {
         c2 = slice;
         h2 += hpb;
         ahead = HeadRows<T>(g, h2, t0, ln.mine, ln.turned);
+        src = ahead.src + c2 * ahead.stride;
       }
     }
+    to = to == mine + (kAhead - 1) * SLOT ? mine : to + SLOT;
     zl::ptx::copies_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kAhead - 1; i++) fetch(i);
-  token_tables<E>(g, t0, tokens, cs, cache);
+  for (int i = 0; i < kAhead - 1; i++) fetch();
+  __syncthreads();
+  fill_shared<T, LG, E>(g, t0, tokens, sh);
   __syncthreads();
   // a warp's groups take their last steps together: the sum over lanes needs them all
-  int s = 0;
   while (__any_sync(0xffffffffu, h < heads)) {
-    fetch((s + kAhead - 1) % kAhead);
+    fetch();
     zl::ptx::copies_wait<kAhead - 1>();
-    const T* slot = reinterpret_cast<const T*>(dyn + (s % kAhead * 2 * 256 + threadIdx.x) * RUN);
     r.use = r.use && h < heads;
     Run<E> a{}, b{};  // zeros in the lanes behind the row's end: they take part in its sum
     if (r.use) {
-      a = load_run(slot, a);
-      b = load_run(slot + 256 * E, b);
+      a = load_run(reinterpret_cast<const T*>(dyn + from), a);
+      b = load_run(reinterpret_cast<const T*>(dyn + from + 256 * RUN), b);
     }
-    finish_row(g, ln, r, c, a, b, cs + c * half, r.use ? cache[c] : -1);
+    finish_row(g, ln, r, a, b, sh, cs + c * (g.rot / 4), out, r.use && r.pool ? cache[c] : -1);
+    from = from == threadIdx.x * RUN + (kAhead - 1) * SLOT ? threadIdx.x * RUN : from + SLOT;
+    out += slices * r.out_stride;
     if (h < heads && (c += slices) >= tokens) {
       c = slice;
       h += hpb;
       r = HeadRows<T>(g, h, t0, ln.mine, ln.turned);
+      out = r.out + c * r.out_stride;
     }
-    s++;
   }
   zl::ptx::copies_wait<0>();
 }
@@ -389,7 +423,7 @@ zl_status launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
   constexpr int NG = 256 / LG;
   const int heads = g.H + 2 * g.Hkv, blocks = (heads + NG - 1) / NG;
   // CTAs that the GPU has room for at once, and tokens to a CTA that fill whole rounds of them
-  const int64_t room = kResident<T> * (int64_t)num_sms, rounds = (g.tokens + room * kTokens - 1) / (room * kTokens);
+  const int64_t room = kResident * (int64_t)num_sms, rounds = (g.tokens + room * kTokens - 1) / (room * kTokens);
   const int64_t per = (g.tokens + room * rounds - 1) / (room * rounds);
   if (per < kFew) {  // one token to a CTA: 1,024 tokens 13.2 us this way, 10.9 two to a CTA; 64 tokens 3.1
     launch_ahead(rope_token_kernel<T, LG, E>, dim3((unsigned)g.tokens, blocks < 65535 ? blocks : 65535), 256, 0, st, g);
