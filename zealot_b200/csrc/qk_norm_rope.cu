@@ -171,7 +171,7 @@ __device__ __forceinline__ void rotate(Run<E>& a, Run<E>& b, const ulonglong2* c
 #pragma unroll
   for (int x = 0; x < E / 2; x++) {
     const ulonglong2 t = cs[x * lanes];
-    if (interleaved) {  // the two pairs are two whole p's of the 2 E elements in a row
+    if (interleaved) {  // the two pairs are two whole p's of a run
       uint64_t(&q)[E / 2] = x < E / 4 ? a.p : b.p;
       const int i = 2 * (x % (E / 4));
       const float2 c = px::f2_unpack(t.x), s = px::f2_unpack(t.y), u = px::f2_unpack(q[i]), v = px::f2_unpack(q[i + 1]);
@@ -187,46 +187,48 @@ __device__ __forceinline__ void rotate(Run<E>& a, Run<E>& b, const ulonglong2* c
 
 // Rows that loads of E elements can read, head_dim and rotary_dim multiples of 2 E. LG lanes
 // (a power of two, at least d / (2 E)) share a row; a lane has two runs of E of its elements,
-// the pairs E u .. E u + E - 1, whose elements lie in the two halves of the rotated part (or,
-// interleaved, side by side), so that a rotation needs no exchange between lanes. A CTA takes
+// one in either half of the rotated part: E pairs (or, interleaved, E / 2 whole pairs in each
+// run), so that a rotation needs no exchange between lanes. A CTA takes
 // `per` tokens; their angles, once for all heads, and their cache rows go to shared memory.
 // A lane group keeps to one head (of q, then k, then v) over its tokens, then takes the next.
 // HeadRows is that head: where its rows come from and go to.
 template <typename T>
 struct HeadRows {
-  const T* src;  // the head's row of the CTA's first token
+  const T* src;  // this lane's first run in the head's row of the CTA's first token; so in out and pool
   T *out, *pool;
   int64_t stride, out_stride;
   bool use, turn, norm, isk;
-  __device__ __forceinline__ HeadRows(const RopeArgs& g, int h, int64_t t0, bool mine, bool turned) {
+  template <typename L>
+  __device__ __forceinline__ HeadRows(const RopeArgs& g, const L& ln, int h, int64_t t0) {
     const bool isq = h < g.H;
     isk = !isq && h < g.H + g.Hkv;
     const int hh = isq ? h : isk ? h - g.H : h - g.H - g.Hkv;
     out = (T*)(isq ? g.q_out : isk ? g.k_out : g.v_out);
     pool = (T*)(isq ? nullptr : isk ? g.k_pool : g.v_pool);
     norm = isq ? g.q_weight != nullptr : isk && g.k_weight;
-    use = mine && h < g.H + 2 * g.Hkv && (out || pool);
-    turn = turned && (isq || isk);
+    use = ln.mine && h < g.H + 2 * g.Hkv && (out || pool);
+    turn = ln.turned && (isq || isk);
     stride = isq ? g.q_stride : isk ? g.k_stride : g.v_stride;
     out_stride = (int64_t)(isq ? g.H : g.Hkv) * g.d;
     src = (const T*)(isq ? g.q : isk ? g.k : g.v);
-    if (use) src += t0 * stride + (int64_t)hh * g.d;
-    if (out) out += t0 * out_stride + (int64_t)hh * g.d;
-    if (pool) pool += (int64_t)hh * g.bs * g.d;
+    if (use) src += t0 * stride + (int64_t)hh * g.d + ln.e0;
+    if (out) out += t0 * out_stride + (int64_t)hh * g.d + ln.e0;
+    if (pool) pool += (int64_t)hh * g.bs * g.d + ln.e0;
   }
 };
 
 template <int LG, int E>
 struct Lane {  // a lane's place in its row
-  int u, e0, e1;
+  int u, e0, gap;  // its first run's place and how far behind it the second lies
   bool mine, turned;
   __device__ __forceinline__ explicit Lane(const RopeArgs& g, int lane = threadIdx.x % LG) {
     u = lane;
     mine = u * 2 * E < g.d;
     turned = u * 2 * E < g.rot;
-    const bool halves = turned && !g.interleaved;
-    e0 = halves ? E * u : 2 * E * u;
-    e1 = halves ? g.rot / 2 + E * u : 2 * E * u + E;
+    // the two halves of the rotated part, or of the rest: neighbouring lanes' runs lie side by side
+    const int from = turned ? 0 : g.rot, len = turned ? g.rot : g.d - g.rot, v = u - from / (2 * E);
+    e0 = from + E * v;
+    gap = len / 2;
   }
 };
 
@@ -244,7 +246,14 @@ __device__ __forceinline__ void fill_shared(const RopeArgs& g, int64_t t0, int t
   const int half = g.rot / 2;
   float* cs = reinterpret_cast<float*>(sh.cs);
   for (int i = threadIdx.x; i < tokens * half; i += 256) {
-    const int t = i / half, p = i - t * half, u = p / E, x = p % E;  // pair x of lane u
+    const int t = i / half, p = i - t * half;
+    // pair x of lane u: its E pairs' elements are in both runs; interleaved, E / 2 pairs in either run
+    int u = p / E, x = p % E;
+    if (g.interleaved) {
+      const int second = p >= half / 2, q = second ? p - half / 2 : p;
+      u = q / (E / 2);
+      x = q % (E / 2) + (second ? E / 2 : 0);
+    }
     const float2 y = turn(g.positions[t0 + t], g.inv_freq[p]);
     float* to = cs + 2 * t * half + (x / 2 * (half / E) + u) * 4 + x % 2;
     to[0] = y.x;
@@ -255,7 +264,7 @@ __device__ __forceinline__ void fill_shared(const RopeArgs& g, int64_t t0, int t
     const T* w = (const T*)(which ? g.k_weight : g.q_weight);
     const Lane<LG, E> ln(g, i % LG);
     if (w && ln.mine) {
-      w += (j < E / 4 ? ln.e0 : ln.e1 - E) + 4 * j;
+      w += ln.e0 + (j < E / 4 ? 0 : ln.gap - E) + 4 * j;
       sh.weights[which][j][ln.u] = make_float4(to_f(w[0]), to_f(w[1]), to_f(w[2]), to_f(w[3]));
     }
   }
@@ -297,12 +306,12 @@ __device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>&
   }
   if (r.turn) rotate(a, b, cs + ln.u, g.rot / (2 * E), g.interleaved);
   if (r.out) {
-    store_run(out + ln.e0, a);
-    store_run(out + ln.e1, b);
+    store_run(out, a);
+    store_run(out + ln.gap, b);
   }
   if (r.pool && at >= 0) {
-    store_run(r.pool + at + ln.e0, a);
-    store_run(r.pool + at + ln.e1, b);
+    store_run(r.pool + at, a);
+    store_run(r.pool + at + ln.gap, b);
   }
 }
 
@@ -318,11 +327,11 @@ __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
   bool tables = false;
   // every group of a CTA goes through the loop equally often (the barrier inside)
   for (int h0 = blockIdx.y * (256 / LG); h0 < g.H + 2 * g.Hkv; h0 += gridDim.y * (256 / LG)) {
-    const HeadRows<T> r(g, h0 + threadIdx.x / LG, t0, ln.mine, ln.turned);
+    const HeadRows<T> r(g, ln, h0 + threadIdx.x / LG, t0);
     Run<E> a{}, b{};
     if (r.use) {
-      a = load_run(r.src + ln.e0, a);
-      b = load_run(r.src + ln.e1, b);
+      a = load_run(r.src, a);
+      b = load_run(r.src + ln.gap, b);
     }
     if (!tables) {  // while the row is on its way
       if (threadIdx.x == 0) {
@@ -344,7 +353,7 @@ __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
 // 53,067 tokens as above: loads into registers 649 us (462 with two tokens at a time: too few
 // bytes on their way), these copies in runs of 8 bytes 268-284, of 16 bytes 273, with the
 // angles in an order without bank conflicts 254-260, on packed pairs 251. Run for a second the
-// board's power limit holds it at 270-274.
+// board's power limit holds it at 268-272.
 // The groups are shared out as `hpb` heads by `slices` parts of the tokens.
 constexpr int kTokens = 16, kAhead = 4, kFew = 2;
 constexpr int kResident = 4;  // CTAs to an SM: 64 registers a thread; with 3 of 80, 252 us and, at 4,096 tokens, 25.6, not 24.1
@@ -367,7 +376,7 @@ __global__ void __launch_bounds__(256, kResident) rope_tokens_kernel(RopeArgs g,
   const uint32_t mine = zl::ptx::smem_u32(dyn) + threadIdx.x * RUN;
   int h2 = group - slice * hpb, c2 = slice;  // head and token of the next copy
   if (c2 >= tokens) h2 = heads;
-  HeadRows<T> ahead(g, h2, t0, ln.mine, ln.turned), r = ahead;
+  HeadRows<T> ahead(g, ln, h2, t0), r = ahead;
   int h = h2, c = c2;
   const T* src = ahead.src + c2 * ahead.stride;
   T* out = r.out + c * r.out_stride;
@@ -375,14 +384,14 @@ __global__ void __launch_bounds__(256, kResident) rope_tokens_kernel(RopeArgs g,
   auto fetch = [&]() {
     if (h2 < heads) {
       if (ahead.use) {
-        zl::ptx::copy_async<RUN>(to, src + ln.e0);
-        zl::ptx::copy_async<RUN>(to + 256 * RUN, src + ln.e1);
+        zl::ptx::copy_async<RUN>(to, src);
+        zl::ptx::copy_async<RUN>(to + 256 * RUN, src + ln.gap);
       }
       src += slices * ahead.stride;
       if ((c2 += slices) >= tokens) {
         c2 = slice;
         h2 += hpb;
-        ahead = HeadRows<T>(g, h2, t0, ln.mine, ln.turned);
+        ahead = HeadRows<T>(g, ln, h2, t0);
         src = ahead.src + c2 * ahead.stride;
       }
     }
@@ -410,7 +419,7 @@ __global__ void __launch_bounds__(256, kResident) rope_tokens_kernel(RopeArgs g,
     if (h < heads && (c += slices) >= tokens) {
       c = slice;
       h += hpb;
-      r = HeadRows<T>(g, h, t0, ln.mine, ln.turned);
+      r = HeadRows<T>(g, ln, h, t0);
       out = r.out + c * r.out_stride;
     }
   }
