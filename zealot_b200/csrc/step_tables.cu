@@ -18,16 +18,15 @@
 // Measured on one B200 (GPU time, replayed back to back): 64 decode rows with
 // tables of 257 blocks 3.7 us, bound by latency (two dependent reads, the sums,
 // one more read). 1,024 requests with tables of 8,192 blocks and 65,536 token
-// rows 17.6 us: 49.7 MB, 2.8 TB/s, of which some 6 us are every CTA's own sums.
+// rows 17.2 us: 49.7 MB, 2.9 TB/s, of which some 5 us are every CTA's own sums.
 // On the way there: 4-byte entries 88 us, 16-byte ones 25, 32-bit divisions
-// 20, all of a stretch's loads before its first store and CTAs of 512 threads 17.
+// 20, all of a stretch's loads before its first store and larger CTAs 17.
 #include "zl_internal.h"
 #include "zl_pages.h"
 #include "zl_ptx.cuh"
 
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kMaxSeqs = 8192;      // requests of one step: 16 bytes of shared memory each
 constexpr int kMaxRows = 1 << 18;   // rows of the persistent table: 2 bits of shared memory each
 
@@ -49,6 +48,7 @@ struct StepArgs {
 };
 
 // Exclusive sums of a[0..n) and b[0..n) in place, total of a returned in a[n].
+template <int kThreads>
 __device__ void scan2(int32_t* a, int32_t* b, int n) {
   __shared__ int32_t wa[kThreads / 32], wb[kThreads / 32];
   const int per = (n + kThreads - 1) / kThreads, lo = min(n, (int)threadIdx.x * per), hi = min(n, lo + per);
@@ -138,7 +138,7 @@ __device__ __forceinline__ bool table_columns(const StepArgs& g, int i, int c, i
 // A CTA takes units: kThreads / lanes stretches of table rows at a time, `lanes` threads (a
 // power of two) to a stretch of lanes * N * kDepth columns, then stretches of kThreads token rows.
 constexpr int kDepth = 4;
-template <int N>
+template <int N, int kThreads>
 __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g, int log_lanes) {
   zl::ptx::griddep_enter();
   extern __shared__ int32_t sh[];
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g, int l
     }
   }
   __syncthreads();
-  scan2(cu, fresh, n);
+  scan2<kThreads>(cu, fresh, n);
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int r = row[i];
@@ -190,9 +190,10 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs g, int l
       g.last_rows[i] = max(min(cu[i + 1], cap) - 1, 0);
     }
   }
-  const int lanes = 1 << log_lanes, width = lanes * N * kDepth, stretches = (g.max_blocks + width - 1) / width, at_once = kThreads >> log_lanes;
-  // fewer than 2^32: at most 2^13 requests of 2^17 stretches (a table row of at most 2^30 columns, and all
-  // threads to a stretch of such), and fewer than 2^23 stretches of tokens
+  const int lanes = 1 << log_lanes, width = lanes * N * kDepth, stretches = (g.max_blocks + width - 1) / width;
+  const int at_once = kThreads >> log_lanes;
+  // fewer than 2^32: at most 2^13 requests of 2^18 stretches (a table row of at most 2^30 columns, and all
+  // threads to a stretch of such), and fewer than 2^22 stretches of tokens
   const uint32_t pieces = (uint32_t)n * stretches, tables = (pieces + at_once - 1) / at_once;
   const uint32_t units = tables + (uint32_t)((g.num_tokens + kThreads - 1) / kThreads);
   for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
@@ -282,14 +283,19 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
              block_size, ctx->d_status};
   const size_t smem = sizeof(int32_t) * (4 * (size_t)num_seqs + 1) + (rows ? 8 * (size_t)((num_rows + 31) / 32) : 0);
   const bool vec = max_blocks_per_seq % 4 == 0 && aligned16(seq_blocks) && aligned16(block_tables);
-  const auto kernel = vec ? step_tables_kernel<4> : step_tables_kernel<1>;
+  // Two CTAs of 512 threads to an SM, or one of 1,024 that takes the sums over many requests once:
+  // 64 rows of 257 blocks 3.5 and 4.2 us, 1,024 rows 7.7 and 5.9, 4,000 rows 24.8 and 12.5.
+  const bool many = num_seqs > 512;
+  const int kThreads = many ? 1024 : 512;
+  const auto kernel = many ? (vec ? step_tables_kernel<4, 1024> : step_tables_kernel<1, 1024>)
+                           : (vec ? step_tables_kernel<4, 512> : step_tables_kernel<1, 512>);
   if (smem > 32 * 1024)  // with the static part it may pass 48 KB
     ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   // Threads to a table row: one step of each while all rows then fit the GPU at once (the
   // shortest way for a small step: 64 rows of 257 blocks 3.7 us, 4.0 with kDepth steps of a
   // quarter of the threads), kDepth steps otherwise (1,024 rows of 8,192: 17.6 us, 20 with one).
   const int wide = vec ? 4 : 1;
-  const int64_t most = 2 * ctx->num_sms;
+  const int64_t most = (many ? 1 : 2) * ctx->num_sms;
   int log_lanes = 3;
   while (1 << log_lanes < kThreads && (int64_t)wide << log_lanes < max_blocks_per_seq) log_lanes++;
   while (log_lanes > 3 && ((int64_t)num_seqs << log_lanes) > most * kThreads &&
