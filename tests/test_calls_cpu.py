@@ -32,6 +32,27 @@ def test_addresses():
         calls.addresses(-1, f, torch.float32, "12")
 
 
+def test_head_rows():
+    import torch
+    from zealot_b200 import calls
+    f = torch.float32
+    row = torch.zeros((5, 40))
+    q, k = row[:, :24].unflatten(1, (6, 4)), row[:, 24:32].unflatten(1, (2, 4))
+    assert calls.head_rows(-1, f, 5, 4, q, 6, k, 2) == (q.data_ptr(), 40, k.data_ptr(), 40)
+    assert calls.head_rows(-1, f, 5, 4) == ()
+    one = torch.zeros((5, 1, 4)).expand(5, 1, 4)
+    assert calls.head_rows(-1, f, 5, 4, one, 1) == (one.data_ptr(), 4)
+    for bad, heads in ((q.transpose(1, 2), 4), (q[..., ::2], 6), (q, 5), (q[:4], 6), (q.double(), 6), (row, 6), (q[None], 6)):
+        assert calls.head_rows(-1, f, 5, 4, k, 2, bad, heads) == 1
+    assert calls.head_rows(0, f, 5, 4, q, 6) == 0  # another device
+    with pytest.raises(TypeError):
+        calls.head_rows(-1, f, 5, 4, q)
+    with pytest.raises(TypeError):
+        calls.head_rows(-1, f, 5, "4", q, 6)
+    with pytest.raises(AttributeError):
+        calls.head_rows(-1, f, 5, 4, "q", 6)
+
+
 @pytest.mark.parametrize("name", list(CALLS))
 def test_calls_pass_what_ctypes_passes(name):
     """Each argument changed in turn to one that the C function refuses in words: the same status and words."""

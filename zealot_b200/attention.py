@@ -66,17 +66,14 @@ class CudaAttention:
         rotation), and the stores: q_out, k_out, v_out packed, and the pools [num_blocks][Hkv][bs][d] at
         slot_mapping. q, k and v may be views of one projection's rows (any stride from token to token)."""
         import torch
-        dtype, device = q.dtype, self.ctx.device
+        dtype = q.dtype
         T, H, d = q.shape
         Hkv = k.shape[1]
-        strides = []
-        for t, n in ((q, H), (k, Hkv), (v, Hkv)):
-            if t.dtype is not dtype or t.get_device() != device or t.shape != (T, n, d):
-                raise InvalidArgument("q [T][H][d], k and v [T][Hkv][d]: one dtype, on the context's device")
-            token, head, element = t.stride()
-            if (element != 1 and d != 1) or (head != d and n != 1):
-                raise InvalidArgument("the heads of a token are packed")
-            strides.append(token)
+        rows = calls.head_rows(self.ctx.device, dtype, T, d, q, H, k, Hkv, v, Hkv)
+        if type(rows) is not tuple:
+            raise InvalidArgument("q [T][H][d], k and v [T][Hkv][d]: one dtype, on the context's device, the heads of a "
+                                  f"token packed; {'qkv'[rows]} is not")
+        qa, qs, ka, ks, va, vs = rows
         rot = bs = num_blocks = pool = 0
         if inv_freq is not None:
             _need(positions is not None, "inv_freq needs positions")
@@ -92,9 +89,9 @@ class CudaAttention:
             q_out, dtype, T * H * d, k_out, dtype, nk, v_out, dtype, nk, q_weight, dtype, d, k_weight, dtype, d,
             positions, torch.int32, T, inv_freq, torch.float64, rot // 2, k_pool, dtype, pool, v_pool, dtype, pool,
             slot_mapping, torch.int64, T)
-        check(calls.qk_norm_rope(self.ctx.address, q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, qw, kw,
-                                 eps, pos, freq, rot, int(interleaved), qo, ko, vo, kp, vp, slots, bs, num_blocks, T,
-                                 H, Hkv, d, dtype_code(dtype), self.ctx.stream(stream)))
+        check(calls.qk_norm_rope(self.ctx.address, qa, ka, va, qs, ks, vs, qw, kw, eps, pos, freq, rot,
+                                 int(interleaved), qo, ko, vo, kp, vp, slots, bs, num_blocks, T, H, Hkv, d,
+                                 dtype_code(dtype), self.ctx.stream(stream)))
 
     # ------------------------------------------------------------ KV scatter
     def reshape_and_cache(self, k, v, k_pool, v_pool, slot_mapping, num_kv_heads: int,

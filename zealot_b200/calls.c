@@ -11,7 +11,7 @@
 
 #include "zealot_attn.h"
 
-static PyObject *s_dtype, *s_numel, *s_get_device, *s_is_contiguous, *s_data_ptr;
+static PyObject *s_dtype, *s_numel, *s_get_device, *s_is_contiguous, *s_data_ptr, *s_shape, *s_stride;
 
 static PyObject* method(PyObject* o, PyObject* name) {
   PyObject* args[1] = {o};
@@ -75,6 +75,46 @@ static PyObject* addresses(PyObject* self, PyObject* const* args, Py_ssize_t nar
       return NULL;
     }
     PyTuple_SET_ITEM(out, i, a);
+  }
+  return out;
+}
+
+/* item i of a tuple of whole numbers */
+static long long item(PyObject* t, Py_ssize_t i) { return PyLong_AsLongLong(PyTuple_GET_ITEM(t, i)); }
+
+/* head_rows(device, dtype, T, d, tensor, heads, tensor, heads, ...) -> (address, token stride, ...)
+ * of tensors [T][heads][d] whose heads lie side by side, or the number of the first that is none. */
+static PyObject* head_rows(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs < 4 || nargs % 2) {
+    PyErr_SetString(PyExc_TypeError, "head_rows(device, dtype, T, d, tensor, heads, ...)");
+    return NULL;
+  }
+  const long long device = PyLong_AsLongLong(args[0]), T = PyLong_AsLongLong(args[2]), d = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred()) return NULL;
+  const Py_ssize_t count = (nargs - 4) / 2;
+  PyObject* out = PyTuple_New(2 * count);
+  if (!out) return NULL;
+  for (Py_ssize_t i = 0; i < count; i++) {
+    PyObject *t = args[4 + 2 * i], *kind = NULL, *shape = NULL, *stride = NULL, *a = NULL, *step = NULL;
+    const long long heads = PyLong_AsLongLong(args[5 + 2 * i]);
+    int ok = !PyErr_Occurred() && (kind = PyObject_GetAttr(t, s_dtype)) && (shape = PyObject_GetAttr(t, s_shape)) &&
+             (stride = method(t, s_stride));
+    if (ok) {
+      ok = kind == args[1] && PyTuple_Check(shape) && PyTuple_Check(stride) && PyTuple_GET_SIZE(shape) == 3 &&
+           PyTuple_GET_SIZE(stride) == 3 && item(shape, 0) == T && item(shape, 1) == heads && item(shape, 2) == d &&
+           (item(stride, 2) == 1 || d == 1) && (item(stride, 1) == d || heads == 1) && number(t, s_get_device) == device;
+      if (ok && (a = method(t, s_data_ptr))) step = Py_NewRef(PyTuple_GET_ITEM(stride, 0));
+    }
+    Py_XDECREF(kind);
+    Py_XDECREF(shape);
+    Py_XDECREF(stride);
+    if (!step) {
+      Py_XDECREF(a);
+      Py_DECREF(out);
+      return PyErr_Occurred() ? NULL : PyLong_FromSsize_t(i);
+    }
+    PyTuple_SET_ITEM(out, 2 * i, a);
+    PyTuple_SET_ITEM(out, 2 * i + 1, step);
   }
   return out;
 }
@@ -151,6 +191,8 @@ RUN(zl_paged_decode_selected(ctx, q, kp, vp, tables, lens, selected, o, B, H, Hk
 static PyMethodDef methods[] = {
     {"addresses", (PyCFunction)(void (*)(void))addresses, METH_FASTCALL,
      "addresses(device, tensor, dtype, elements, ...): a tuple, or the number of the first tensor that does not fit"},
+    {"head_rows", (PyCFunction)(void (*)(void))head_rows, METH_FASTCALL,
+     "head_rows(device, dtype, T, d, tensor, heads, ...): a tuple, or the number of the first tensor that does not fit"},
     ENTRY(step_tables), ENTRY(qk_norm_rope), ENTRY(block_bounds), ENTRY(block_scores), ENTRY(select_blocks),
     ENTRY(paged_decode_selected), {NULL, NULL, 0, NULL}};
 
@@ -162,6 +204,8 @@ PyMODINIT_FUNC PyInit_calls(void) {
   s_get_device = PyUnicode_InternFromString("get_device");
   s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
   s_data_ptr = PyUnicode_InternFromString("data_ptr");
-  if (!s_dtype || !s_numel || !s_get_device || !s_is_contiguous || !s_data_ptr) return NULL;
+  s_shape = PyUnicode_InternFromString("shape");
+  s_stride = PyUnicode_InternFromString("stride");
+  if (!s_dtype || !s_numel || !s_get_device || !s_is_contiguous || !s_data_ptr || !s_shape || !s_stride) return NULL;
   return PyModule_Create(&module);
 }
