@@ -457,9 +457,11 @@ __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts,
 // the number of keys above the threshold before it and of equal ones, of which the
 // first few count: no key's place depends on the order of the threads.
 //
-// Reads 4 bytes a block, so bound by its own steps: some 100 instructions a key and
-// warp, and the barriers between digits. 256 of up to 8,192 blocks in 512 rows 18-19
-// us (72 % of issue slots used), in 8 rows 7 us; 32 of some 100 in 32 rows 3.6 us.
+// Reads 4 bytes a block, so bound by its own steps: the instructions for each key, and
+// the barriers between digits. 256 of up to 8,192 blocks in 512 rows 14.7 us, in 8 rows
+// 5.2 us; 32 of some 100 in 32 rows 2.9 us. On the way there 512 rows took 18.5 with every
+// lane finding its own keys' places (now one lane walks the chosen bits of 32 keys) and the
+// keys past a row's end taken along.
 struct SelectArgs {
   const float* scores;
   const int32_t* seq_lens;
@@ -492,13 +494,15 @@ __device__ __forceinline__ bool select_ends(const SelectArgs& g, int64_t row, in
 
 // The threshold among keys in registers, BITS bits at a time (the last digit has what is
 // left): a histogram in shared memory for each digit over the keys that share the digits
-// before it.
+// before it. Keys past the first `used` of each thread are 0, as are those that do not count:
+// below every score's, so that they change no digit that is found. m becomes the number of
+// keys at the threshold that are to be chosen, `whole` whether that is all of them.
 template <int THREADS, int R, int BITS>
-__device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], int m) {
+__device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], int used, int& m, bool& whole) {
   constexpr int BINS = 1 << BITS, PER = BINS > THREADS ? BINS / THREADS : 1, W = THREADS / 32;
   __shared__ int hist[BINS];
   __shared__ int sums[W];
-  __shared__ int found[2];  // the digit, and how many keys of its bin are still to be chosen
+  __shared__ int found[3];  // the digit, how many keys of its bin are still to be chosen, how many it has
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t limit = 0, mask = 0;
 #pragma unroll
@@ -510,7 +514,8 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < R; i++) {
-      const bool in = key[i] != 0 && (key[i] & mask) == limit;
+      if (i >= used) break;
+      const bool in = key[i] != 0 && ((key[i] ^ limit) & mask) == 0;
       const int bin = key[i] >> shift & ((1 << width) - 1);
       if (in) atomicAdd(&hist[bin], 1);
     }
@@ -535,6 +540,7 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
       if (above < m && m <= above + c) {
         found[0] = top - k;
         found[1] = m - above;
+        found[2] = c;
       }
       above += c;
     }
@@ -543,6 +549,7 @@ __device__ __forceinline__ uint32_t limit_by_digits(const uint32_t (&key)[R], in
     m = found[1];
     mask |= ((1u << width) - 1) << shift;
   }
+  whole = m == found[2];
   return limit;
 }
 
@@ -553,7 +560,6 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 4 : 1) select_reg_ke
   zl::ptx::griddep_enter();
   constexpr int W = THREADS / 32;
   __shared__ uint32_t before[R * W];
-  __shared__ int total_above;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x;
   const float* sc = g.scores + row * g.max_blocks;
@@ -566,19 +572,29 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 4 : 1) select_reg_ke
   }
   int lo, hi, m;
   if (select_ends<THREADS>(g, row, lo, hi, m)) return;
+  const int used = R < 8 ? R : (hi + THREADS - 1) / THREADS;  // keys of a thread that can be in the middle
 #pragma unroll
   for (int i = 0; i < R; i++) {
     const int j = i * THREADS + tid;
-    key[i] = j >= lo && j < hi ? zl::score_key(key[i]) : 0;  // 0 is no score's key (-inf has 0x007fffff)
+    if (i < used) key[i] = j >= lo && j < hi ? zl::score_key(key[i]) : 0;  // 0 is no score's key (-inf has 0x007fffff)
   }
-  const uint32_t limit = limit_by_digits<THREADS, R, BITS>(key, m);
-  // counts of each warp's keys above (low half) and at the limit (high half), by index order
+  bool whole;
+  const uint32_t limit = limit_by_digits<THREADS, R, BITS>(key, used, m, whole);
+  // each warp's keys above the limit and, where only some of those at it are chosen, those at
+  // it: bit l of lane i's words for key i of lane l
+  const uint32_t over = whole ? limit - 1 : limit;
+  uint32_t gts = 0, eqs = 0;
 #pragma unroll
   for (int i = 0; i < R; i++) {
-    const uint32_t gt = __popc(__ballot_sync(0xffffffffu, key[i] > limit));
-    const uint32_t eq = __popc(__ballot_sync(0xffffffffu, key[i] == limit));
-    if (lane == 0) before[i * W + warp] = gt | eq << 16;
+    if (i >= used) break;
+    const uint32_t gt = __ballot_sync(0xffffffffu, key[i] > over);
+    const uint32_t eq = whole ? 0 : __ballot_sync(0xffffffffu, key[i] == limit);
+    if (lane == i) {
+      gts = gt;
+      eqs = eq;
+    }
   }
+  if (lane < R) before[lane * W + warp] = __popc(gts) | __popc(eqs) << 16;  // counts, in index order
   __syncthreads();
   if (warp == 0) {  // exclusive sums of both halves; no total passes 31 * 1024
     constexpr int PER = (R * W + 31) / 32;
@@ -600,16 +616,23 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 4 : 1) select_reg_ke
       if (lane * PER + k < R * W) before[lane * PER + k] = at;
       at += mine[k];
     }
-    if (lane == 31) total_above = (int)(incl & 0xffff);
   }
   __syncthreads();
-  const int ties = m - total_above;
+  const int ties = whole ? 0 : m;
+  const uint32_t b = lane < R ? before[lane * W + warp] : 0;
+  int at = lo + (int)(b & 0xffff) + min((int)(b >> 16), ties);
+  const int take = min(max(ties - (int)(b >> 16), 0), __popc(eqs));  // of the equal keys, the first so many
+  while (__popc(eqs) > take) eqs &= ~(0x80000000u >> __clz(eqs));
+  if constexpr (R >= 8) {  // lane i writes its words' keys: few are chosen of many
+    for (uint32_t out_keys = gts | eqs; out_keys; out_keys &= out_keys - 1)
+      out[at++] = lane * THREADS + warp * 32 + __ffs(out_keys) - 1;
+  } else {
 #pragma unroll
-  for (int i = 0; i < R; i++) {
-    const uint32_t gts = __ballot_sync(0xffffffffu, key[i] > limit), eqs = __ballot_sync(0xffffffffu, key[i] == limit);
-    const uint32_t below = (1u << lane) - 1, b = before[i * W + warp];
-    const int gt = (int)(b & 0xffff) + __popc(gts & below), eq = (int)(b >> 16) + __popc(eqs & below);
-    if (key[i] > limit || (key[i] == limit && eq < ties)) out[lo + gt + min(eq, ties)] = i * THREADS + tid;
+    for (int i = 0; i < R; i++) {
+      const uint32_t chosen = __shfl_sync(0xffffffffu, gts | eqs, i);
+      const int from = __shfl_sync(0xffffffffu, at, i);
+      if (chosen >> lane & 1) out[from + __popc(chosen & ((1u << lane) - 1))] = i * THREADS + tid;
+    }
   }
 }
 
@@ -826,9 +849,11 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
   // Threads by the table's width, a few keys to each: with 256 threads and 32 keys instead of
   // 1,024 and 8, 8 rows of 8,192 blocks take 15.4 us, not 7.0. Digits of 8 bits need 256 bins to
   // clear and sum, of 11 bits one pass less: 1,600 rows of 650 blocks 10.4 and 21 us, 512 rows of
-  // 8,192 20.4 and 19.1. More rows than CTAs of 1,024 threads at once take half the threads (18.1).
+  // 8,192 15.6 and 15.1. More rows than CTAs of 1,024 threads at once take half the threads
+  // (18.1 us, not 19.1; 20.7 with 256). One key to a thread for narrow tables: 2.9 us, 3.2 with 4.
   const bool many = rows > 2 * ctx->num_sms;
-  if (max_blocks_per_seq <= 512) zl::launch_ahead(select_reg_kernel<128, 4, 8>, n, 128, 0, st, g);
+  if (max_blocks_per_seq <= 128) zl::launch_ahead(select_reg_kernel<128, 1, 8>, n, 128, 0, st, g);
+  else if (max_blocks_per_seq <= 512) zl::launch_ahead(select_reg_kernel<128, 4, 8>, n, 128, 0, st, g);
   else if (max_blocks_per_seq <= 1024) zl::launch_ahead(select_reg_kernel<256, 4, 8>, n, 256, 0, st, g);
   else if (max_blocks_per_seq <= 2048) zl::launch_ahead(select_reg_kernel<512, 4, 8>, n, 512, 0, st, g);
   else if (max_blocks_per_seq <= 8192 && many) zl::launch_ahead(select_reg_kernel<512, 16, 11>, n, 512, 0, st, g);
