@@ -113,7 +113,10 @@ template <int N>
 __device__ __forceinline__ bool table_columns(const StepArgs& g, int i, int c, int r, int had, int has, int fresh,
                                               Ids<N> id) {
   bool bad = false;
-  if (c + N > had) {  // past the old blocks: new ones, then nothing
+  if (c >= has) {
+#pragma unroll
+    for (int k = 0; k < N; k++) id.x[k] = -1;
+  } else if (c + N > had) {  // past the old blocks: new ones, then nothing
 #pragma unroll
     for (int k = 0; k < N; k++) {
       if (c + k < had) continue;
@@ -123,12 +126,18 @@ __device__ __forceinline__ bool table_columns(const StepArgs& g, int i, int c, i
       if (c + k < has) g.seq_blocks[(int64_t)r * g.max_blocks + c + k] = id.x[k];
     }
   }
+  // ids that are no block's become -1: seldom any but those past the end
+  bool other = false;
 #pragma unroll
-  for (int k = 0; k < N; k++)
-    if ((uint32_t)id.x[k] >= (uint32_t)g.num_blocks) {
-      id.x[k] = -1;
-      bad |= c + k < has;
-    }
+  for (int k = 0; k < N; k++) other |= (uint32_t)id.x[k] >= (uint32_t)g.num_blocks;
+  if (other && c < has) {
+#pragma unroll
+    for (int k = 0; k < N; k++)
+      if ((uint32_t)id.x[k] >= (uint32_t)g.num_blocks) {
+        id.x[k] = -1;
+        bad |= c + k < has;
+      }
+  }
   int32_t* to = g.block_tables + (int64_t)i * g.max_blocks + c;
   if constexpr (N == 4) *reinterpret_cast<int4*>(to) = make_int4(id.x[0], id.x[1], id.x[2], id.x[3]);
   else *to = id.x[0];
