@@ -18,9 +18,10 @@
 // Measured on one B200 (GPU time, replayed back to back): 64 decode rows with
 // tables of 257 blocks 3.7 us, bound by latency (two dependent reads, the sums,
 // one more read). 1,024 requests with tables of 8,192 blocks and 65,536 token
-// rows 17.2 us: 49.7 MB, 2.9 TB/s, of which some 5 us are every CTA's own sums.
-// On the way there: 4-byte entries 88 us, 16-byte ones 25, 32-bit divisions
-// 20, all of a stretch's loads before its first store and larger CTAs 17.
+// rows 14.8 us: 49.7 MB, 3.4 TB/s, of which 3.9 us are the launch and every CTA's
+// own sums. On the way there: 4-byte entries 88 us, 16-byte ones 25, 32-bit
+// divisions 20, all of a stretch's loads before its first store and larger CTAs 17.
+// Stretches shared out by warps instead of CTAs: 15.3; eight loads ahead: 15.5.
 #include "zl_internal.h"
 #include "zl_pages.h"
 #include "zl_ptx.cuh"
@@ -293,7 +294,7 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   const size_t smem = sizeof(int32_t) * (4 * (size_t)num_seqs + 1) + (rows ? 8 * (size_t)((num_rows + 31) / 32) : 0);
   const bool vec = max_blocks_per_seq % 4 == 0 && aligned16(seq_blocks) && aligned16(block_tables);
   // Two CTAs of 512 threads to an SM, or one of 1,024 that takes the sums over many requests once:
-  // 64 rows of 257 blocks 3.5 and 4.2 us, 1,024 rows 7.7 and 5.9, 4,000 rows 24.8 and 12.5.
+  // 64 rows of 257 blocks 3.5 and 4.2 us, 1,024 rows 7.7 and 5.9, 4,000 rows 24.8 and 12.0.
   const bool many = num_seqs > 512;
   const int kThreads = many ? 1024 : 512;
   const auto kernel = many ? (vec ? step_tables_kernel<4, 1024> : step_tables_kernel<1, 1024>)
