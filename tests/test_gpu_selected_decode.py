@@ -101,6 +101,18 @@ def test_selected(ctx, lens, H, Hkv, d, bs, top, modulo, bf16):
 
 
 @pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("B", [15, 16, 33, 34, 71, 72, 75, 149])
+def test_selected_lists_about_the_clusters_that_run_at_once(ctx, B, d, bf16):
+    """Lists of 1,024 tokens, so that all cluster sizes are open to the choice."""
+    rng = np.random.default_rng(B + d)
+    q, kp, vp, _, _ = decode_case(rng, B, [1] * B, 2, 1, d, 64, 150)
+    table = rng.integers(0, 150, (B, 16), dtype=np.int32)  # sequences that share blocks
+    lens = np.array([1024 - i % 3 * 500 for i in range(B)], np.int32)
+    check(ctx, q, kp, vp, table, lens, np.tile(np.arange(16, dtype=np.int32), (B, 1, 1)), bf16)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
 @pytest.mark.parametrize("d,bs", [(128, 16), (64, 8), (72, 5)])
 def test_selected_odd_lists(ctx, d, bs, bf16):
     """Any order, an index twice, an empty list, a list ended early, blocks past the length."""

@@ -113,6 +113,7 @@ zl_status zl_ctx_create(const zl_ctx_cfg* cfg, zl_ctx** out) {
                      dev, prop.major, prop.minor);
   }
   ctx->num_sms = prop.multiProcessorCount;
+  find_cluster_room(ctx);
   // status word at [0]; the persistent prefill's two work counters at [32], a
   // 128-byte line of their own
   e = cudaMalloc(&ctx->d_status, 64 * sizeof(int));

@@ -563,6 +563,34 @@ zl_status launch(zl_ctx* ctx, void (*kernel)(SelArgs, int), size_t smem, const S
 
 namespace zl {
 
+// A cluster's CTAs share a GPC, and the GPCs' SMs are no multiple of its size: with one CTA to
+// an SM 148 clusters of one, 74 of two, 33 of four, 15 of eight run at once. A size that cannot
+// be asked for is taken not to run.
+void find_cluster_room(zl_ctx* ctx) {
+  for (int two = 0; two < 2; two++) {
+    ctx->cluster_room[two][0] = ctx->num_sms << two;
+    void (*const kernel)(SelArgs, int) = two ? selected_mma_kernel<128, 3> : selected_mma_kernel<256, 3>;
+    const size_t smem = ring_bytes(two ? 256 : 512, 16, 3);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    for (int log = 1; log < 4; log++) {
+      cudaLaunchConfig_t cfg{};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1 << log;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3(1 << log);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = smem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+      ctx->cluster_room[two][log] = e == cudaSuccess ? clusters << log : 0;
+    }
+  }
+  cudaGetLastError();
+}
+
 zl_status launch_decode_selected_fast(zl_ctx* ctx, const void* q, const void* k_pool, const void* v_pool,
                                       const int32_t* block_tables, const int32_t* seq_lens,
                                       const int32_t* selected, void* out, int B, int H, int Hkv, int d, int bs,
@@ -584,10 +612,16 @@ zl_status launch_decode_selected_fast(zl_ctx* ctx, const void* q, const void* k_
   // CTAs per list: as many as one wave of the GPU has room for, while each warp has a tile or
   // two of its own. A CTA costs some 5 us beside its tokens: one sequence (8 lists of 128 blocks)
   // 28.5 / 17.8 / 11.8 / 8.9 us with 1 / 2 / 4 / 8 CTAs to a list, 64 sequences 88 / 103 / 119
-  // with 1 / 2 / 4; sizes that are no power of two and 16 gave nothing.
-  const int64_t tokens = (int64_t)max_selected * bs, room = (d <= 128 ? 2 : 1) * (int64_t)ctx->num_sms;
-  int cluster = 1;
-  while (cluster < kMaxCluster && 2 * jobs * cluster <= room && tokens >= cluster * 128) cluster *= 2;
+  // with 1 / 2 / 4; sizes that are no power of two and 16 gave nothing. One cluster more than
+  // run at once costs a second round: 34 lists 19.4 us with 8 CTAs to a list, 14.2 with 4; heads
+  // of 256, 16 lists 23.6 and 18.1.
+  const int64_t tokens = (int64_t)max_selected * bs;
+  const int* room = ctx->cluster_room[d <= 128];  // two CTAs to an SM, or one
+  int log_cluster = 0;
+  while (2 << log_cluster <= kMaxCluster && jobs << (log_cluster + 1) <= room[log_cluster + 1] &&
+         tokens >= 128 << log_cluster)
+    log_cluster++;
+  const int cluster = 1 << log_cluster;
   if (jobs * cluster > INT32_MAX) return ZL_ERR_UNSUPPORTED;
   // Heads of 65 to 128 elements: two CTAs of three ring slots or three of two to an SM, the
   // same bytes on their way but other rounds. A round that fills the SMs costs its bytes, the

@@ -22,6 +22,7 @@ struct zl_ctx {
   int device = 0;
   uint32_t flags = 0;             // ZL_CTX_* (zl_ctx_set_flags)
   int num_sms = 148;
+  int cluster_room[2][4] = {};    // CTAs of clusters of 1, 2, 4 and 8 that run at once, one CTA or two to an SM
   int* d_status = nullptr;        // device status word
   int* prefill_work = nullptr;    // [0] next work item, [1] CTAs finished: the persistent prefill's
                                   // counters (zero between launches; in the status allocation)
@@ -145,6 +146,8 @@ zl_status launch_decode_selected_fast(zl_ctx* ctx, const void* q, const void* k_
                                       const int32_t* selected, void* out, int B, int H, int Hkv, int d, int bs,
                                       int max_blocks, int64_t num_blocks, int max_selected, float scale,
                                       zl_gqa_map map, zl_dtype dtype, cudaStream_t st);
+// Fills ctx->cluster_room (selected_decode.cu); the device is current.
+void find_cluster_room(zl_ctx* ctx);
 // Both prefill launchers check cu_seqlens on the device against total_tokens
 // (ZL_DEV_OOB and the sequence skipped when it leaves [0, total_tokens]).
 zl_status launch_prefill_generic(zl_ctx* ctx, const void* q, const void* k, const void* v,
