@@ -134,7 +134,7 @@ __device__ __forceinline__ void merge(uint4& lo, uint4& hi, const uint4& a, cons
 // to a row (a power of two), CH chunks to a lane, ROWS = 32 / LPR * DEPTH rows at a time,
 // all of whose loads are in flight at once. A warp keeps to one head; the warps of the
 // heads of one block, whose keys lie side by side, are neighbours. HBM-bound: 16 prompts of
-// 256 to 8,192 tokens, 8 heads of 128 bf16, 27.9 us for 156 MB (5.6 TB/s); 64 of 2,048 to 4,096
+// 256 to 8,192 tokens, 8 heads of 128 bf16, 27.3 us for 156 MB (5.7 TB/s); 64 of 2,048 to 4,096
 // 72 us (6.2 TB/s). The work per block had to shrink for that: with a division and a search for
 // each block 34 us, and 37 with copies ahead through shared memory on top.
 template <typename T, int LPR, int CH>
@@ -258,10 +258,10 @@ scores_elem_kernel(PagedArgs g, const T* __restrict__ q, const T* __restrict__ b
 // Each warp keeps a ring of ST tiles (16 blocks' bounds) in shared memory, filled by
 // asynchronous copies, and the block ids of one tile more. Chunk ch of row r lies at
 // ch ^ swz(r), so that the two rows that a quarter warp reads do not meet in a bank.
-// HBM-bound: 8 sequences of 131,072 tokens, 64 query and 8 key heads, 44.2 us for 271 MB (6.1
+// HBM-bound: 8 sequences of 131,072 tokens, 64 query and 8 key heads, 45.8 us for 271 MB (5.9
 // TB/s). Loads straight into registers took 74 us, the ring 60, 32-bit row numbers and whole
 // rounds of CTAs 45. CTAs of one warp start and end on their own: 64 sequences of 2,048 to 4,096
-// tokens 11.6 us against 13.4 with four warps to a CTA.
+// tokens 11.6 us against 13.4 with four warps to a CTA, of 512 to 4,096 9.8.
 constexpr int kScoreWarps = 1, kScoreCtas = 12;
 template <int DT, int ST>
 __global__ void __launch_bounds__(kScoreWarps * 32)
