@@ -185,6 +185,27 @@ def test_special_values(ctx):
     assert torch.isfinite(out[1]).all(-1).sum() == 5
 
 
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("T,d", [(3, 128), (3000, 128), (3, 33)])
+def test_squares_past_the_range(ctx, T, d, bf16):
+    """A row whose squares add up to infinity is divided by it, in every kernel: 0, NaN where it is infinite itself.
+    Without eps a row of zeros is 0 / 0."""
+    import torch
+    import zealot_b200 as zb
+    _, q, k, v, w = make(T, 2, 1, d, bf16)
+    q, k = q.clone(), k.clone()
+    q[0, 0, 5] = 1e30
+    q[1, 1, 7] = -float("inf")
+    k[2, 0] = 0
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    zb.CudaAttention(ctx).qk_norm_rope(q, k, v, None, None, q_out=qo, k_out=ko, q_weight=w[0], k_weight=w[1], eps=0.0)
+    ctx.check_status()
+    assert torch.all(qo[0, 0] == 0)
+    assert torch.isnan(qo[1, 1, 7]) and torch.all(qo[1, 1, :7] == 0) and torch.all(qo[1, 1, 8:] == 0)
+    assert torch.all(torch.isnan(ko[2]))
+    assert torch.all(torch.isfinite(ko[:2])) and torch.all(torch.isfinite(qo[0])) and torch.all(torch.isfinite(qo[2:]))
+
+
 def test_refusals(ctx):
     import torch
     import zealot_b200 as zb

@@ -292,7 +292,8 @@ __device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>&
   if (!r.use) return;
   if (r.norm) {
     const float y = ss * g.inv_d + g.eps, q = rsqrtf(y);
-    const float inv = q * fmaf(-0.5f * y * q, q, 1.5f);  // a Newton step: right to fp32's last place or so
+    const float step = q * fmaf(-0.5f * y * q, q, 1.5f);  // a Newton step: right to fp32's last place or so
+    const float inv = step == step ? step : q;             // a sum past fp32's range, or 0 without eps: 1 / sqrt as it is
     const uint64_t inv2 = px::f2_pack(inv, inv);
     const ulonglong2* w = reinterpret_cast<const ulonglong2*>(&sh.weights[r.isk][0][ln.u]);
 #pragma unroll
