@@ -53,6 +53,37 @@ def test_head_rows():
         calls.head_rows(-1, f, 5, 4, "q", 6)
 
 
+def test_tensors_of_other_kinds():
+    """Parameters, subclasses, views of parts, empty and single elements; types and places that no operator takes."""
+    import torch
+    from zealot_b200 import calls
+    f = torch.float32
+
+    class Mine(torch.Tensor):
+        pass
+
+    t = torch.zeros((4, 6))
+    for x in (torch.nn.Parameter(t), t.requires_grad_(), t.as_subclass(Mine), t.detach()):
+        assert calls.addresses(-1, x, f, 24) == (x.data_ptr(),)
+        assert calls.addresses(-1, x, torch.bfloat16, 24) == 0
+    part = t.detach()[1:3]
+    assert calls.addresses(-1, part, f, 12) == (t.data_ptr() + 24,)  # an offset into its memory
+    assert calls.addresses(-1, t.detach()[:, :1], f, 4) == 0
+    assert calls.addresses(-1, t.detach()[:1, None, :], f, 6) == (t.data_ptr(),)  # strides of single elements do not count
+    assert calls.addresses(-1, torch.zeros((0, 7)).T, f, 0) == (0,)
+    assert calls.addresses(-1, torch.zeros(()), f, 1) != 0
+    for kind in (torch.int32, torch.int64, torch.float32, torch.float64, torch.bfloat16, torch.float16, torch.bool):
+        x = torch.zeros(3, dtype=kind)
+        for other in (torch.int32, torch.int64, torch.float32, torch.float64, torch.bfloat16, torch.float16, torch.bool):
+            assert calls.addresses(-1, x, other, 3) == ((x.data_ptr(),) if kind is other else 0)
+    assert calls.addresses(-1, torch.zeros([1] * 8), f, 1) != 0
+    with pytest.raises((TypeError, RuntimeError)):
+        calls.addresses(-1, torch.zeros([1] * 9), f, 1)  # more dimensions than any argument has
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        calls.addresses(-1, torch.zeros(3).to_sparse(), f, 3)
+    assert calls.addresses(0, torch.zeros(3, device="meta"), f, 3) == 0
+
+
 @pytest.mark.parametrize("name", list(CALLS))
 def test_calls_pass_what_ctypes_passes(name):
     """Each argument changed in turn to one that the C function refuses in words: the same status and words."""

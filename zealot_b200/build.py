@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import subprocess
 import sys
@@ -84,8 +85,9 @@ def _build_calls(force: bool) -> None:
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "zealot_attn.h")))
     if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest:
         return
-    cmd = ["gcc", "-O2", "-Wall", "-shared", "-fPIC", f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", src,
-           "-o", CALLS, f"-L{HERE}", "-l:libzealot_attn.so", "-Wl,-rpath,$ORIGIN"]
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]  # its tensor exchange header
+    cmd = ["gcc", "-O2", "-Wall", "-shared", "-fPIC", f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
+           f"-I{os.path.join(torch, 'include')}", src, "-o", CALLS, f"-L{HERE}", "-l:libzealot_attn.so", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"gcc failed for {src}:\n{r.stdout}\n{r.stderr}")

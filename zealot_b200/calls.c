@@ -2,47 +2,135 @@
  * pass over a call's tensors and one typed call of the C ABI.
  *
  * ctypes and five method calls a tensor from bytecode cost 5-9 us where the
- * launch behind them costs 3 (a step makes several such calls for every layer);
- * this module takes them in 2-4. It computes nothing and keeps nothing: what is
- * checked and what is passed stands in attention.py.
+ * launch behind them costs 3 (a step makes several such calls for every layer).
+ * A tensor is read through the C exchange table that torch.Tensor offers
+ * (__dlpack_c_exchange_api__), in one call without a Python object made; what
+ * that does not take (a tensor that is only like one, a conjugate) through its
+ * methods. This module computes nothing and keeps nothing: what is checked and
+ * what is passed stands in attention.py.
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/dlpack.h>
+
 #include "zealot_attn.h"
 
-static PyObject *s_dtype, *s_numel, *s_get_device, *s_is_contiguous, *s_data_ptr, *s_shape, *s_stride;
+static PyObject *s_dtype, *s_get_device, *s_data_ptr, *s_shape, *s_stride;
+
+/* torch, from the first call that has a tensor on */
+static struct {
+  const DLPackExchangeAPI* exchange;
+  PyObject* tensor;
+  struct {
+    PyObject* dtype;
+    uint8_t code, bits;
+  } kinds[5];
+} torch;
+
+static int find_torch(void) {
+  static const struct {
+    const char* name;
+    uint8_t code, bits;
+  } kinds[5] = {{"int32", kDLInt, 32}, {"int64", kDLInt, 64}, {"float32", kDLFloat, 32}, {"float64", kDLFloat, 64}, {"bfloat16", kDLBfloat, 16}};
+  PyObject *m = PyImport_ImportModule("torch"), *tensor = m ? PyObject_GetAttrString(m, "Tensor") : NULL;
+  PyObject* table = tensor ? PyObject_GetAttrString(tensor, "__dlpack_c_exchange_api__") : NULL;
+  const DLPackExchangeAPI* exchange = table ? PyCapsule_GetPointer(table, "dlpack_exchange_api") : NULL;
+  int ok = exchange != NULL;
+  for (int i = 0; i < 5 && ok; i++) {
+    torch.kinds[i].code = kinds[i].code;
+    torch.kinds[i].bits = kinds[i].bits;
+    ok = (torch.kinds[i].dtype = PyObject_GetAttrString(m, kinds[i].name)) != NULL;
+  }
+  if (ok && exchange->header.version.major != DLPACK_MAJOR_VERSION) {
+    PyErr_SetString(PyExc_ImportError, "torch's tensor exchange has another major version: build zealot_b200 again");
+    ok = 0;
+  }
+  if (ok) {
+    torch.tensor = Py_NewRef(tensor);
+    torch.exchange = exchange; /* last: it says that the rest is there */
+  }
+  Py_XDECREF(table);
+  Py_XDECREF(tensor);
+  Py_XDECREF(m);
+  return ok;
+}
 
 static PyObject* method(PyObject* o, PyObject* name) {
   PyObject* args[1] = {o};
   return PyObject_VectorcallMethod(name, args, 1 | PY_VECTORCALL_ARGUMENTS_OFFSET, NULL);
 }
 
-/* o.name() as a whole number; -1 with an exception set on failure. */
-static long long number(PyObject* o, PyObject* name) {
-  PyObject* r = method(o, name);
-  if (!r) return -1;
-  const long long v = PyLong_AsLongLong(r);
-  Py_DECREF(r);
-  return v;
+#define MAX_DIMS 8
+/* What the checks ask of a tensor. */
+typedef struct {
+  int is_dtype, dims;
+  long long device; /* -1: the host */
+  int64_t shape[MAX_DIMS], stride[MAX_DIMS];
+  unsigned long long address;
+} View;
+
+/* 0: filled, with is_dtype whether `dtype` is the tensor's; -1: exception. */
+static int look_slowly(PyObject* t, PyObject* dtype, View* v) {
+  PyObject *kind = PyObject_GetAttr(t, s_dtype), *shape = NULL, *stride = NULL, *device = NULL, *address = NULL;
+  int ok = kind && (shape = PyObject_GetAttr(t, s_shape)) && (stride = method(t, s_stride)) &&
+           (device = method(t, s_get_device)) && (address = method(t, s_data_ptr));
+  if (ok && !(PyTuple_Check(shape) && PyTuple_Check(stride) && PyTuple_GET_SIZE(shape) <= MAX_DIMS &&
+              PyTuple_GET_SIZE(shape) == PyTuple_GET_SIZE(stride))) {
+    PyErr_Format(PyExc_TypeError, "no tensor of up to %d dimensions", MAX_DIMS);
+    ok = 0;
+  }
+  if (ok) {
+    v->is_dtype = kind == dtype;
+    v->dims = (int)PyTuple_GET_SIZE(shape);
+    for (int i = 0; i < v->dims; i++) {
+      v->shape[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+      v->stride[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(stride, i));
+    }
+    v->device = PyLong_AsLongLong(device);
+    v->address = PyLong_AsUnsignedLongLong(address);
+    ok = !PyErr_Occurred();
+  }
+  Py_XDECREF(kind);
+  Py_XDECREF(shape);
+  Py_XDECREF(stride);
+  Py_XDECREF(device);
+  Py_XDECREF(address);
+  return ok ? 0 : -1;
 }
 
-/* 1: a contiguous tensor of `dtype` with n elements on the device, 0: not, -1: exception. */
-static int fits(PyObject* t, PyObject* dtype, long long n, long long device) {
-  PyObject* d = PyObject_GetAttr(t, s_dtype);
-  if (!d) return -1;
-  Py_DECREF(d);
-  if (d != dtype) return 0;
-  const long long have = number(t, s_numel);
-  if (have == -1 && PyErr_Occurred()) return -1;
-  const long long on = number(t, s_get_device);
-  if (on == -1 && PyErr_Occurred()) return -1;
-  if (have != n || on != device) return 0;
-  PyObject* c = method(t, s_is_contiguous);
-  if (!c) return -1;
-  const int whole = PyObject_IsTrue(c);
-  Py_DECREF(c);
-  return whole;
+static int look(PyObject* t, PyObject* dtype, View* v) {
+  if (!torch.exchange && !find_torch()) return -1;
+  int kind = 0;
+  while (kind < 5 && torch.kinds[kind].dtype != dtype) kind++;
+  DLTensor d;
+  if (kind == 5 || !PyObject_TypeCheck(t, (PyTypeObject*)torch.tensor)) return look_slowly(t, dtype, v);
+  if (torch.exchange->dltensor_from_py_object_no_sync(t, &d) != 0) {
+    PyErr_Clear();
+    return look_slowly(t, dtype, v);
+  }
+  if (d.ndim > MAX_DIMS || !d.strides || (d.device.device_type != kDLCPU && d.device.device_type != kDLCUDA))
+    return look_slowly(t, dtype, v);
+  v->is_dtype = d.dtype.code == torch.kinds[kind].code && d.dtype.bits == torch.kinds[kind].bits && d.dtype.lanes == 1;
+  v->dims = d.ndim;
+  v->device = d.device.device_type == kDLCUDA ? d.device.device_id : -1;
+  for (int i = 0; i < d.ndim; i++) {
+    v->shape[i] = d.shape[i];
+    v->stride[i] = d.strides[i];
+  }
+  v->address = (unsigned long long)((uintptr_t)d.data + d.byte_offset);
+  return 0;
+}
+
+/* Whether the view is of n elements that lie in order. */
+static int in_order(const View* v, long long n) {
+  unsigned long long have = 1;
+  int whole = 1;
+  for (int i = v->dims - 1; i >= 0; i--) {
+    whole &= v->shape[i] == 1 || (unsigned long long)v->stride[i] == have;
+    have *= (unsigned long long)v->shape[i];
+  }
+  return n >= 0 && have == (unsigned long long)n && (whole || n == 0);
 }
 
 /* addresses(device, tensor, dtype, elements, tensor, dtype, elements, ...) -> the tensors'
@@ -58,18 +146,18 @@ static PyObject* addresses(PyObject* self, PyObject* const* args, Py_ssize_t nar
   PyObject* out = PyTuple_New(count);
   if (!out) return NULL;
   for (Py_ssize_t i = 0; i < count; i++) {
-    PyObject *t = args[1 + 3 * i], *a;
-    if (t == Py_None) {
-      a = PyLong_FromLong(0);
-    } else {
+    unsigned long long address = 0;
+    if (args[1 + 3 * i] != Py_None) {
+      View v;
       const long long n = PyLong_AsLongLong(args[3 + 3 * i]);
-      const int ok = n == -1 && PyErr_Occurred() ? -1 : fits(t, args[2 + 3 * i], n, device);
-      if (ok != 1) {
+      const int bad = (n == -1 && PyErr_Occurred()) || look(args[1 + 3 * i], args[2 + 3 * i], &v);
+      if (bad || !v.is_dtype || v.device != device || !in_order(&v, n)) {
         Py_DECREF(out);
-        return ok == 0 ? PyLong_FromSsize_t(i) : NULL;
+        return bad ? NULL : PyLong_FromSsize_t(i);
       }
-      a = method(t, s_data_ptr);
+      address = n ? v.address : 0;
     }
+    PyObject* a = PyLong_FromUnsignedLongLong(address);
     if (!a) {
       Py_DECREF(out);
       return NULL;
@@ -78,9 +166,6 @@ static PyObject* addresses(PyObject* self, PyObject* const* args, Py_ssize_t nar
   }
   return out;
 }
-
-/* item i of a tuple of whole numbers */
-static long long item(PyObject* t, Py_ssize_t i) { return PyLong_AsLongLong(PyTuple_GET_ITEM(t, i)); }
 
 /* head_rows(device, dtype, T, d, tensor, heads, tensor, heads, ...) -> (address, token stride, ...)
  * of tensors [T][heads][d] whose heads lie side by side, or the number of the first that is none. */
@@ -95,23 +180,20 @@ static PyObject* head_rows(PyObject* self, PyObject* const* args, Py_ssize_t nar
   PyObject* out = PyTuple_New(2 * count);
   if (!out) return NULL;
   for (Py_ssize_t i = 0; i < count; i++) {
-    PyObject *t = args[4 + 2 * i], *kind = NULL, *shape = NULL, *stride = NULL, *a = NULL, *step = NULL;
+    View v;
     const long long heads = PyLong_AsLongLong(args[5 + 2 * i]);
-    int ok = !PyErr_Occurred() && (kind = PyObject_GetAttr(t, s_dtype)) && (shape = PyObject_GetAttr(t, s_shape)) &&
-             (stride = method(t, s_stride));
-    if (ok) {
-      ok = kind == args[1] && PyTuple_Check(shape) && PyTuple_Check(stride) && PyTuple_GET_SIZE(shape) == 3 &&
-           PyTuple_GET_SIZE(stride) == 3 && item(shape, 0) == T && item(shape, 1) == heads && item(shape, 2) == d &&
-           (item(stride, 2) == 1 || d == 1) && (item(stride, 1) == d || heads == 1) && number(t, s_get_device) == device;
-      if (ok && (a = method(t, s_data_ptr))) step = Py_NewRef(PyTuple_GET_ITEM(stride, 0));
-    }
-    Py_XDECREF(kind);
-    Py_XDECREF(shape);
-    Py_XDECREF(stride);
-    if (!step) {
-      Py_XDECREF(a);
+    const int bad = (heads == -1 && PyErr_Occurred()) || look(args[4 + 2 * i], args[1], &v);
+    if (bad || !v.is_dtype || v.device != device || v.dims != 3 || v.shape[0] != T || v.shape[1] != heads ||
+        v.shape[2] != d || (v.stride[2] != 1 && d != 1) || (v.stride[1] != d && heads != 1)) {
       Py_DECREF(out);
-      return PyErr_Occurred() ? NULL : PyLong_FromSsize_t(i);
+      return bad ? NULL : PyLong_FromSsize_t(i);
+    }
+    PyObject *a = PyLong_FromUnsignedLongLong(T && heads && d ? v.address : 0), *step = PyLong_FromLongLong(v.stride[0]);
+    if (!a || !step) {
+      Py_XDECREF(a);
+      Py_XDECREF(step);
+      Py_DECREF(out);
+      return NULL;
     }
     PyTuple_SET_ITEM(out, 2 * i, a);
     PyTuple_SET_ITEM(out, 2 * i + 1, step);
@@ -200,12 +282,10 @@ static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "calls", "Call path o
 
 PyMODINIT_FUNC PyInit_calls(void) {
   s_dtype = PyUnicode_InternFromString("dtype");
-  s_numel = PyUnicode_InternFromString("numel");
   s_get_device = PyUnicode_InternFromString("get_device");
-  s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
   s_data_ptr = PyUnicode_InternFromString("data_ptr");
   s_shape = PyUnicode_InternFromString("shape");
   s_stride = PyUnicode_InternFromString("stride");
-  if (!s_dtype || !s_numel || !s_get_device || !s_is_contiguous || !s_data_ptr || !s_shape || !s_stride) return NULL;
+  if (!s_dtype || !s_get_device || !s_data_ptr || !s_shape || !s_stride) return NULL;
   return PyModule_Create(&module);
 }
