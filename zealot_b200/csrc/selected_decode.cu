@@ -587,8 +587,8 @@ void find_cluster_room(zl_ctx* ctx) {
       if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
       ctx->cluster_room[two][log] = e == cudaSuccess ? clusters << log : 0;
     }
+    if (e != cudaSuccess) cudaGetLastError();  // answered: no later call reports it
   }
-  cudaGetLastError();
 }
 
 zl_status launch_decode_selected_fast(zl_ctx* ctx, const void* q, const void* k_pool, const void* v_pool,
