@@ -710,9 +710,13 @@ void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* to
                        cudaStream_t st) {
   const int chunks = g.d * (int)sizeof(T) / 16;
   // CTAs for each sequence: with tok_begin, which is a step's few tokens or a chunk of a
-  // prompt, some 4 to an SM in all; for whole prompts of any lengths some kBoundsWaves.
+  // prompt, some 4 to an SM in all (16 chunks of 512 tokens 4.1 us, 5.8 with one), or one where
+  // there are many sequences, which are seldom chunks (the step's tokens and scores of 64
+  // sequences of 512 tokens 6.3 us, 6.8 with 4 to an SM, of 256 15.3 and 16.7; 64 chunks of 512
+  // tokens 18.9 and 18.3); for whole prompts of any lengths some kBoundsWaves.
   int64_t x = ((int64_t)g.max_blocks * g.Hkv + 7) / 8;
-  const int64_t few = ((tok_begin ? 4 : kBoundsWaves) * (int64_t)num_sms + g.B - 1) / g.B, least = (g.Hkv + 7) / 8;
+  const int an_sm = !tok_begin ? kBoundsWaves : g.B >= num_sms / 4 ? 1 : 4;
+  const int64_t few = (an_sm * (int64_t)num_sms + g.B - 1) / g.B, least = (g.Hkv + 7) / 8;
   x = x > few ? few : x;
   x = x < least ? least : x;
   const dim3 grid((unsigned)x, (unsigned)(g.B < 65535 ? g.B : 65535));
