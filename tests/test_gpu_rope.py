@@ -224,3 +224,25 @@ def test_refusals(ctx):
                  (q, k, v, pos, torch.zeros(33, dtype=torch.float64, device="cuda"))):
         with pytest.raises(zb.InvalidArgument):
             attn.qk_norm_rope(*args, q_out=o)
+
+
+def c_call(ctx, **args):
+    """zl_qk_norm_rope by its C signature; what is not named is NULL or 0. Tensors give their addresses."""
+    order = ("q k v q_stride k_stride v_stride q_weight k_weight eps positions inv_freq rotary_dim interleaved q_out k_out "
+             "v_out k_pool v_pool slot_mapping block_size num_blocks num_tokens num_heads num_kv_heads head_dim dtype stream").split()
+    assert not set(args) - set(order)
+    value = lambda x: x.data_ptr() if hasattr(x, "data_ptr") else x
+    return ctx.lib.zl_qk_norm_rope(ctx.handle, *(value(args.get(n, 0.0 if n == "eps" else 0)) for n in order))
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("T,d", [(3, 64), (2000, 64), (3, 33)])
+def test_values_alone_need_no_positions(ctx, T, d, bf16):
+    """A model's rotary size with only values to move, in each kernel: no angle is needed, so no position is read."""
+    import torch
+    _, _, _, v, _ = make(T, 2, 3, d, bf16)
+    out = torch.empty((T, 3, d), dtype=v.dtype, device="cuda")
+    assert c_call(ctx, v=v, v_stride=v.stride(0), rotary_dim=d // 2 * 2, v_out=out, num_tokens=T, num_heads=2, num_kv_heads=3,
+                  head_dim=d, q_stride=2 * d, dtype=int(bf16), stream=torch.cuda.current_stream().cuda_stream) == 0
+    ctx.check_status()
+    assert torch.equal(out, v)

@@ -488,6 +488,7 @@ extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, 
     return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: in place only on packed rows");
   DeviceScope dev(ctx);
   if (dev.status != ZL_OK) return dev.status;
+  if (!q_out && !need_k) rotary_dim = 0;  // values alone: there are no angles, and positions may be missing
   RopeArgs g{q, k, v, q_stride, k_stride, v_stride, q_weight, k_weight, eps, positions, inv_freq, rotary_dim,
              interleaved, q_out, k_out, v_out, k_pool, v_pool, k_pool ? slot_mapping : nullptr, block_size,
              num_blocks, num_tokens, num_heads, num_kv_heads, head_dim, 1.f / head_dim, ctx->d_status};
