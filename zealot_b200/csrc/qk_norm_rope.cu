@@ -441,8 +441,10 @@ zl_status launch_rope_vec(const RopeArgs& g, int num_sms, cudaStream_t st) {
   }
   const int hpb = (heads + blocks - 1) / blocks, slices = NG / hpb < per ? NG / hpb : (int)per;
   const size_t smem = (size_t)kAhead * 256 * 2 * E * sizeof(T) + per * (g.rot / 2) * sizeof(float2);
+  // the limit is one of the function on the device, for all threads' calls: always the same, the largest
+  constexpr int most = kAhead * 256 * 2 * E * (int)sizeof(T) + kTokens * (kMaxDim / 2) * (int)sizeof(float2);
   const auto kernel = rope_tokens_kernel<T, LG, E>;
-  ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
   launch_ahead(kernel, (unsigned)((g.tokens + per - 1) / per), 256, smem, st, g, (int)per, hpb, slices);
   return ZL_OK;
 }

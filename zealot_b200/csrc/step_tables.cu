@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kMaxSeqs = 8192;      // requests of one step: 16 bytes of shared memory each
 constexpr int kMaxRows = 1 << 18;   // rows of the persistent table: 2 bits of shared memory each
+constexpr int kMostShared = 4 * (4 * kMaxSeqs + 1) + 2 * kMaxRows / 8;
 
 struct StepArgs {
   int32_t* seq_blocks;
@@ -300,7 +301,8 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   const auto kernel = many ? (vec ? step_tables_kernel<4, 1024> : step_tables_kernel<1, 1024>)
                            : (vec ? step_tables_kernel<4, 512> : step_tables_kernel<1, 512>);
   if (smem > 32 * 1024)  // with the static part it may pass 48 KB
-    ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // one limit of the function on the device, for all threads' calls: always the same, the largest
+    ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
   // Threads to a table row: one step of each while all rows then fit the GPU at once (the
   // shortest way for a small step: 64 rows of 257 blocks 3.7 us, 4.0 with kDepth steps of a
   // quarter of the threads), kDepth steps otherwise (1,024 rows of 8,192: 17.6 us, 20 with one).
