@@ -144,3 +144,42 @@ def test_decode_loop(ctx, graph):
         assert np.all(np.abs(loop.o.double().cpu().numpy() - want) <= tol)
     if graph:
         del captured
+
+
+@pytest.mark.parametrize("first_ahead", [False, True])
+def test_decode_that_reads_ahead_behind_step_tables(first_ahead):
+    """Step tables, a decode on other tables, then a decode of the new tables that reads them ahead of the kernel
+    before it: they were written before that kernel's place in the stream, so it finds the new ones."""
+    import torch
+    import zealot_b200 as zb
+    from zealot_b200.context import CTX_INPUTS_AHEAD
+    n, width, nb, bs = 1024, 64, 4096, 16
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    k_pool, v_pool, q = rand(nb, 1, bs, 128), rand(nb, 1, bs, 128), rand(n, 4, 128)
+    seq_blocks = torch.randint(0, nb, (n, width), generator=g, device="cuda", dtype=torch.int32)
+    other, other_lens = torch.randint(0, nb, (4, width), generator=g, device="cuda", dtype=torch.int32), i32(4) + 40
+    tables, cu, lens, last, ones = i32(n, width), i32(n + 1), i32(n), i32(n), i32(n) + 1
+    pos, slots, o, o4, want = i32(n), i32(n).long(), torch.empty_like(q), rand(4, 4, 128), torch.empty_like(q)
+    new = torch.randint(0, nb, (n,), generator=g, device="cuda", dtype=torch.int32)
+    with zb.GpuContext(0) as own:
+        attn = zb.CudaAttention(own)
+        decode = lambda q, t, l, out: attn.paged_forward(q, k_pool, v_pool, t, l, out, len(l), 4, 1, 128, bs, width, num_blocks=nb)
+        decode(q, tables, lens, want)  # (the first call sets the workspace up)
+        for step in range(30):
+            context = torch.randint(1, 400, (n,), generator=g, device="cuda", dtype=torch.int32)
+            context[::3] = 0
+            tables.zero_(), lens.fill_(1 + step % 2 * 200)
+            torch.cuda.synchronize()
+            attn.step_tables(seq_blocks, None, context, ones, new, tables, cu, lens, pos, slots, last, bs, nb)
+            own.set_flags(CTX_INPUTS_AHEAD if first_ahead else 0)
+            decode(q[:4], other, other_lens, o4)
+            own.set_flags(CTX_INPUTS_AHEAD)
+            decode(q, tables, lens, o)
+            own.check_status()
+            own.set_flags(0)
+            decode(q, tables, lens, want)
+            torch.cuda.synchronize()
+            assert torch.equal(lens, context + 1) and torch.equal(o, want)
+        own.check_status()

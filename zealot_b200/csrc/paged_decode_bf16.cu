@@ -351,15 +351,20 @@ paged_decode_bf16_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap
   const int lane = tid & 31;
   const int B = a.B, Hkv = a.Hkv;
 
-  // Programmatic dependent launch: the next kernel may be scheduled now; this
-  // one waits for its predecessor before the first read of anything that
-  // kernel could write (at once, unless the caller declared the tables and
-  // lengths ready ahead: then after the prologue and the first table reads).
-  griddep_launch_dependents();
-  if (!a.inputs_ahead) griddep_wait();
+  // Programmatic dependent launch: this kernel waits for its predecessor before
+  // the first read of anything that kernel could write (at once, unless the
+  // caller declared the tables and lengths ready ahead: then after the prologue
+  // and the first table reads), and lets the next kernel be scheduled only after
+  // that wait. A decode that reads ahead may follow: what it reads was written
+  // before this kernel's place in the stream, but perhaps by a predecessor that
+  // let this kernel start ahead of its end (zl_step_tables).
+  if (!a.inputs_ahead) griddep_enter();
   // An earlier launch timed out and was not cleared: return, the whole CTA
   // alike (its warps may meet at CTA barriers further on).
-  if (__syncthreads_or(aborted(a.status))) return;
+  if (__syncthreads_or(aborted(a.status))) {
+    griddep_wait();  // this grid does not end before its predecessor
+    return;
+  }
   if (tid == 0) {
     prefetch_tmap(&tmK);
     prefetch_tmap(&tmV);
@@ -640,7 +645,7 @@ paged_decode_bf16_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap
     fetch_chunk(0);
     build_chunk(0);
   }
-  griddep_wait();  // K/V, q and the outputs belong to the stream order from here on
+  griddep_enter();  // K/V, q and the outputs belong to the stream order from here on
   {
     const int pre = min(nwork, STAGES);
     for (int k = 0; k < pre; k++) produce(k);
