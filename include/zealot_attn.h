@@ -263,14 +263,19 @@ zl_status zl_merge_partials(zl_ctx* ctx, const float* m, const float* l, const f
  * zl_select_blocks and zl_paged_decode_selected. No reference counterpart.
  * Tables, lengths, pools and the head mapping are those of zl_paged_decode; a
  * negative table entry is a block that is not there (it does not end the
- * sequence). Several tokens of one sequence are served as several rows with
- * the same table and their own lengths. */
+ * sequence). Several tokens of one sequence are served as several rows of
+ * zl_block_scores, zl_select_blocks and zl_paged_decode_selected with the same
+ * table and their own lengths, after one row of zl_block_bounds for all of them
+ * (the length after the last, tok_begin before the first). */
 
-/* Bounds of the keys of every block that holds a token in [tok_begin[b],
- * seq_lens[b]) (tok_begin NULL: from 0): bounds [num_blocks][Hkv][2][d] in
+/* Bounds of the keys of every block from the one of token tok_begin[b] (NULL:
+ * 0) to the one of the last below seq_lens[b]: bounds [num_blocks][Hkv][2][d] in
  * `dtype`, the elementwise minimum and maximum over the block's tokens below
- * seq_lens[b]. After a decode step tok_begin is the length before it. A block
- * shared by sequences is shared whole. NaN keys give NaN bounds. */
+ * seq_lens[b]. After a decode step tok_begin is the length before it. Rows of
+ * one call that bound the same block agree on how many of its tokens there are:
+ * a sequence is listed once, and a block that sequences share is full or part
+ * full in all of them alike (otherwise the row that happens to store last
+ * leaves its bounds). NaN keys give NaN bounds. */
 zl_status zl_block_bounds(zl_ctx* ctx, const void* k_pool /*device*/, const int32_t* block_tables /*device*/,
                           const int32_t* tok_begin /*device*/, const int32_t* seq_lens /*device*/,
                           void* bounds /*device*/, int num_seqs, int num_kv_heads, int head_dim,

@@ -183,3 +183,45 @@ def test_decode_that_reads_ahead_behind_step_tables(first_ahead):
             torch.cuda.synchronize()
             assert torch.equal(lens, context + 1) and torch.equal(o, want)
         own.check_status()
+
+
+def test_several_tokens_of_a_sequence(ctx):
+    """Three new tokens of each of two sequences, which end in one block and in two: bounds once for each sequence, then
+    a row for each token. A shorter row's bounds cover the later tokens too and still bound its own."""
+    import torch
+    import zealot_b200 as zb
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)
+    dev = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    before, after = [130, 94], [133, 97]
+    k_pool, v_pool, q = rand(NB, HKV, BS, D), rand(NB, HKV, BS, D), rand(6, H, D)
+    table = torch.randperm(NB, generator=g, device="cuda")[:2 * MB].reshape(2, MB).to(torch.int32)
+    attn = zb.CudaAttention(ctx)
+    bounds = torch.zeros((NB, HKV, 2, D), dtype=torch.bfloat16, device="cuda")
+    attn.block_bounds(k_pool, table, dev(before), bounds)
+    attn.block_bounds(k_pool, table, dev(after), bounds, tok_begin=dev(before))
+    t = table.cpu().numpy()
+    want = blocks.plain_bounds(k_pool, t, after, None, torch.zeros_like(bounds), BS)
+    for b in range(2):
+        ids = t[b, :-(-after[b] // BS)]
+        assert np.array_equal(bounds.float().cpu().numpy()[ids], want[ids])
+    lens = [131, 132, 133, 95, 96, 97]
+    rows = table.repeat_interleave(3, 0)
+    scores, sel = torch.zeros((6, HKV, MB), device="cuda"), torch.zeros((6, HKV, TOP), dtype=torch.int32, device="cuda")
+    o = torch.empty_like(q)
+    attn.block_scores(q, bounds, rows, dev(lens), scores, BS)
+    attn.select_blocks(scores, dev(lens), sel, BS)
+    attn.paged_forward_selected(q, k_pool, v_pool, rows, dev(lens), sel, o)
+    ctx.check_status()
+    t, qh, kh, got = rows.cpu().numpy(), q.double().cpu().numpy(), k_pool.double().cpu().numpy(), scores.double().cpu().numpy()
+    _, tol = blocks.plain_scores(q, bounds, t, lens, HKV, BS, D ** -0.5, False)
+    for b, n in enumerate(lens):
+        for j in range(-(-n // BS)):
+            for h in range(H):
+                kv = h // (H // HKV)
+                s = kh[t[b, j], kv, :min(BS, n - j * BS)] @ qh[b, h] * D ** -0.5
+                assert s.max() <= got[b, kv, j] + tol[b, kv, j]
+    picked = sel.cpu().numpy()
+    assert np.array_equal(picked, blocks.plain_select(scores.cpu().numpy(), lens, BS, TOP, 1, 1))
+    want, tol = selected.plain(qh, kh, v_pool.double().cpu().numpy(), t, lens, picked, D ** -0.5, False, True)
+    assert np.all(np.abs(o.double().cpu().numpy() - want) <= tol)

@@ -159,8 +159,10 @@ class CudaAttention:
 
     # ------------------------------------------- decode over selected blocks
     def block_bounds(self, k_pool, block_tables, seq_lens, bounds, tok_begin=None, stream=None) -> None:
-        """Elementwise minimum and maximum of the keys of each block that holds a token in
-        [tok_begin[b], seq_lens[b]): k_pool [num_blocks][Hkv][bs][d] -> bounds [num_blocks][Hkv][2][d]."""
+        """Elementwise minimum and maximum of the keys of each block from that of token tok_begin[b] (None: 0)
+        to that of the last of seq_lens[b]: k_pool [num_blocks][Hkv][bs][d] -> bounds [num_blocks][Hkv][2][d].
+        A sequence is listed once, with its largest length: rows that bound the same block must agree on how
+        many of its tokens there are."""
         import torch
         _need(k_pool.dim() == 4 and block_tables.dim() == 2, "k_pool [num_blocks][Hkv][bs][d], block_tables [B][max]")
         num_blocks, Hkv, bs, d = k_pool.shape
