@@ -149,8 +149,8 @@ zl_status zl_reshape_and_cache(zl_ctx* ctx, const void* k /*device*/, const void
  * passed over, so that the other requests keep theirs. An id outside the pool
  * (or one that new_blocks does not have) becomes -1, with slot -1, and is
  * reported too. seq_blocks entries that open no new block are left as they were.
- * block_tables does not overlap seq_blocks. At most 8192 requests and, with
- * rows, 262144 table rows: ZL_ERR_UNSUPPORTED. */
+ * seq_blocks and the outputs overlap no other argument (ZL_ERR_INVALID_ARG).
+ * At most 8192 requests and, with rows, 262144 table rows: ZL_ERR_UNSUPPORTED. */
 zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks /*device*/, int num_rows,
                          const int32_t* rows /*device*/, const int32_t* context_lens /*device*/,
                          const int32_t* query_lens /*device*/, const int32_t* new_blocks /*device*/,

@@ -195,3 +195,39 @@ def test_step_tables_no_requests(ctx):
     assert got["cu_seqlens"].tolist() == [0]
     assert got["positions"].tolist() == [0] * 5 and got["slot_mapping"].tolist() == [-1] * 5
     ctx.check_status()
+
+
+def test_step_tables_overlaps_are_refused(ctx):
+    """Outputs on inputs or on one another, the lengths in place above all: every CTA reads them while others write."""
+    import torch
+    import zealot_b200 as zb
+    new = lambda *s, dtype=torch.int32: torch.zeros(s, dtype=dtype, device="cuda")
+    names = ("seq_blocks rows context_lens query_lens new_blocks block_tables cu_seqlens seq_lens positions slot_mapping "
+             "last_rows").split()
+    shapes = dict(seq_blocks=(4, 4), block_tables=(3, 4), cu_seqlens=(4,), positions=(5,), slot_mapping=(5,))
+    make = lambda: {n: new(*shapes.get(n, (3,)), dtype=torch.int64 if n == "slot_mapping" else torch.int32) for n in names}
+    attn = zb.CudaAttention(ctx)
+
+    def call(a):
+        """A call that is taken; its requests all name row 0, which is reported."""
+        attn.step_tables(*(a[n] for n in names), 16, 8)
+        with pytest.raises(zb.OobBlockError):
+            ctx.check_status()
+
+    call(make())
+    a = make()
+    call(dict(a, context_lens=a["query_lens"], new_blocks=a["query_lens"]))  # inputs may be the same
+    for one, other in (("seq_lens", "context_lens"), ("seq_lens", "query_lens"), ("last_rows", "rows"), ("seq_lens", "new_blocks"),
+                       ("seq_lens", "last_rows"), ("last_rows", "query_lens")):
+        with pytest.raises(zb.InvalidArgument, match="overlaps"):
+            call(dict(a, **{one: a[other]}))
+    with pytest.raises(zb.InvalidArgument, match="overlaps"):
+        call(dict(a, cu_seqlens=a["positions"][:4]))
+    with pytest.raises(zb.InvalidArgument, match="overlaps"):
+        call(dict(a, context_lens=a["cu_seqlens"][1:]))
+    with pytest.raises(zb.InvalidArgument, match="overlaps"):
+        call(dict(a, rows=a["seq_blocks"].view(-1)[13:]))
+    with pytest.raises(zb.InvalidArgument, match="overlaps"):
+        call(dict(a, positions=a["slot_mapping"].view(torch.int32)[5:]))
+    neighbours = new(7)  # side by side is no overlap
+    call(dict(a, context_lens=neighbours[:3], cu_seqlens=neighbours[3:]))

@@ -289,6 +289,21 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
     return set_error(ZL_ERR_INVALID_ARG, "step_tables: block_tables overlaps seq_blocks");
   DeviceScope dev(ctx);
   if (dev.status != ZL_OK) return dev.status;
+  // Every CTA reads all requests, at no known time beside another's writes: what is written (the
+  // first seven) overlaps nothing.
+  const struct {
+    const void* p;
+    size_t bytes;
+  } parts[] = {{seq_blocks, num_rows * row_bytes}, {block_tables, num_seqs * row_bytes}, {cu_seqlens, 4 * (size_t)num_seqs + 4},
+               {seq_lens, 4 * (size_t)num_seqs}, {last_rows, 4 * (size_t)num_seqs}, {positions, 4 * (size_t)num_tokens},
+               {slot_mapping, 8 * (size_t)num_tokens}, {rows, rows ? 4 * (size_t)num_seqs : 0},
+               {context_lens, 4 * (size_t)num_seqs}, {query_lens, 4 * (size_t)num_seqs}, {new_blocks, 4 * (size_t)num_new}};
+  for (int i = 0; i < 7; i++)
+    for (int j = i + 1; j < 11; j++) {
+      const auto a = reinterpret_cast<uintptr_t>(parts[i].p), b = reinterpret_cast<uintptr_t>(parts[j].p);
+      if (parts[i].bytes && parts[j].bytes && a < b + parts[j].bytes && b < a + parts[i].bytes)
+        return set_error(ZL_ERR_INVALID_ARG, "step_tables: an output overlaps another argument");
+    }
   StepArgs g{seq_blocks, rows, context_lens, query_lens, new_blocks, block_tables, cu_seqlens, seq_lens, positions,
              slot_mapping, last_rows, num_new, num_tokens, num_blocks, num_rows, num_seqs, max_blocks_per_seq,
              block_size, ctx->d_status};
