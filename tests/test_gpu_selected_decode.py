@@ -259,3 +259,41 @@ def test_closed_context_is_refused(ctx):
     other.close()
     with pytest.raises(zb.InvalidArgument, match="null context"):
         attn.select_blocks(scores, lens, selected, 16)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("lens,d,bs,top", [([1], 128, 16, 1), ([60, 17], 128, 16, 4), ([60, 17], 64, 16, 4), ([60, 17], 256, 16, 4),
+                                           ([60, 17], 72, 5, 12), ([60, 17], 33, 16, 4), ([5000], 128, 16, 300), ([40] * 90, 128, 8, 5)])
+def test_selected_infinite_values(ctx, lens, d, bs, top, bf16):
+    """Infinite and NaN values in places that count: infinity of the value's sign where all of them agree, NaN where they
+    do not, whatever the token's weight (the scores here leave each token 2^-40 of its row or more), and the other
+    elements as if nothing were there. In every kernel."""
+    import torch
+    import zealot_b200 as zb
+    rng = np.random.default_rng(len(lens) + d)
+    H, Hkv = 8, 2
+    nb = sum(-(-n // bs) for n in lens) + 3
+    q, kp, vp, table, lens = decode_case(rng, len(lens), lens, H, Hkv, d, bs, nb)
+    sel = lists(rng, lens, Hkv, bs, top)
+    places = {}  # (sequence, kv head, element) -> values
+    for b in range(len(lens)):
+        for h in range(Hkv):
+            tokens = [j * bs + t for j in sel[b, h] if j >= 0 for t in range(bs) if j * bs + t < lens[b]]
+            for t, e, x in zip(rng.permutation(tokens * 8)[:8], (0, 1, 2, 3, 3, 4, 4, d - 1),
+                               (np.inf, -np.inf, np.inf, np.inf, np.inf, np.inf, -np.inf, np.nan)):
+                old = vp[table[b, t // bs], h, t % bs, e]
+                vp[table[b, t // bs], h, t % bs, e] = x if np.isfinite(old) else old + x  # one token twice: both
+                places.setdefault((b, h, e), []).append(x)
+    dt = torch.bfloat16 if bf16 else torch.float32
+    tq, tk, tv = dev(q, dt), dev(kp, dt), dev(vp, dt)
+    o = torch.empty(q.shape, dtype=dt, device="cuda")
+    zb.CudaAttention(ctx).paged_forward_selected(tq, tk, tv, dev(table), dev(lens), dev(sel), o)
+    ctx.check_status()
+    got = o.double().cpu().numpy()
+    finite = torch.where(torch.isfinite(tv), tv, torch.zeros_like(tv))
+    want, tol = plain(*(t.double().cpu().numpy() for t in (tq, tk, finite)), table, lens, sel, d ** -0.5, False, bf16)
+    for (b, h, e), x in places.items():
+        heads = slice(h * H // Hkv, (h + 1) * H // Hkv)
+        assert np.array_equal(got[b, heads, e], np.full(H // Hkv, sum(x)), equal_nan=True), (b, h, e, x)
+        got[b, heads, e] = want[b, heads, e] = 0
+    assert np.all(np.abs(got - want) <= tol)

@@ -19,8 +19,10 @@
 // order. O^T = V^T P^T has 16 elements of a value row as M and the heads as N: a
 // lane reads 16 bytes of each of four token rows and pairs two tokens' elements
 // with a byte permute. S's accumulators are P^T's operands as they stand. P enters
-// as two bf16 parts, p - bf16(p) being the second: the weights then keep 16 bits,
-// for one more instruction per tile in a kernel that waits for memory.
+// as two bf16 parts that are both positive: the weights then keep 16 bits, for one more
+// instruction per tile in a kernel that waits for memory, and an infinite value gives infinity,
+// as it does with one weight (a second part of 0 or below would make it NaN), down to weights
+// of 2^-110 of the largest, where the second part leaves bf16's range.
 //
 // fp32 (selected_f32_kernel), tiles of 8 tokens: eight lanes share a token's row,
 // on the CUDA cores with packed pairs.
@@ -236,6 +238,9 @@ __device__ __forceinline__ uint32_t fetch_tile(const SelArgs& g, const Entry* en
 // take over at the end.
 constexpr size_t ring_bytes(int rowb, int tok, int st) { return (size_t)kWarps * st * tok * rowb * 2; }
 
+// The bits of the largest float below p > 0; of 0 where p is 0.
+__device__ __forceinline__ uint32_t below(float p) { return max(__float_as_int(p), 1) - 1; }
+
 // head_dim up to DT, a multiple of 8. Column n of the score tile i in {0, 1} is token 2 (n / 2) + i for even n and
 // 8 + i + (2 (n / 2) + 4) % 8 for odd n: the two rows that a quarter warp reads of the
 // keys then differ in bit 2 of the row, the four that it reads of the values in bits 1
@@ -340,9 +345,10 @@ __global__ void __launch_bounds__(kThreads) selected_mma_kernel(SelArgs g, int c
         for (int i = 0; i < 2; i++) {
           const float p0 = zl::ptx::ex2(s[i][0] - base), p1 = zl::ptx::ex2(s[i][1] - base);
           l += p0 + p1;
-          hi[i] = zl::ptx::pack_bf16x2(p0, p1);
-          const __nv_bfloat162 hb = *reinterpret_cast<const __nv_bfloat162*>(&hi[i]);
-          lo[i] = zl::ptx::pack_bf16x2(p0 - __low2float(hb), p1 - __high2float(hb));
+          // hi: what lies below p, cut to 8 bits; so lo = p - hi > 0 wherever p > 0
+          const uint32_t h0 = below(p0) & 0xffff0000u, h1 = below(p1) & 0xffff0000u;
+          hi[i] = __byte_perm(h0, h1, 0x7632);
+          lo[i] = zl::ptx::pack_bf16x2(p0 - __uint_as_float(h0), p1 - __uint_as_float(h1));
         }
         // O^T: rows n and n + 8 of tile (a, j) are elements 64 a + 8 n + j and + 4
 #pragma unroll
