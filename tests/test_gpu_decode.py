@@ -347,3 +347,34 @@ def test_bf16_one_kv_head_long_split(ctx, oracle):
     ref = oracle.paged_decode(tq.float().cpu().numpy(), tk.float().cpu().numpy(), tv.float().cpu().numpy(),
                               table, lens, H, Hkv, d, bs, nb, num_threads=8)
     assert np.max(np.abs(out.float().cpu().numpy() - ref)) <= BF16_ATOL
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+def test_generic_kernels_keep_nan(ctx, bf16):
+    """A query of NaN in the kernels for every shape: every score is NaN, and so is the row, as in the oracle's softmax;
+    the other rows are those of the same call without it."""
+    import torch
+    import zealot_b200 as zb
+    rng = np.random.default_rng(1)
+    dt = torch.bfloat16 if bf16 else torch.float32
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.float32)).cuda().to(dt)
+    from helpers import decode_case
+    q, kp, vp, table, lens = decode_case(rng, 2, [300, 5], 4, 2, 33, 16, 30)
+    attn = zb.CudaAttention(ctx)
+    outs = []
+    for bad in (False, True):
+        q[1, 2, 7] = np.nan if bad else 0.5
+        o = torch.empty((2, 4, 33), dtype=dt, device="cuda")
+        attn.paged_forward(dev(q), dev(kp), dev(vp), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(), o, 2, 4,
+                           2, 33, 16, table.shape[1], num_blocks=30)
+        x = rng.standard_normal((9, 8, 33)) if not bad else x
+        x[4, 1, 0] = np.nan if bad else 0.5
+        p = torch.empty((9, 4, 33), dtype=dt, device="cuda")
+        attn.forward_gpu(dev(x[:, :4]), dev(x[:, 4:6]), dev(x[:, 6:]), torch.tensor([0, 6, 9], dtype=torch.int32, device="cuda"),
+                         p, 4, 2, 33, 6)
+        ctx.check_status()
+        outs.append((o, p))
+    for (a, b), row in zip(zip(*outs), ((1, 2), (4, 1))):
+        assert torch.isfinite(a).all() and torch.isnan(b[row]).all()
+        b[row] = a[row]
+        assert torch.equal(a, b)

@@ -297,3 +297,34 @@ def test_selected_infinite_values(ctx, lens, d, bs, top, bf16):
         assert np.array_equal(got[b, heads, e], np.full(H // Hkv, sum(x)), equal_nan=True), (b, h, e, x)
         got[b, heads, e] = want[b, heads, e] = 0
     assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("d,bs", [(128, 16), (64, 8), (256, 16), (72, 5), (33, 16), (8, 16)])
+def test_selected_nan_reaches_the_output(ctx, d, bs, bf16):
+    """A NaN in a query head: that head's row. Lists whose keys are all NaN, short or longer than one chunk of keys, and
+    one NaN key among others: the kv head's rows. The rest as the formula has it."""
+    import torch
+    import zealot_b200 as zb
+    rng = np.random.default_rng(d)
+    q, kp, vp, table, lens = decode_case(rng, 4, [60, 7, 400, 300], 8, 2, d, bs, 400)
+    sel = lists(rng, lens, 2, bs, 400 // bs)
+    dt = torch.bfloat16 if bf16 else torch.float32
+    clean = [dev(x, dt).double().cpu().numpy() for x in (q, kp, vp)]
+    want, tol = plain(*clean, table, lens, sel, d ** -0.5, False, bf16)
+    q[0, 5, 0] = np.nan
+    want[0, 5] = np.nan
+    for b, h in ((1, 0), (2, 1)):
+        for j in sel[b, h][sel[b, h] >= 0]:
+            kp[table[b, j], h, :, d - 1] = np.nan
+        want[b, 4 * h:4 * h + 4] = np.nan
+    j = sel[3, 0, 2]
+    kp[table[3, j], 0, 1, 0] = np.nan
+    want[3, :4] = np.nan
+    o = torch.full(q.shape, 9.0, dtype=dt, device="cuda")
+    zb.CudaAttention(ctx).paged_forward_selected(dev(q, dt), dev(kp, dt), dev(vp, dt), dev(table), dev(lens), dev(sel), o)
+    ctx.check_status()
+    got = o.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    ok = ~np.isnan(want)
+    assert np.all(np.abs(got - want)[ok] <= tol[ok])

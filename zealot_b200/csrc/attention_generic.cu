@@ -82,7 +82,7 @@ __device__ void attend(const T* __restrict__ kbase, const T* __restrict__ vbase,
     const float cmax = block_max(s, sh.red);
     const float m_new = fmaxf(m, cmax);
     float p = 0.f;
-    if (row >= 0 && m_new != -INFINITY) p = expf(s - m_new);
+    if (row >= 0) p = expf(s - (m_new == -INFINITY ? 0.f : m_new));  // NaN where the score is, also if all are
     const float alpha = (m == -INFINITY) ? 0.f : expf(m - m_new);
     sh.p[tid] = p;
     sh.row[tid] = row;
