@@ -175,7 +175,8 @@ zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks /*device*/, int num_ro
  * q_out [T][H][d], k_out and v_out [T][Hkv][d] packed (what zl_prefill_varlen
  * takes), and k_pool / v_pool, both or neither, at slot_mapping[t] as
  * zl_reshape_and_cache writes them: slot < 0 skips the token's write, slot >=
- * num_blocks * block_size is reported and skipped, and slots are distinct.
+ * num_blocks * block_size is reported and skipped, and slots are distinct. An
+ * input of which no output is asked for may be NULL.
  * Values are copied bit for bit; the rest is computed in fp32 and rounded once.
  * An output may be its own input where that is packed; otherwise outputs do
  * not overlap inputs. head_dim up to 256 (larger: ZL_ERR_UNSUPPORTED). */

@@ -120,3 +120,13 @@ def test_c_floats_arrive():
         calls.block_scores(*dict(SCORES, scale="x").values())
     with pytest.raises(TypeError):
         calls.qk_norm_rope(*dict(ROPE, eps=None).values())
+
+
+def test_head_rows_of_none():
+    import torch
+    from zealot_b200 import calls
+    k = torch.zeros((5, 2, 4))
+    assert calls.head_rows(-1, torch.float32, 5, 4, None, 6, k, 2, None, 2) == (0, 0, k.data_ptr(), 8, 0, 0)
+    assert calls.head_rows(-1, torch.float32, 5, 4, None, 6, k, 3) == 1
+    with pytest.raises(TypeError):
+        calls.head_rows(-1, torch.float32, 5, 4, None, None)

@@ -246,3 +246,32 @@ def test_values_alone_need_no_positions(ctx, T, d, bf16):
                   head_dim=d, q_stride=2 * d, dtype=int(bf16), stream=torch.cuda.current_stream().cuda_stream) == 0
     ctx.check_status()
     assert torch.equal(out, v)
+
+
+@pytest.mark.parametrize("T,d", [(5, 64), (1500, 64), (5, 33)])
+def test_keys_or_values_alone(ctx, T, d):
+    """Without queries, from Python and with any query stride in the C call; values alone; None with something asked of it."""
+    import torch
+    import zealot_b200 as zb
+    _, q, k, v, w = make(T, 8, 2, d, True)
+    rot = d // 2 * 2
+    pos, freq = torch.arange(T, dtype=torch.int32, device="cuda"), torch.from_numpy(freqs(rot)).cuda()
+    attn = zb.CudaAttention(ctx)
+    full = [torch.empty((T, n, d), dtype=q.dtype, device="cuda") for n in (8, 2, 2)]
+    attn.qk_norm_rope(q, k, v, pos, freq, *full, q_weight=w[0], k_weight=w[1])
+    out = [torch.empty_like(full[1]) for _ in range(3)]
+    attn.qk_norm_rope(None, k, None, pos, freq, k_out=out[0], k_weight=w[1])
+    attn.qk_norm_rope(None, None, v, None, None, v_out=out[1])
+    assert c_call(ctx, k=k, q_stride=1, k_stride=k.stride(0), k_weight=w[1], eps=1e-6, positions=pos, inv_freq=freq, rotary_dim=rot,
+                  k_out=out[2], num_tokens=T, num_heads=8, num_kv_heads=2, head_dim=d, dtype=1,
+                  stream=torch.cuda.current_stream().cuda_stream) == 0
+    ctx.check_status()
+    # another query stride may take another kernel: within both of their tolerances
+    near(out[0], formula(k.float().cpu().numpy(), w[1].float().cpu().numpy(), 1e-6, pos.cpu().numpy(), freqs(rot), False), True, d)
+    near(out[2], formula(k.float().cpu().numpy(), w[1].float().cpu().numpy(), 1e-6, pos.cpu().numpy(), freqs(rot), False), True, d)
+    assert torch.equal(out[1], v)
+    for args, asked in (((None, k, v), "q_out"), ((q, None, v), "k_out"), ((q, k, None), "v_out")):
+        with pytest.raises(zb.InvalidArgument):
+            attn.qk_norm_rope(*args, pos, freq, **{asked: full["qkv".index(asked[0])]})
+    with pytest.raises(zb.InvalidArgument):
+        attn.qk_norm_rope(None, None, None, pos, freq, q_out=full[0])

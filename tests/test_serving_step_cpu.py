@@ -167,3 +167,11 @@ def test_python_checks_refuse_other_devices(attn):
         attn.select_blocks(f, i, i2[None], 16)
     with pytest.raises(zb.InvalidArgument, match="cuda:0"):
         attn.paged_forward_selected(f, pool, pool, i2, i, i2[None], f)
+
+
+def test_qk_norm_rope_takes_keys_alone(lib):
+    """No queries: their stride says nothing. (With a context the call would launch: "null context" is its last check.)"""
+    for change in (dict(q_stride=0), dict(q_stride=1), dict(q_stride=768), dict(q_stride=512)):
+        _refused(lib, "zl_qk_norm_rope", ROPE, INVALID, "null context", q=None, q_out=None, **change)
+    _refused(lib, "zl_qk_norm_rope", ROPE, INVALID, "null context", q=None, q_out=None, k=None, k_out=None, v_out=P,
+             positions=None, q_stride=0, k_stride=0)

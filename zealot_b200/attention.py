@@ -64,11 +64,15 @@ class CudaAttention:
         """RMS norm of each head of q [T][H][d] and k [T][Hkv][d] (a weight [d] or None), rotation of the
         first 2 * inv_freq.numel() elements of each head by positions[t] * inv_freq (float64; None: no
         rotation), and the stores: q_out, k_out, v_out packed, and the pools [num_blocks][Hkv][bs][d] at
-        slot_mapping. q, k and v may be views of one projection's rows (any stride from token to token)."""
+        slot_mapping. q, k and v may be views of one projection's rows (any stride from token to token), and
+        None where nothing of them is asked for."""
         import torch
-        dtype = q.dtype
-        T, H, d = q.shape
-        Hkv = k.shape[1]
+        x = q if q is not None else k if k is not None else v
+        _need(x is not None, "one of q, k and v")
+        dtype = x.dtype
+        T, heads, d = x.shape
+        Hkv = k.shape[1] if k is not None else v.shape[1] if v is not None else heads
+        H = heads if q is not None else Hkv
         rows = calls.head_rows(self.ctx.device, dtype, T, d, q, H, k, Hkv, v, Hkv)
         if type(rows) is not tuple:
             raise InvalidArgument("q [T][H][d], k and v [T][Hkv][d]: one dtype, on the context's device, the heads of a "

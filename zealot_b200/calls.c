@@ -168,7 +168,7 @@ static PyObject* addresses(PyObject* self, PyObject* const* args, Py_ssize_t nar
 }
 
 /* head_rows(device, dtype, T, d, tensor, heads, tensor, heads, ...) -> (address, token stride, ...)
- * of tensors [T][heads][d] whose heads lie side by side, or the number of the first that is none. */
+ * of tensors [T][heads][d] whose heads lie side by side (0, 0 for None), or the number of the first that is none. */
 static PyObject* head_rows(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs < 4 || nargs % 2) {
     PyErr_SetString(PyExc_TypeError, "head_rows(device, dtype, T, d, tensor, heads, ...)");
@@ -180,11 +180,12 @@ static PyObject* head_rows(PyObject* self, PyObject* const* args, Py_ssize_t nar
   PyObject* out = PyTuple_New(2 * count);
   if (!out) return NULL;
   for (Py_ssize_t i = 0; i < count; i++) {
-    View v;
+    View v = {0};
+    const int none = args[4 + 2 * i] == Py_None;
     const long long heads = PyLong_AsLongLong(args[5 + 2 * i]);
-    const int bad = (heads == -1 && PyErr_Occurred()) || look(args[4 + 2 * i], args[1], &v);
-    if (bad || !v.is_dtype || v.device != device || v.dims != 3 || v.shape[0] != T || v.shape[1] != heads ||
-        v.shape[2] != d || (v.stride[2] != 1 && d != 1) || (v.stride[1] != d && heads != 1)) {
+    const int bad = (heads == -1 && PyErr_Occurred()) || (!none && look(args[4 + 2 * i], args[1], &v));
+    if (bad || (!none && (!v.is_dtype || v.device != device || v.dims != 3 || v.shape[0] != T || v.shape[1] != heads ||
+        v.shape[2] != d || (v.stride[2] != 1 && d != 1) || (v.stride[1] != d && heads != 1)))) {
       Py_DECREF(out);
       return bad ? NULL : PyLong_FromSsize_t(i);
     }

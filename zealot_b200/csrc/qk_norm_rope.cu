@@ -485,7 +485,7 @@ extern "C" zl_status zl_qk_norm_rope(zl_ctx* ctx, const void* q, const void* k, 
   const int64_t nq = (int64_t)num_heads * head_dim, nk = (int64_t)num_kv_heads * head_dim;
   if (num_tokens > 1 && ((q_out && q_stride < nq) || (need_k && k_stride < nk) || (need_v && v_stride < nk)))
     return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: a token stride is below its row");
-  if ((q_out == q && q_stride != nq && num_tokens > 1) || (k_out && k_out == k && k_stride != nk && num_tokens > 1) ||
+  if ((q_out && q_out == q && q_stride != nq && num_tokens > 1) || (k_out && k_out == k && k_stride != nk && num_tokens > 1) ||
       (v_out && v_out == v && v_stride != nk && num_tokens > 1))
     return set_error(ZL_ERR_INVALID_ARG, "qk_norm_rope: in place only on packed rows");
   DeviceScope dev(ctx);
