@@ -275,3 +275,30 @@ def test_keys_or_values_alone(ctx, T, d):
             attn.qk_norm_rope(*args, pos, freq, **{asked: full["qkv".index(asked[0])]})
     with pytest.raises(zb.InvalidArgument):
         attn.qk_norm_rope(None, None, None, pos, freq, q_out=full[0])
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("T,d", [(3, 64), (2000, 128), (2000, 72), (3, 33), (1500, 20)])
+def test_values_keep_their_bits(ctx, T, d, bf16):
+    """Every kind of number in the values, NaNs of any sign and payload among them: the same bits in the packed rows and
+    in the pools, as reshape_and_cache leaves them."""
+    import torch
+    import zealot_b200 as zb
+    g = torch.Generator(device="cuda").manual_seed(d)
+    bits, kind = (torch.int16, torch.bfloat16) if bf16 else (torch.int32, torch.float32)
+    size = torch.iinfo(bits)
+    v = torch.randint(size.min, size.max + 1, (T, 3, d), generator=g, device="cuda", dtype=torch.int64).to(bits)
+    v.view(-1)[:6] = torch.tensor([-1, size.min, size.max, 0, 0x7F81 << (0 if bf16 else 16), -2], dtype=torch.int64).to(bits).cuda()
+    v = v.view(kind)
+    assert torch.isnan(v).any()
+    k = torch.randn((T, 3, d), generator=g, device="cuda").to(kind)
+    nb = T // 16 + 2
+    slots = torch.randperm(nb * 16, generator=g, device="cuda")[:T]
+    pools = [torch.zeros((nb, 3, 16, d), dtype=kind, device="cuda") for _ in range(4)]
+    out = torch.empty_like(v)
+    pos, freq = torch.arange(T, dtype=torch.int32, device="cuda"), torch.from_numpy(freqs(d // 4 * 2)).cuda()
+    attn = zb.CudaAttention(ctx)
+    attn.qk_norm_rope(k, k, v, pos, freq, v_out=out, k_weight=k[0, 0].contiguous(), k_pool=pools[0], v_pool=pools[1], slot_mapping=slots)
+    attn.reshape_and_cache(k, v, pools[2], pools[3], slots, 3, d, 16, nb)
+    ctx.check_status()
+    assert torch.equal(out.view(bits), v.view(bits)) and torch.equal(pools[1].view(bits), pools[3].view(bits))

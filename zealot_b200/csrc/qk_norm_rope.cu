@@ -45,8 +45,12 @@ struct RopeArgs {
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void put(float* p, float x) { *p = x; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+// With `copied` x is an element as it was loaded, which keeps its bits: a rounding would make
+// every NaN the same one.
+__device__ __forceinline__ void put(float* p, float x, bool) { *p = x; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float x, bool copied) {
+  *p = copied ? __ushort_as_bfloat16((unsigned short)(__float_as_uint(x) >> 16)) : __float2bfloat16_rn(x);
+}
 
 // cos and sin of position * frequency: the angle in turns, with 1 / (2 pi) in two parts, less
 // its whole turns.
@@ -117,12 +121,12 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(RopeArgs g) {
     __syncwarp();
     if (out) {
       out += (t * (isq ? g.H : g.Hkv) + hh) * (int64_t)g.d;
-      for (int e = lane; e < g.d; e += 32) put(out + e, x[e]);
+      for (int e = lane; e < g.d; e += 32) put(out + e, x[e], !isq && !isk);
     }
     if (pool) {
       const int64_t row = cache_row(g, t, hh);
       if (row >= 0)
-        for (int e = lane; e < g.d; e += 32) put(pool + row * g.d + e, x[e]);
+        for (int e = lane; e < g.d; e += 32) put(pool + row * g.d + e, x[e], !isk);
     }
   }
 }
@@ -161,6 +165,16 @@ __device__ __forceinline__ void store_run(__nv_bfloat16* p, const Run<4>& q) {
 }
 __device__ __forceinline__ void store_run(__nv_bfloat16* p, const Run<8>& q) {
   *reinterpret_cast<uint4*>(p) = make_uint4(bf16_pair(q.p[0]), bf16_pair(q.p[1]), bf16_pair(q.p[2]), bf16_pair(q.p[3]));
+}
+
+// The bits of bf16 elements as they were loaded.
+__device__ __forceinline__ uint32_t bits_of(uint64_t p) {
+  const float2 f = px::f2_unpack(p);
+  return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
+}
+__device__ __forceinline__ uint2 bits_of(const Run<4>& q) { return make_uint2(bits_of(q.p[0]), bits_of(q.p[1])); }
+__device__ __forceinline__ uint4 bits_of(const Run<8>& q) {
+  return make_uint4(bits_of(q.p[0]), bits_of(q.p[1]), bits_of(q.p[2]), bits_of(q.p[3]));
 }
 
 // Rotates a lane's two runs by the angles of its E pairs: 16 bytes (c0, c1, s0, s1) for two of
@@ -275,9 +289,10 @@ __device__ __forceinline__ void fill_shared(const RopeArgs& g, int64_t t0, int t
 }
 
 // Norms and rotates one row and stores it to `out` (unless r.out is null) and to the pool row at
-// element `at` (unless -1); cs: its token's angles.
+// element `at` (unless -1); cs: its token's angles. Returns whether the row is of values with a NaN,
+// which the rounding has made another one: copy_row then puts its bits right.
 template <typename T, int LG, int E>
-__device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>& ln, const HeadRows<T>& r, Run<E> a,
+__device__ __forceinline__ bool finish_row(const RopeArgs& g, const Lane<LG, E>& ln, const HeadRows<T>& r, Run<E> a,
                                            Run<E> b, const Shared<LG, E>& sh, const ulonglong2* cs, T* out, int64_t at) {
   uint64_t sa = 0, sb = 0;
 #pragma unroll
@@ -289,7 +304,7 @@ __device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>&
   float ss = both.x + both.y;
 #pragma unroll
   for (int o = LG / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (!r.use) return;
+  if (!r.use) return false;
   if (r.norm) {
     const float y = ss * g.inv_d + g.eps, q = rsqrtf(y);
     const float step = q * fmaf(-0.5f * y * q, q, 1.5f);  // a Newton step: right to fp32's last place or so
@@ -313,6 +328,21 @@ __device__ __forceinline__ void finish_row(const RopeArgs& g, const Lane<LG, E>&
   if (r.pool && at >= 0) {
     store_run(r.pool + at, a);
     store_run(r.pool + at + ln.gap, b);
+  }
+  return ss != ss && !r.norm && !r.turn;
+}
+
+// Stores a row's two runs with their bits as they are, where finish_row stores them.
+template <typename Bits, typename T, int LG, int E>
+__device__ __forceinline__ void copy_row(const Lane<LG, E>& ln, const HeadRows<T>& r, Bits a, Bits b, T* out, int64_t at) {
+  static_assert(sizeof(Bits) == E * sizeof(T), "a run");
+  if (r.out) {
+    *reinterpret_cast<Bits*>(out) = a;
+    *reinterpret_cast<Bits*>(out + ln.gap) = b;
+  }
+  if (r.pool && at >= 0) {
+    *reinterpret_cast<Bits*>(r.pool + at) = a;
+    *reinterpret_cast<Bits*>(r.pool + at + ln.gap) = b;
   }
 }
 
@@ -344,7 +374,10 @@ __global__ void __launch_bounds__(256) rope_token_kernel(RopeArgs g) {
       __syncthreads();
       tables = true;
     }
-    finish_row(g, ln, r, a, b, sh, cs, r.out, cache[0]);
+    const bool lost = finish_row(g, ln, r, a, b, sh, cs, r.out, cache[0]);
+    if constexpr (sizeof(T) == 2) {
+      if (lost) copy_row(ln, r, bits_of(a), bits_of(b), r.out, cache[0]);
+    }
   }
 }
 
@@ -414,7 +447,13 @@ __global__ void __launch_bounds__(256, kResident) rope_tokens_kernel(RopeArgs g,
       a = load_run(reinterpret_cast<const T*>(dyn + from), a);
       b = load_run(reinterpret_cast<const T*>(dyn + from + 256 * RUN), b);
     }
-    finish_row(g, ln, r, a, b, sh, cs + c * (g.rot / 4), out, r.use && r.pool ? cache[c] : -1);
+    const int64_t at = r.use && r.pool ? cache[c] : -1;
+    const bool lost = finish_row(g, ln, r, a, b, sh, cs + c * (g.rot / 4), out, at);
+    if constexpr (sizeof(T) == 2) {
+      using Bits = decltype(bits_of(a));
+      if (lost)
+        copy_row(ln, r, *reinterpret_cast<const Bits*>(dyn + from), *reinterpret_cast<const Bits*>(dyn + from + 256 * RUN), out, at);
+    }
     from = from == threadIdx.x * RUN + (kAhead - 1) * SLOT ? threadIdx.x * RUN : from + SLOT;
     out += slices * r.out_stride;
     if (h < heads && (c += slices) >= tokens) {
