@@ -11,7 +11,8 @@ Every .cu / .cc file under zealot_b200/csrc is compiled with
 zealot_b200/libzealot_attn.so (static CUDA runtime, no libcuda link: the
 driver entry points are resolved at run time, so the library also loads on a
 machine without a GPU driver). zealot_b200/calls.c, the Python call path of the
-small operators, becomes zealot_b200/calls.so beside it.
+small operators, becomes zealot_b200/calls.so beside it, where there are torch
+and Python's headers; a host in another language needs only the library.
 """
 from __future__ import annotations
 
@@ -85,9 +86,15 @@ def _build_calls(force: bool) -> None:
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "zealot_attn.h")))
     if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest:
         return
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]  # its tensor exchange header
-    cmd = ["gcc", "-O2", "-Wall", "-shared", "-fPIC", f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
-           f"-I{os.path.join(torch, 'include')}", src, "-o", CALLS, f"-L{HERE}", "-l:libzealot_attn.so", "-Wl,-rpath,$ORIGIN"]
+    torch = importlib.util.find_spec("torch")  # for its tensor exchange header
+    python = sysconfig.get_paths()["include"]
+    if torch is None or not os.path.exists(os.path.join(python, "Python.h")):
+        sys.stderr.write(f"{os.path.basename(CALLS)} is not built (no {'Python.h' if torch else 'torch'} here): the library "
+                         "is complete without it, the Python methods of the serving-step operators are not\n")
+        return
+    cmd = ["gcc", "-O2", "-Wall", "-shared", "-fPIC", f"-I{python}", f"-I{INCLUDE}",
+           f"-I{os.path.join(torch.submodule_search_locations[0], 'include')}", src, "-o", CALLS, f"-L{HERE}",
+           "-l:libzealot_attn.so", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"gcc failed for {src}:\n{r.stdout}\n{r.stderr}")
