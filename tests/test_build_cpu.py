@@ -38,3 +38,37 @@ def test_a_call_path_that_does_not_compile_is_an_error(build, monkeypatch):
 def test_the_call_path_is_built_where_both_are(build):
     build._build_calls(force=False)
     assert os.path.exists(build.CALLS)
+
+
+def _python(code):
+    import subprocess
+    import sys
+    return subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+
+
+def test_the_package_without_its_call_path():
+    """Only the calls that go through it are refused, in words; what does not need it works."""
+    r = _python("""
+import sys
+sys.modules["zealot_b200.calls"] = None  # importing it fails
+import torch
+import zealot_b200 as zb
+assert zb.BlockManager(4, 16).allocate().block_id >= 0
+class Context:
+    device, lib, address = 0, zb.lib, 0
+x = torch.zeros((1, 1, 4))
+try:
+    zb.CudaAttention(Context()).select_blocks(x, x, x, 16)
+except ImportError as e:
+    assert "build.py" in str(e), e
+else:
+    assert False
+""")
+    assert r.returncode == 0, r.stderr
+
+
+def test_the_call_path_is_one_for_each_python(build):
+    import sysconfig
+    from zealot_b200 import calls
+    assert os.path.basename(calls.__file__) == "calls" + sysconfig.get_config_var("EXT_SUFFIX")
+    assert not os.path.exists(os.path.join(os.path.dirname(calls.__file__), "calls.so"))

@@ -11,9 +11,21 @@ tensors, checked here and handed to the C ABI by address.
 """
 from __future__ import annotations
 
-from . import calls  # native, built by build.py beside the library
 from .context import GpuContext, GQA_GROUPED, dtype_code, ptr
 from .errors import check, InvalidArgument
+
+try:
+    from . import calls  # native, built by build.py beside the library
+except ImportError as _error:  # not built for this Python: the operators that go through it say so, the others work
+    class _NoCalls:
+        def __init__(self, why: str):
+            self._why = why
+
+        def __getattr__(self, name):
+            raise ImportError(f"this call needs zealot_b200's call path for this Python ({self._why}): build it with "
+                              "`python zealot_b200/build.py`")
+
+    calls = _NoCalls(str(_error))
 
 
 def _need(cond: bool, msg: str) -> None:

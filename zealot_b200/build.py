@@ -11,7 +11,7 @@ Every .cu / .cc file under zealot_b200/csrc is compiled with
 zealot_b200/libzealot_attn.so (static CUDA runtime, no libcuda link: the
 driver entry points are resolved at run time, so the library also loads on a
 machine without a GPU driver). zealot_b200/calls.c, the Python call path of the
-small operators, becomes zealot_b200/calls.so beside it, where there are torch
+small operators, becomes a module of this CPython beside it, where there are torch
 and Python's headers; a host in another language needs only the library.
 """
 from __future__ import annotations
@@ -28,7 +28,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libzealot_attn.so")
-CALLS = os.path.join(HERE, "calls.so")
+CALLS = os.path.join(HERE, "calls" + sysconfig.get_config_var("EXT_SUFFIX"))  # one for each CPython
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -83,6 +83,9 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
 
 def _build_calls(force: bool) -> None:
     src = os.path.join(HERE, "calls.c")
+    untagged = os.path.join(HERE, "calls.so")
+    if os.path.exists(untagged):  # of a build before the name said which CPython: any would take it
+        os.remove(untagged)
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "zealot_attn.h")))
     if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest:
         return
