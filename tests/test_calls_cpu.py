@@ -130,3 +130,21 @@ def test_head_rows_of_none():
     assert calls.head_rows(-1, torch.float32, 5, 4, None, 6, k, 3) == 1
     with pytest.raises(TypeError):
         calls.head_rows(-1, torch.float32, 5, 4, None, None)
+
+
+@pytest.mark.parametrize("lost", ["torch.Tensor.__dlpack_c_exchange_api__ = None", "del torch.Tensor.__dlpack_c_exchange_api__"])
+def test_a_torch_without_the_exchange_table(lost):
+    """The tests of the checks above, with every tensor read through its methods."""
+    import os
+    import subprocess
+    import sys
+    code = f"""
+import sys, torch
+sys.path.insert(0, "tests")
+{lost}
+import test_calls_cpu as t
+t.test_addresses(), t.test_head_rows(), t.test_tensors_of_other_kinds(), t.test_head_rows_of_none()
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

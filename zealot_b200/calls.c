@@ -5,8 +5,8 @@
  * launch behind them costs 3 (a step makes several such calls for every layer).
  * A tensor is read through the C exchange table that torch.Tensor offers
  * (__dlpack_c_exchange_api__), in one call without a Python object made; what
- * that does not take (a tensor that is only like one, a conjugate) through its
- * methods. This module computes nothing and keeps nothing: what is checked and
+ * that does not take (a tensor that is only like one, a conjugate), and every
+ * tensor of a torch that has no such table, through its methods. This module computes nothing and keeps nothing: what is checked and
  * what is passed stands in attention.py.
  */
 #define PY_SSIZE_T_CLEAN
@@ -20,7 +20,8 @@ static PyObject *s_dtype, *s_get_device, *s_data_ptr, *s_shape, *s_stride;
 
 /* torch, from the first call that has a tensor on */
 static struct {
-  const DLPackExchangeAPI* exchange;
+  int found;
+  const DLPackExchangeAPI* exchange; /* NULL where this torch has none that is known here: tensors through their methods */
   PyObject* tensor;
   struct {
     PyObject* dtype;
@@ -34,23 +35,21 @@ static int find_torch(void) {
     uint8_t code, bits;
   } kinds[5] = {{"int32", kDLInt, 32}, {"int64", kDLInt, 64}, {"float32", kDLFloat, 32}, {"float64", kDLFloat, 64}, {"bfloat16", kDLBfloat, 16}};
   PyObject *m = PyImport_ImportModule("torch"), *tensor = m ? PyObject_GetAttrString(m, "Tensor") : NULL;
-  PyObject* table = tensor ? PyObject_GetAttrString(tensor, "__dlpack_c_exchange_api__") : NULL;
-  const DLPackExchangeAPI* exchange = table ? PyCapsule_GetPointer(table, "dlpack_exchange_api") : NULL;
-  int ok = exchange != NULL;
+  int ok = tensor != NULL;
   for (int i = 0; i < 5 && ok; i++) {
     torch.kinds[i].code = kinds[i].code;
     torch.kinds[i].bits = kinds[i].bits;
     ok = (torch.kinds[i].dtype = PyObject_GetAttrString(m, kinds[i].name)) != NULL;
   }
-  if (ok && exchange->header.version.major != DLPACK_MAJOR_VERSION) {
-    PyErr_SetString(PyExc_ImportError, "torch's tensor exchange has another major version: build zealot_b200 again");
-    ok = 0;
-  }
   if (ok) {
+    PyObject* table = PyObject_GetAttrString(tensor, "__dlpack_c_exchange_api__");
+    const DLPackExchangeAPI* exchange = table ? PyCapsule_GetPointer(table, "dlpack_exchange_api") : NULL;
+    PyErr_Clear();
+    torch.exchange = exchange && exchange->header.version.major == DLPACK_MAJOR_VERSION ? exchange : NULL;
     torch.tensor = Py_NewRef(tensor);
-    torch.exchange = exchange; /* last: it says that the rest is there */
+    torch.found = 1; /* last: it says that the rest is there */
+    Py_XDECREF(table);
   }
-  Py_XDECREF(table);
   Py_XDECREF(tensor);
   Py_XDECREF(m);
   return ok;
@@ -100,11 +99,11 @@ static int look_slowly(PyObject* t, PyObject* dtype, View* v) {
 }
 
 static int look(PyObject* t, PyObject* dtype, View* v) {
-  if (!torch.exchange && !find_torch()) return -1;
+  if (!torch.found && !find_torch()) return -1;
   int kind = 0;
   while (kind < 5 && torch.kinds[kind].dtype != dtype) kind++;
   DLTensor d;
-  if (kind == 5 || !PyObject_TypeCheck(t, (PyTypeObject*)torch.tensor)) return look_slowly(t, dtype, v);
+  if (!torch.exchange || kind == 5 || !PyObject_TypeCheck(t, (PyTypeObject*)torch.tensor)) return look_slowly(t, dtype, v);
   if (torch.exchange->dltensor_from_py_object_no_sync(t, &d) != 0) {
     PyErr_Clear();
     return look_slowly(t, dtype, v);
