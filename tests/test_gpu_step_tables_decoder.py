@@ -71,3 +71,31 @@ def test_step_tables_build_refusals(ctx):
         steps.build(toks(3), [0, 1, 2], [1, 1, 1], [1, 1, 1], [], 0)  # three requests
     with pytest.raises(zb.InvalidArgument):
         steps.build(toks(11), [0], [0], [11], [0], 1)        # eleven tokens
+
+
+def test_step_tables_build_on_a_raw_stream(ctx, monkeypatch):
+    """A raw handle is a stream of the context's device, whatever the current one is: the upload is held back for that
+    device's stream. The batch is that of the current stream."""
+    import torch
+    from zealot_b200.decoder import StepTables
+    seen, real = [], torch.cuda.ExternalStream
+
+    def stream(handle, device=None, **rest):
+        seen.append(device)
+        return real(handle, device=device, **rest)
+
+    monkeypatch.setattr(torch.cuda, "ExternalStream", stream)
+    toks = torch.zeros(22, dtype=torch.int64, device="cuda")
+    batches = []
+    for raw in (False, True):
+        steps = StepTables(ctx, 4, 4, 3, 30, 16, 32)
+        own = torch.cuda.Stream()
+        own.wait_stream(torch.cuda.current_stream())
+        b = steps.build(toks, [2, 0, 3], [0, 0, 17], [20, 1, 1], [5, 6, 7], 2, stream=own.cuda_stream if raw else None)
+        torch.cuda.synchronize()
+        batches.append([getattr(b, n).clone() for n in ("slot_mapping", "cu_prefill", "block_tables", "seq_lens", "last_rows")])
+    assert seen == [toks.device]
+    assert all(torch.equal(x, y) for x, y in zip(*batches))
+    import zealot_b200 as zb
+    with pytest.raises(zb.OobBlockError):  # row 3 has no blocks yet for its 17 tokens
+        ctx.check_status()

@@ -190,7 +190,7 @@ class StepTables:
                               self.cu_seqlens[:n + 1], self.seq_lens[:n], self.positions[:T], self.slot_mapping[:T],
                               self.last_rows[:n], self.block_size, self.num_blocks, stream=stream)
         if stream is not None:  # `up` stays until that stream has read it
-            up.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
+            up.record_stream(torch.cuda.ExternalStream(stream, device=up.device) if isinstance(stream, int) else stream)
         return StepBatch(
             tokens=tokens, slot_mapping=self.slot_mapping[:T], cu_prefill=self.cu_seqlens[:num_prefill + 1],
             num_prefill=num_prefill, max_prefill_len=int(max(query_lens[:num_prefill], default=0)), prefill_tokens=P,
