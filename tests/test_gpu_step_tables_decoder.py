@@ -99,3 +99,20 @@ def test_step_tables_build_on_a_raw_stream(ctx, monkeypatch):
     import zealot_b200 as zb
     with pytest.raises(zb.OobBlockError):  # row 3 has no blocks yet for its 17 tokens
         ctx.check_status()
+
+
+def test_step_tables_build_refuses_lengths_and_counts_that_are_none(ctx):
+    import torch
+    import zealot_b200 as zb
+    from zealot_b200.decoder import StepTables
+    steps = StepTables(ctx, 4, 4, 3, 30, 16, 32)
+    toks = lambda n: torch.zeros(n, dtype=torch.int64, device="cuda")
+    for tokens, query, num_prefill in ((4, [5], 2),        # more chunks than requests: a decode row of minus one
+                                       (4, [2, 1], -1),    # counted from the end
+                                       (2, [3, -1], 2),    # the sum fits, one length is none
+                                       (0, [-1], 1)):
+        with pytest.raises(zb.InvalidArgument):
+            steps.build(toks(tokens), list(range(len(query))), [0] * len(query), query, [0], num_prefill)
+    b = steps.build(toks(0), [0], [0], [0], [], 1)         # an empty prompt is one
+    assert b.prefill_tokens == 0 and b.seq_lens.numel() == 0 and b.last_rows.tolist() == [0]
+    ctx.check_status()

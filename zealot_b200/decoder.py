@@ -177,7 +177,10 @@ class StepTables:
         the ids that the requests open, in request order (blocks_needed of each). The batch holds views
         of this object's buffers: the next build on it overwrites them."""
         import torch
-        n, P = len(query_lens), int(sum(query_lens[:num_prefill]))
+        n = len(query_lens)
+        if not 0 <= num_prefill <= n or any(q < 0 for q in query_lens):
+            raise InvalidArgument(f"{num_prefill} prompt chunks of {n} requests, lengths from 0")
+        P = int(sum(query_lens[:num_prefill]))
         T = P + n - num_prefill
         if len(rows) != n or len(context_lens) != n or any(c != 0 for c in context_lens[:num_prefill]):
             raise InvalidArgument("a row and lengths for each request, prompt chunks from position 0")
