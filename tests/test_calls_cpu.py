@@ -132,6 +132,20 @@ def test_head_rows_of_none():
         calls.head_rows(-1, torch.float32, 5, 4, None, None)
 
 
+def test_addresses_of_shapes():
+    import torch
+    from zealot_b200 import calls
+    f = torch.zeros((3, 4))
+    assert calls.addresses(-1, f, torch.float32, (3, 4), None, torch.float32, (9,)) == (f.data_ptr(), 0)
+    for bad in ((4, 3), (12,), (3, 4, 1), (1, 3, 4), (), (3, -4)):
+        assert calls.addresses(-1, f, torch.float32, bad) == 0
+    assert calls.addresses(-1, f.T, torch.float32, (4, 3)) == 0  # that shape, but not in order
+    assert calls.addresses(-1, torch.zeros(()), torch.float32, ()) != 0
+    assert calls.addresses(-1, torch.zeros((0, 7)), torch.float32, (0, 7)) == (0,)
+    with pytest.raises(TypeError):
+        calls.addresses(-1, f, torch.float32, (3, "4"))
+
+
 @pytest.mark.parametrize("lost", ["torch.Tensor.__dlpack_c_exchange_api__ = None", "del torch.Tensor.__dlpack_c_exchange_api__"])
 def test_a_torch_without_the_exchange_table(lost):
     """The tests of the checks above, with every tensor read through its methods."""
@@ -143,7 +157,7 @@ import sys, torch
 sys.path.insert(0, "tests")
 {lost}
 import test_calls_cpu as t
-t.test_addresses(), t.test_head_rows(), t.test_tensors_of_other_kinds(), t.test_head_rows_of_none()
+t.test_addresses(), t.test_head_rows(), t.test_tensors_of_other_kinds(), t.test_head_rows_of_none(), t.test_addresses_of_shapes()
 """
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)

@@ -225,3 +225,33 @@ def test_several_tokens_of_a_sequence(ctx):
     assert np.array_equal(picked, blocks.plain_select(scores.cpu().numpy(), lens, BS, TOP, 1, 1))
     want, tol = selected.plain(qh, kh, v_pool.double().cpu().numpy(), t, lens, picked, D ** -0.5, False, True)
     assert np.all(np.abs(o.double().cpu().numpy() - want) <= tol)
+
+
+def test_other_shapes_of_the_same_size_are_refused(ctx):
+    """As many elements in another shape would be read as if they had the documented one."""
+    import torch
+    import zealot_b200 as zb
+    attn = zb.CudaAttention(ctx)
+    f32 = lambda *s: torch.zeros(s, device="cuda")
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    q, pool, bounds, table, lens, sel, scores = f32(3, 8, 64), f32(5, 2, 16, 64), f32(5, 2, 2, 64), i32(3, 4), i32(3), i32(3, 2, 4), f32(3, 2, 4)
+    attn.paged_forward_selected(q, pool, pool, table, lens, sel, torch.empty_like(q))
+    attn.block_scores(q, bounds, table, lens, scores, 16)
+    attn.select_blocks(scores, lens, sel, 16)
+    for bad in (q.view(6, 8, 32), q.view(1, 8, 192), q.view(2, 12, 64)):
+        with pytest.raises(zb.InvalidArgument):
+            attn.paged_forward_selected(bad, pool, pool, table, lens, sel, torch.empty_like(q))
+        with pytest.raises(zb.InvalidArgument):
+            attn.block_scores(bad, bounds, table, lens, scores, 16)
+    for bad in (sel.view(2, 3, 4), sel.view(1, 6, 4)):
+        with pytest.raises(zb.InvalidArgument):
+            attn.paged_forward_selected(q, pool, pool, table, lens, bad, torch.empty_like(q))
+        with pytest.raises(zb.InvalidArgument):
+            attn.select_blocks(scores, lens, bad, 16)
+    with pytest.raises(zb.InvalidArgument):
+        attn.paged_forward_selected(q, pool, pool.view(5, 16, 2, 64), table, lens, sel, torch.empty_like(q))
+    x, slots = f32(3, 2, 64), torch.zeros(3, dtype=torch.int64, device="cuda") - 1
+    attn.qk_norm_rope(q, x, x, None, None, k_pool=pool, v_pool=pool.clone(), slot_mapping=slots)
+    with pytest.raises(zb.InvalidArgument):
+        attn.qk_norm_rope(q, x, x, None, None, k_pool=pool, v_pool=pool.clone().view(5, 16, 2, 64), slot_mapping=slots)
+    ctx.check_status()

@@ -39,13 +39,13 @@ class CudaAttention:
         self.lib = ctx.lib
 
     def _addresses(self, *triples):
-        """(tensor or None, dtype, elements), flat: the addresses of tensors that are contiguous, of that
-        dtype and size and on the context's device. Small calls are bound by such checks, so one native
+        """(tensor or None, dtype, elements or shape), flat: the addresses of tensors that are contiguous, of
+        that dtype and size and on the context's device. Small calls are bound by such checks, so one native
         pass does them (calls.c)."""
         got = calls.addresses(self.ctx.device, *triples)
         if type(got) is not tuple:
             t, dtype, n = triples[3 * got:3 * got + 3]
-            raise InvalidArgument(f"need a contiguous {dtype} tensor of {n} elements on cuda:{self.ctx.device}, got "
+            raise InvalidArgument(f"need a contiguous {dtype} tensor of {n} {'elements ' if isinstance(n, int) else ''}on cuda:{self.ctx.device}, got "
                                   f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}")
         return got
 
@@ -99,7 +99,7 @@ class CudaAttention:
                   "both pools and a slot_mapping, or none")
             num_blocks, pool_heads, bs, pool_d = k_pool.shape
             _need(pool_heads == Hkv and pool_d == d, "pools are [num_blocks][Hkv][bs][d]")
-            pool = num_blocks * Hkv * bs * d
+            pool = (num_blocks, Hkv, bs, d)
         nk = T * Hkv * d
         qo, ko, vo, qw, kw, pos, freq, kp, vp, slots = self._addresses(
             q_out, dtype, T * H * d, k_out, dtype, nk, v_out, dtype, nk, q_weight, dtype, d, k_weight, dtype, d,
@@ -201,7 +201,7 @@ class CudaAttention:
         H, i32, dtype = q.shape[1], torch.int32, q.dtype
         _need(two == 2, "bounds is [num_blocks][Hkv][2][d]")
         x, ends, table, lens, out = self._addresses(
-            q, dtype, B * H * d, bounds, dtype, num_blocks * Hkv * 2 * d, block_tables, i32, B * width, seq_lens, i32, B,
+            q, dtype, (B, H, d), bounds, dtype, num_blocks * Hkv * 2 * d, block_tables, i32, B * width, seq_lens, i32, B,
             scores, torch.float32, B * Hkv * width)
         check(calls.block_scores(self.ctx.address, x, ends, table, lens, out, B, H, Hkv, d, block_size, width,
                                  num_blocks, scale, gqa_map, dtype_code(dtype), self.ctx.stream(stream)))
@@ -215,7 +215,7 @@ class CudaAttention:
         B, Hkv, width = scores.shape
         top = selected.shape[2]
         sc, lens, out = self._addresses(scores, torch.float32, B * Hkv * width, seq_lens, torch.int32, B,
-                                        selected, torch.int32, B * Hkv * top)
+                                        selected, torch.int32, (B, Hkv, top))
         check(calls.select_blocks(self.ctx.address, sc, lens, out, B, Hkv, block_size, width, top, num_first,
                                   num_last, self.ctx.stream(stream)))
 
@@ -229,10 +229,10 @@ class CudaAttention:
         num_blocks, Hkv, bs, d = k_pool.shape
         B, width = block_tables.shape
         H, top, i32, dtype = q.shape[1], selected.shape[2], torch.int32, q.dtype
-        pool = num_blocks * Hkv * bs * d
+        pool = (num_blocks, Hkv, bs, d)
         x, k, v, table, lens, picked, out = self._addresses(
-            q, dtype, B * H * d, k_pool, dtype, pool, v_pool, dtype, pool, block_tables, i32, B * width, seq_lens, i32, B,
-            selected, i32, B * Hkv * top, o, dtype, B * H * d)
+            q, dtype, (B, H, d), k_pool, dtype, pool, v_pool, dtype, pool, block_tables, i32, B * width, seq_lens, i32, B,
+            selected, i32, (B, Hkv, top), o, dtype, B * H * d)
         check(calls.paged_decode_selected(self.ctx.address, x, k, v, table, lens, picked, out, B, H, Hkv, d, bs,
                                           width, num_blocks, top, scale, gqa_map, dtype_code(dtype),
                                           self.ctx.stream(stream)))

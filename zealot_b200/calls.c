@@ -132,11 +132,29 @@ static int in_order(const View* v, long long n) {
   return n >= 0 && have == (unsigned long long)n && (whole || n == 0);
 }
 
-/* addresses(device, tensor, dtype, elements, tensor, dtype, elements, ...) -> the tensors'
- * addresses as a tuple (0 for None), or the number of the first that does not fit. */
+/* What a tensor is asked to have: a number of elements, or a shape (a tuple). 1: it has, with the
+ * number in *n; 0: not; -1: exception. */
+static int has(const View* v, PyObject* want, long long* n) {
+  if (!PyTuple_Check(want)) {
+    *n = PyLong_AsLongLong(want);
+    return *n == -1 && PyErr_Occurred() ? -1 : 1;
+  }
+  int same = PyTuple_GET_SIZE(want) == v->dims;
+  *n = 1;
+  for (int i = 0; i < v->dims && same; i++) {
+    const long long x = PyLong_AsLongLong(PyTuple_GET_ITEM(want, i));
+    if (x == -1 && PyErr_Occurred()) return -1;
+    same = x == v->shape[i];
+    *n *= v->shape[i];
+  }
+  return same;
+}
+
+/* addresses(device, tensor, dtype, elements or shape, tensor, dtype, elements or shape, ...) -> the
+ * tensors' addresses as a tuple (0 for None), or the number of the first that does not fit. */
 static PyObject* addresses(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs < 1 || nargs % 3 != 1) {
-    PyErr_SetString(PyExc_TypeError, "addresses(device, tensor, dtype, elements, ...)");
+    PyErr_SetString(PyExc_TypeError, "addresses(device, tensor, dtype, elements or shape, ...)");
     return NULL;
   }
   const long long device = PyLong_AsLongLong(args[0]);
@@ -148,11 +166,11 @@ static PyObject* addresses(PyObject* self, PyObject* const* args, Py_ssize_t nar
     unsigned long long address = 0;
     if (args[1 + 3 * i] != Py_None) {
       View v;
-      const long long n = PyLong_AsLongLong(args[3 + 3 * i]);
-      const int bad = (n == -1 && PyErr_Occurred()) || look(args[1 + 3 * i], args[2 + 3 * i], &v);
-      if (bad || !v.is_dtype || v.device != device || !in_order(&v, n)) {
+      long long n = 0;
+      const int fits = look(args[1 + 3 * i], args[2 + 3 * i], &v) ? -1 : has(&v, args[3 + 3 * i], &n);
+      if (fits <= 0 || !v.is_dtype || v.device != device || !in_order(&v, n)) {
         Py_DECREF(out);
-        return bad ? NULL : PyLong_FromSsize_t(i);
+        return fits < 0 ? NULL : PyLong_FromSsize_t(i);
       }
       address = n ? v.address : 0;
     }
@@ -272,7 +290,7 @@ RUN(zl_paged_decode_selected(ctx, q, kp, vp, tables, lens, selected, o, B, H, Hk
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))call_##name, METH_FASTCALL, "zl_" #name " of the C ABI, argument by argument"}
 static PyMethodDef methods[] = {
     {"addresses", (PyCFunction)(void (*)(void))addresses, METH_FASTCALL,
-     "addresses(device, tensor, dtype, elements, ...): a tuple, or the number of the first tensor that does not fit"},
+     "addresses(device, tensor, dtype, elements or shape, ...): a tuple, or the number of the first tensor that does not fit"},
     {"head_rows", (PyCFunction)(void (*)(void))head_rows, METH_FASTCALL,
      "head_rows(device, dtype, T, d, tensor, heads, ...): a tuple, or the number of the first tensor that does not fit"},
     ENTRY(step_tables), ENTRY(qk_norm_rope), ENTRY(block_bounds), ENTRY(block_scores), ENTRY(select_blocks),
