@@ -221,3 +221,65 @@ def test_select_length_past_table(ctx):
     with pytest.raises(zb.OobBlockError):
         ctx.check_status()
     assert np.array_equal(selected.cpu().numpy(), plain_select(scores.cpu().numpy(), [160, 0], 16, 4, 1, 1))
+
+
+@pytest.mark.parametrize("kind", ["normal", "ties", "equal", "special"])
+@pytest.mark.parametrize("rows,top,first,last,mb", [
+    (40, 64, 1, 2, 1025), (40, 200, 0, 0, 2048), (5, 1, 0, 0, 1600), (400, 50, 2, 3, 2049), (330, 256, 1, 4, 8192),
+    (320, 700, 0, 1, 5000), (7, 256, 1, 1, 2049), (6, 100, 1, 0, 4099), (9, 300, 2, 2, 8193), (8, 256, 1, 4, 16384),
+    (4, 900, 0, 0, 12001), (5, 64, 1, 1, 16385), (3, 64, 1, 1, 24577)])
+def test_select_wide_tables(ctx, rows, top, first, last, mb, kind):
+    """Each range of widths that has a kernel of its own, with few rows and with more than the GPU takes at once; rows of
+    every length, some of them with nothing to choose from."""
+    import torch
+    import zealot_b200 as zb
+    rng = np.random.default_rng(mb + rows)
+    lens = rng.integers(0, mb + 1, rows) * 8 - rng.integers(0, 8, rows)
+    lens[0], lens[-1] = mb * 8, min(top + 1, mb) * 8
+    scores = rng.standard_normal((rows, 1, mb)).astype(np.float32)
+    if kind == "ties":
+        scores = np.round(scores * 4) / 4
+    elif kind == "equal":
+        scores[:] = 1.5
+    elif kind == "special":
+        scores[..., ::3] = -np.inf
+        scores[..., 1::500] = np.nan
+        scores[..., 7::600] = np.inf
+        scores[..., 5::40] = np.float32(-3.4028235e38)
+        scores[..., 6::40] = np.float32(1e-45)
+    want = np.full((rows, 1, top), -1, np.int32)
+    for b in range(rows):
+        n = max(0, -(-int(lens[b]) // 8))
+        if n <= top:
+            want[b, 0, :n] = np.arange(n)
+            continue
+        mid = np.arange(first, n - last)
+        s = scores[b, 0, mid]
+        nan = np.isnan(s)
+        order = mid[np.lexsort((mid, -np.where(nan, 0, s), ~nan))]
+        want[b, 0] = np.sort(np.concatenate([np.arange(first), order[:top - first - last], np.arange(n - last, n)]))
+    selected = torch.full((rows, 1, top), 9, dtype=torch.int32, device="cuda")
+    zb.CudaAttention(ctx).select_blocks(dev(scores), dev(lens.astype(np.int32)), selected, 8, num_first=first, num_last=last)
+    ctx.check_status()
+    assert np.array_equal(selected.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("lens,H,Hkv,d,bs", [([90, 300, 0], 9, 1, 256, 16), ([500, 31], 24, 2, 160, 8), ([77], 40, 4, 256, 64),
+                                             ([200, 64], 34, 2, 136, 16)])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_scores_of_many_heads_of_more_than_128(ctx, lens, H, Hkv, d, bs, bf16):
+    import torch
+    import zealot_b200 as zb
+    rng = np.random.default_rng(d * 5 + bs)
+    q, kp, table, tl, nb = keys(rng, lens, H, Hkv, d, bs, bf16, max_blocks=-(-max(lens) // bs) + 2)
+    bounds = torch.zeros((nb, Hkv, 2, d), dtype=kp.dtype, device="cuda")
+    attn = zb.CudaAttention(ctx)
+    attn.block_bounds(kp, table, tl, bounds)
+    scores = torch.full((len(lens), Hkv, table.shape[1]), 5.0, device="cuda")
+    attn.block_scores(q, bounds, table, tl, scores, bs)
+    ctx.check_status()
+    want, tol = plain_scores(q, bounds, table.cpu().numpy(), lens, Hkv, bs, d ** -0.5, False)
+    got = scores.double().cpu().numpy()
+    there = np.isfinite(want)
+    assert np.array_equal(got[~there], want[~there])
+    assert np.all(np.abs(got[there] - want[there]) <= tol[there])

@@ -302,3 +302,24 @@ def test_values_keep_their_bits(ctx, T, d, bf16):
     attn.reshape_and_cache(k, v, pools[2], pools[3], slots, 3, d, 16, nb)
     ctx.check_status()
     assert torch.equal(out.view(bits), v.view(bits)) and torch.equal(pools[1].view(bits), pools[3].view(bits))
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("T,d,rot,inter", [(1500, 128, 128, False), (9700, 64, 32, True), (2500, 80, 80, False), (1500, 33, 32, False)])
+def test_in_place_many_tokens(ctx, T, d, rot, inter, bf16):
+    """Rows that are copied ahead while others are stored over their inputs; NaN values among them."""
+    import torch
+    import zealot_b200 as zb
+    _, q, k, v, w = make(T, 8, 2, d, bf16)
+    q, k, v = q.contiguous(), k.contiguous(), v.clone()
+    v[::7, 1, 3] = float("nan")
+    pos = torch.arange(T, dtype=torch.int32, device="cuda") * 31
+    freq = torch.from_numpy(freqs(rot)).cuda()
+    out = [torch.empty_like(t) for t in (q, k, v)]
+    attn = zb.CudaAttention(ctx)
+    attn.qk_norm_rope(q, k, v, pos, freq, *out, q_weight=w[0], k_weight=w[1], interleaved=inter)
+    attn.qk_norm_rope(q, k, v, pos, freq, q, k, v, q_weight=w[0], k_weight=w[1], interleaved=inter)
+    ctx.check_status()
+    bits = torch.int16 if bf16 else torch.int32
+    for a, b in zip(out, (q, k, v)):
+        assert torch.equal(a.view(bits), b.view(bits))

@@ -231,3 +231,19 @@ def test_step_tables_overlaps_are_refused(ctx):
         call(dict(a, positions=a["slot_mapping"].view(torch.int32)[5:]))
     neighbours = new(7)  # side by side is no overlap
     call(dict(a, context_lens=neighbours[:3], cu_seqlens=neighbours[3:]))
+
+
+@pytest.mark.parametrize("n,bs,mb,with_rows,longest,pad", [
+    # more than 512 requests, tables of 16-byte columns (the step of every request's threads, and several steps)
+    (700, 16, 132, True, 40, 8), (513, 16, 8, False, 20, 0), (600, 8, 1028, True, 5, 3),
+    # rows of more than one stretch: past 2,048 columns of 4 bytes and past 8,192 of 16, few requests and many
+    (3, 16, 2051, True, 70, 0), (2, 1, 6001, False, 300, 5), (3, 16, 8196, True, 200, 1), (2, 2, 20000, True, 50, 0),
+    (520, 16, 4100, True, 3, 2)])
+def test_step_tables_wide_and_many(ctx, n, bs, mb, with_rows, longest, pad):
+    rng = np.random.default_rng(n * 1000 + mb)
+    seq_blocks, rows, c, q, new, num_blocks = make(rng, n, bs, mb, with_rows, longest)
+    T = int(q.sum()) + pad
+    want, bad = plain(seq_blocks, rows, c, q, new, bs, num_blocks, T)
+    assert not bad
+    same(run(ctx, seq_blocks, rows, c, q, new, bs, num_blocks, T), want)
+    ctx.check_status()
