@@ -378,6 +378,8 @@ scores_mma_kernel(PagedArgs g, int parts, const __nv_bfloat16* __restrict__ q,
 // are in shared memory, 8 heads at a time. 8 sequences of 65,536 to 131,072 tokens, 32
 // fp32 query heads: 91 us for 402 MB (4.4 TB/s), bound by the latency of each tile's
 // loads and products; three CTAs of more registers to an SM took 115.
+// bf16, 8 sequences of 131,072 tokens, 8 key heads of 128: 9 query heads to each 321 us, 16 531
+// (8, on the matrix instructions, 46): bound by the products, one head at a time.
 template <typename T, int NV>
 __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts, const T* __restrict__ q,
                                                          const T* __restrict__ bounds, float scale,
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(256) scores_vec_kernel(PagedArgs g, int parts,
 //
 // Reads 4 bytes a block, so bound by its own steps: the instructions for each key, and
 // the barriers between digits. 256 of up to 8,192 blocks in 512 rows 14.7 us, in 8 rows
-// 5.2 us; 32 of some 100 in 32 rows 2.9 us. On the way there 512 rows took 18.5 with every
+// 6.2 us; 32 of some 100 in 32 rows 2.8 us. On the way there 512 rows took 18.5 with every
 // lane finding its own keys' places (now one lane walks the chosen bits of 32 keys) and the
 // keys past a row's end taken along.
 struct SelectArgs {
@@ -709,11 +711,13 @@ template <typename T>
 void launch_bounds_vec(const PagedArgs& g, const void* k_pool, const int32_t* tok_begin, void* bounds, int num_sms,
                        cudaStream_t st) {
   const int chunks = g.d * (int)sizeof(T) / 16;
-  // CTAs for each sequence: with tok_begin, which is a step's few tokens or a chunk of a
-  // prompt, some 4 to an SM in all (16 chunks of 512 tokens 4.1 us, 5.8 with one), or one where
-  // there are many sequences, which are seldom chunks (the step's tokens and scores of 64
-  // sequences of 512 tokens 6.3 us, 6.8 with 4 to an SM, of 256 15.3 and 16.7; 64 chunks of 512
-  // tokens 18.9 and 18.3); for whole prompts of any lengths some kBoundsWaves.
+  // CTAs for each sequence: some kBoundsWaves to an SM in all for whole prompts of any lengths. With
+  // tok_begin, which is a step's few tokens or a chunk of a prompt (the lengths, on the device, say
+  // which), some 4 to an SM, or one where there are many sequences, which are seldom chunks. One and
+  // 4 to an SM: 16 sequences of a new token 1.9 and 4.4 us, 64 2.0 and 4.7, 128 2.4 and 4.6; chunks
+  // of 512 tokens of 16 sequences 5.8 and 4.0, of 37 8.2 and 5.7, of 64 12.8 and 11.2, of 128 28 and
+  // 31; of 8,192 tokens of 16 68 and 54, of 64 229 and 217 (184 with kBoundsWaves). So few sequences
+  // of one token pay 2.5 us, and long chunks of many up to a fifth.
   int64_t x = ((int64_t)g.max_blocks * g.Hkv + 7) / 8;
   const int an_sm = !tok_begin ? kBoundsWaves : g.B >= num_sms / 4 ? 1 : 4;
   const int64_t few = (an_sm * (int64_t)num_sms + g.B - 1) / g.B, least = (g.Hkv + 7) / 8;
@@ -851,10 +855,11 @@ zl_status zl_select_blocks(zl_ctx* ctx, const float* scores, const int32_t* seq_
   const unsigned n = (unsigned)rows;
   const cudaStream_t st = S(stream);
   // Threads by the table's width, a few keys to each: with 256 threads and 32 keys instead of
-  // 1,024 and 8, 8 rows of 8,192 blocks take 15.4 us, not 7.0. Digits of 8 bits need 256 bins to
-  // clear and sum, of 11 bits one pass less: 1,600 rows of 650 blocks 10.4 and 21 us, 512 rows of
-  // 8,192 15.6 and 15.1. More rows than CTAs of 1,024 threads at once take half the threads
-  // (18.1 us, not 19.1; 20.7 with 256). One key to a thread for narrow tables: 2.9 us, 3.2 with 4.
+  // 1,024 and 8, 8 rows of 8,192 blocks take 10.1 us, not 6.2. Digits of 8 bits need 256 bins to
+  // clear and sum, of 11 bits one pass less: 1,600 rows of 650 blocks 9.5 and 25.8 us, 512 rows of
+  // 8,192 15.1 and 14.7. More rows than CTAs of 1,024 threads at once take half the threads (512
+  // rows of 8,192 14.7 us, not 20.6; 20.5 with 256). One key to a thread for narrow tables: 32 rows
+  // of some 100 blocks 2.8 us, 3.3 with 4.
   const bool many = rows > 2 * ctx->num_sms;
   if (max_blocks_per_seq <= 128) zl::launch_ahead(select_reg_kernel<128, 1, 8>, n, 128, 0, st, g);
   else if (max_blocks_per_seq <= 512) zl::launch_ahead(select_reg_kernel<128, 4, 8>, n, 128, 0, st, g);

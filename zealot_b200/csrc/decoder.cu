@@ -13,7 +13,8 @@
 // more compute gate/up and SiLU-gate in one tcgen05 kernel of this library
 // (gemm_swiglu.cu); smaller steps use the library GEMM and a small kernel.
 // RMSNorm and the embedding gather are small kernels; attention uses this
-// library's kernels. As in the reference runner there is no rotary embedding.
+// library's kernels. As in the reference runner there is no rotary embedding
+// (zl_qk_norm_rope serves engines that have one and their own layer loop).
 #include <dlfcn.h>
 
 #include <mutex>

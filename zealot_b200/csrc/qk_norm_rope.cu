@@ -15,7 +15,7 @@
 // the product in fp32 would be off by 0.06 radians.
 //
 // Measured on one B200 (GPU time, replayed back to back), 32 query and 8 key
-// heads of 128, bf16: 64 tokens into the cache 2.9 us, bound by latency; 53,067
+// heads of 128, bf16: 64 tokens into the cache 3.0 us, bound by latency; 53,067
 // tokens into the cache and packed rows 251 us, 1.52 GB at 6.07 TB/s (93 % of
 // the copy rate), bound by HBM.
 #include "zl_internal.h"

@@ -16,10 +16,11 @@
 // list of new ids.
 //
 // Measured on one B200 (GPU time, replayed back to back): 64 decode rows with
-// tables of 257 blocks 3.7 us, bound by latency (two dependent reads, the sums,
+// tables of 257 blocks 3.6 us, bound by latency (two dependent reads, the sums,
 // one more read). 1,024 requests with tables of 8,192 blocks and 65,536 token
 // rows 14.8 us: 49.7 MB, 3.4 TB/s, of which 3.9 us are the launch and every CTA's
-// own sums. On the way there: 4-byte entries 88 us, 16-byte ones 25, 32-bit
+// own sums. The rest is bound by instructions, not by HBM: 63 % of the issue slots
+// are taken, by one CTA of 1,024 threads to an SM, and 12 % of the DRAM's rate. On the way there: 4-byte entries 88 us, 16-byte ones 25, 32-bit
 // divisions 20, all of a stretch's loads before its first store and larger CTAs 17.
 // Stretches shared out by warps instead of CTAs: 15.3; eight loads ahead: 15.5.
 #include "zl_internal.h"
@@ -310,7 +311,8 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   const size_t smem = sizeof(int32_t) * (4 * (size_t)num_seqs + 1) + (rows ? 8 * (size_t)((num_rows + 31) / 32) : 0);
   const bool vec = max_blocks_per_seq % 4 == 0 && aligned16(seq_blocks) && aligned16(block_tables);
   // Two CTAs of 512 threads to an SM, or one of 1,024 that takes the sums over many requests once:
-  // 64 rows of 257 blocks 3.5 and 4.2 us, 1,024 rows 7.7 and 5.9, 4,000 rows 24.8 and 12.0.
+  // 64 rows of 257 blocks 3.6 and 4.3 us, 256 rows 5.5 and 4.6, 1,024 rows 7.6 and 5.9, 4,000 rows
+  // 23.8 and 11.9.
   const bool many = num_seqs > 512;
   const int kThreads = many ? 1024 : 512;
   const auto kernel = many ? (vec ? step_tables_kernel<4, 1024> : step_tables_kernel<1, 1024>)
@@ -318,9 +320,10 @@ extern "C" zl_status zl_step_tables(zl_ctx* ctx, int32_t* seq_blocks, int num_ro
   if (smem > 32 * 1024)  // with the static part it may pass 48 KB
     // one limit of the function on the device, for all threads' calls: always the same, the largest
     ZL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
-  // Threads to a table row: one step of each while all rows then fit the GPU at once (the
-  // shortest way for a small step: 64 rows of 257 blocks 3.7 us, 4.0 with kDepth steps of a
-  // quarter of the threads), kDepth steps otherwise (1,024 rows of 8,192: 17.6 us, 20 with one).
+  // Threads to a table row: one step of each while all rows then fit the GPU at once, the shortest
+  // way for a small step, kDepth steps otherwise. One and kDepth steps: 64 rows of 256 blocks 3.7 and
+  // 4.3 us, of 1,024 3.8 and 4.1; 1,024 rows of 8,192 17.5 and 14.8. Between them either: 256 rows
+  // of 256 blocks 4.0 and 4.7, of 257 5.2 and 3.9, 512 rows of 1,024 5.3 and 4.4.
   const int wide = vec ? 4 : 1;
   const int64_t most = (many ? 1 : 2) * ctx->num_sms;
   int log_lanes = 3;
