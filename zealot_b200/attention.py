@@ -45,7 +45,8 @@ class CudaAttention:
         got = calls.addresses(self.ctx.device, *triples)
         if type(got) is not tuple:
             t, dtype, n = triples[3 * got:3 * got + 3]
-            raise InvalidArgument(f"need a contiguous {dtype} tensor of {n} {'elements ' if isinstance(n, int) else ''}on cuda:{self.ctx.device}, got "
+            what = f"{n} elements" if isinstance(n, int) else f"shape {n}"
+            raise InvalidArgument(f"need a contiguous {dtype} tensor of {what} on cuda:{self.ctx.device}, got "
                                   f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}")
         return got
 

@@ -6,8 +6,9 @@
  * A tensor is read through the C exchange table that torch.Tensor offers
  * (__dlpack_c_exchange_api__), in one call without a Python object made; what
  * that does not take (a tensor that is only like one, a conjugate), and every
- * tensor of a torch that has no such table, through its methods. This module computes nothing and keeps nothing: what is checked and
- * what is passed stands in attention.py.
+ * tensor of a torch that has no such table, through its methods. This module
+ * computes nothing and keeps nothing: what is checked and what is passed stands
+ * in attention.py.
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>

@@ -20,9 +20,10 @@
 // one more read). 1,024 requests with tables of 8,192 blocks and 65,536 token
 // rows 14.8 us: 49.7 MB, 3.4 TB/s, of which 3.9 us are the launch and every CTA's
 // own sums. The rest is bound by instructions, not by HBM: 63 % of the issue slots
-// are taken, by one CTA of 1,024 threads to an SM, and 12 % of the DRAM's rate. On the way there: 4-byte entries 88 us, 16-byte ones 25, 32-bit
-// divisions 20, all of a stretch's loads before its first store and larger CTAs 17.
-// Stretches shared out by warps instead of CTAs: 15.3; eight loads ahead: 15.5.
+// are taken, by one CTA of 1,024 threads to an SM, and 12 % of the DRAM's rate. On
+// the way there: 4-byte entries 88 us, 16-byte ones 25, 32-bit divisions 20, all of
+// a stretch's loads before its first store and larger CTAs 17. Stretches shared out
+// by warps instead of CTAs: 15.3; eight loads ahead: 15.5.
 #include "zl_internal.h"
 #include "zl_pages.h"
 #include "zl_ptx.cuh"
